@@ -10,7 +10,10 @@ from ._abi import BackendError, BackendUnavailable, BackendUnsupported
 from ._api import (Compactor, CompactSum, Model, Reducer, Runner, RunReport, SimResult, StagedRunner, cell_op,
                    compact, entry, gambler, lorenz, mask_count, oscillator, reduce, reorder, reorder_classes, restore, simulate,
                    until_done)
+from ._sequences import BlockTables, Embedding, EmbeddingGrad, SlotMap, block_tables, embedding, embedding_grad, slot_map
 
-__all__ = ["BackendError", "BackendUnavailable", "BackendUnsupported", "Compactor", "CompactSum", "Model", "Reducer",
-           "Runner", "RunReport", "SimResult", "StagedRunner", "cell_op", "compact", "entry", "gambler", "lorenz",
-           "mask_count", "oscillator", "reduce", "reorder", "reorder_classes", "restore", "simulate", "until_done"]
+__all__ = ["BackendError", "BackendUnavailable", "BackendUnsupported", "BlockTables", "Compactor", "CompactSum",
+           "Embedding", "EmbeddingGrad", "Model", "Reducer", "Runner", "RunReport", "SimResult", "SlotMap",
+           "StagedRunner", "block_tables", "cell_op", "compact", "embedding", "embedding_grad", "entry", "gambler",
+           "lorenz", "mask_count", "oscillator", "reduce", "reorder", "reorder_classes", "restore", "simulate",
+           "slot_map", "until_done"]

@@ -36,6 +36,8 @@ MEM_DEVICE, MEM_PINNED = 0, 1
 
 MODEL_OSCILLATOR, MODEL_OSCILLATOR_SPREAD, MODEL_GAMBLER, MODEL_LORENZ = 0, 1, 2, 3
 MODE_BAND, MODE_PERSIST, MODE_FUSED, MODE_BAND_EAGER = 0, 1, 2, 3
+TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_I32, TYPE_I64 = range(5)
+EMBEDDING_ACCUMULATE = 1
 FLAG_FMA = 1
 FLAG_INDEX_ORDER = 2
 
@@ -174,6 +176,24 @@ class GraphDesc(ctypes.Structure):
     _fields_ = [("struct_size", _u32), ("flags", _u32), ("device", _i32), ("reserved0", _i32)]
 
 
+class EmbeddingDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("flags", _u32), ("device", _i32), ("table_type", _u32),
+                ("values_type", _u32), ("token_type", _u32), ("table", _u64), ("tokens", _u64), ("values", _u64),
+                ("scratch", _u64), ("rows", _i64), ("dim", _i64), ("first", _i64), ("batch", _i64), ("seq", _i64),
+                ("table_stride", _i64), ("token_strides", _i64 * 2), ("value_strides", _i64 * 3), ("scale", _f64),
+                ("stream", _u64), ("scratch_bytes", _i64)]
+
+
+class PagedDesc(ctypes.Structure):
+    _fields_ = [("struct_size", _u32), ("flags", _u32), ("device", _i32), ("length_type", _u32),
+                ("slot_type", _u32), ("reserved0", _u32), ("requests", _i64), ("width", _i64),
+                ("table_stride", _i64), ("block", _i64), ("table", _u64), ("terminated", _u64), ("lengths", _u64),
+                ("held", _u64), ("pool", _u64), ("count", _u64), ("pool_size", _i64), ("used", _u64),
+                ("used_size", _i64), ("blocks", _u64), ("cells", _u64), ("start", _u64), ("fresh", _u64),
+                ("capacity", _i64), ("slots", _u64), ("positions", _u64), ("token_requests", _u64),
+                ("offsets", _u64), ("scratch", _u64), ("stream", _u64), ("scratch_bytes", _i64)]
+
+
 def new(struct_type, **fields):
     """A zero-filled desc with ``struct_size`` set, then ``fields``."""
     s = struct_type()
@@ -309,6 +329,10 @@ SIGNATURES = {
     "eagle_backend_x_b200_reduce_counted": (_i32, [ctypes.POINTER(ReduceDesc), _u64]),
     "eagle_backend_x_b200_reduce_fixed": (_i32, [ctypes.POINTER(ReduceDesc)]),
     "eagle_backend_x_b200_compact_sum": (_i32, [ctypes.POINTER(CompactDesc), _u64, _u64, _u32]),
+    "eagle_backend_x_b200_embedding": (_i32, [ctypes.POINTER(EmbeddingDesc)]),
+    "eagle_backend_x_b200_embedding_grad": (_i32, [ctypes.POINTER(EmbeddingDesc)]),
+    "eagle_backend_x_b200_block_tables": (_i32, [ctypes.POINTER(PagedDesc)]),
+    "eagle_backend_x_b200_slot_map": (_i32, [ctypes.POINTER(PagedDesc)]),
     "eagle_backend_x_b200_engine_create": (_i32, [ctypes.POINTER(EngineDesc), ctypes.POINTER(_P)]),
     "eagle_backend_x_b200_engine_launch": (_i32, [_P, _u64]),
     "eagle_backend_x_b200_engine_report": (_i32, [_P, _u64, ctypes.POINTER(Report)]),

@@ -1,0 +1,956 @@
+// The embedding rows of a batch's tokens, and the gradient of their table.
+//
+//   embedding       values[t, :] = round(scale * table[token[t] - first, :])
+//   embedding_grad  table[v, :] = round(scale * sum over {t : token[t] = first + v} of values[t, :])
+//
+// The lookup is a gather of rows: every thread moves 16-byte pieces of the flattened
+// output, several in flight, so it is bound by HBM (by the launch for a few tokens).
+//
+// The gradient is a scatter-add, done without atomics on the values: the tokens are
+// sorted by id (stable, so equal ids keep token order), the sorted order is cut into
+// chunks of a fixed length, and every run of equal ids inside a chunk is summed in
+// registers by the lanes that own its columns. A run inside one chunk goes straight to
+// its row; one that crosses chunks leaves a 32-bit partial per chunk, joined in
+// chunk order by a second kernel. A row is thus one sum in an order fixed by the sizes
+// alone. Rows without a token are zeroed by CTAs that only store, beside those that sum.
+//
+// The sort is least-significant-digit radix over bits(rows) bits, at most 9 a pass. A
+// tile is 4096 keys: each warp ranks its 256 by match_any, a scan over the warps orders
+// the tile. Up to one tile the whole sort is one CTA's, in shared memory. Past it every
+// pass adds up the tiles' digit counts itself (no look-back, no wait on another CTA): the
+// first counts come from a kernel of their own, each later pass's are gathered by the pass
+// before, which knows where its keys land.
+#include "sequences.cuh"
+
+#include <algorithm>
+
+#define EB_API extern "C" __attribute__((visibility("default")))
+
+namespace eb {
+namespace {
+
+// ------------------------------------------------------------------ lookup
+
+struct LookupArgs {
+    const void* table;
+    const void* tokens;
+    void* values;
+    int64_t rows, first;
+    int64_t tableStride;
+    int64_t tokenBatch, tokenSeq;  // strides of the ids
+    int64_t valueBatch, valueSeq;  // strides of the outputs
+    int64_t n;                     // tokens
+    uint32_t pieces;               // packs per row
+    FastDiv perRow;                // by pieces
+    FastDiv perBatch;              // by seq
+    bool flat;                     // one stride serves batch and seq
+    float scale;
+};
+
+constexpr int kLookupThreads = 256;
+
+/** The row of token ``t``, or -1 where the table has none. */
+template <class Tok>
+__device__ __forceinline__ int64_t rowOfToken(const void* tokens, int64_t at, int64_t first, int64_t rows)
+{
+    const int64_t id = int64_t(__ldg(reinterpret_cast<const Tok*>(tokens) + at));
+    if (id < first)
+        return -1;
+    const uint64_t r = uint64_t(id) - uint64_t(first);  // first >= 0, so the difference is exact
+    return r < uint64_t(rows) ? int64_t(r) : -1;
+}
+
+/** ``Unroll`` packs of N values per thread, a CTA's width apart: neighbouring threads hold
+ *  neighbouring packs of the flattened (token, column) plane, so loads and stores are
+ *  whole lines whatever the row length, and short rows leave no lane idle. */
+template <class In, class Out, class Tok, int N, int Unroll>
+__global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
+{
+    const int64_t base = int64_t(blockIdx.x) * (kLookupThreads * Unroll);
+    const int64_t row0 = base / a.pieces;
+    const uint32_t col0 = uint32_t(base - row0 * a.pieces);
+    const In* table = reinterpret_cast<const In*>(a.table);
+    Out* values = reinterpret_cast<Out*>(a.values);
+    int64_t from[Unroll], to[Unroll];
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u) {
+        const uint32_t k = col0 + uint32_t(u) * kLookupThreads + threadIdx.x;
+        const uint32_t down = a.perRow(k);
+        const uint32_t col = (k - down * a.pieces) * N;
+        const int64_t t = row0 + down;
+        from[u] = -2;
+        to[u] = 0;
+        if (t < a.n) {
+            const uint32_t b = a.flat ? 0u : a.perBatch(uint32_t(t));
+            const int64_t s = t - int64_t(b) * a.perBatch.d;
+            const int64_t in = a.flat ? t : s;
+            const int64_t r = rowOfToken<Tok>(a.tokens, int64_t(b) * a.tokenBatch + in * a.tokenSeq, a.first, a.rows);
+            from[u] = r < 0 ? -1 : r * a.tableStride + col;
+            to[u] = int64_t(b) * a.valueBatch + in * a.valueSeq + col;
+        }
+    }
+    Pack<In, N> got[Unroll];
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u)
+        if (from[u] >= 0)
+            got[u] = *reinterpret_cast<const Pack<In, N>*>(table + from[u]);
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u) {
+        if (from[u] == -2)
+            continue;
+        Pack<Out, N> out;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            out.e[e] = fromFloat<Out>(from[u] >= 0 ? toFloat(got[u].e[e]) * a.scale : 0.0f);
+        *reinterpret_cast<Pack<Out, N>*>(values + to[u]) = out;
+    }
+}
+
+// ------------------------------------------------------------------ gradient: sort
+
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortItems = 8;
+constexpr uint32_t kSortTile = uint32_t(kSortThreads) * kSortItems;  // 4096 keys
+constexpr uint32_t kMaxBins = 512;                                  // 9 bits a pass, one bin per thread
+constexpr uint32_t kNoKey = 0xffffffffu;  // behind the last key: every digit of it is the highest
+
+struct GradArgs {
+    const void* tokens;
+    const void* values;
+    void* table;
+    int64_t rows, first;
+    int64_t tableStride;
+    int64_t tokenBatch, tokenSeq;
+    int64_t valueBatch, valueSeq, valueDim;
+    FastDiv perBatch;  // by seq
+    bool flatTokens, flatValues;
+    bool accumulate;
+    float scale;
+    uint32_t n;
+    uint32_t dim;
+    // sort
+    uint32_t tiles, bins, digitBits;
+    uint32_t* present;  // a bit per row that has a token
+    uint32_t* hist;     // this pass's digit counts, [tile][bin]
+    uint32_t* nextHist; // the next pass's, gathered by this one
+    const uint32_t* keyIn;
+    const uint32_t* posIn;
+    uint32_t* keyOut;
+    uint32_t* posOut;
+    uint32_t shift;
+    // sums
+    const uint32_t* keys;   // sorted; ``rows`` for a token without a row
+    const uint32_t* order;  // the sorted keys' token positions
+    uint32_t chunk, chunks;
+    uint32_t group;      // lanes that share a row's pieces
+    uint32_t slices;     // groups a row takes
+    uint32_t pieces;     // packs (or columns) per row
+    uint32_t sumBlocks;  // CTAs that sum; the others zero
+    uint32_t* listCount; // chunks whose last run goes on into the next
+    uint32_t* list;
+    float* head;         // [chunk][width]: the part of a run that began in an earlier chunk
+    float* tail;         // [chunk][width]: the part of a run that goes on
+    uint32_t width;      // dim rounded up to 4
+    // zeroing
+    uint32_t zeroRows;   // rows a zeroing CTA takes at a time
+    bool zeroWide;       // rows are whole aligned 16-byte words
+};
+
+template <class Tok>
+__device__ __forceinline__ uint32_t keyOfToken(const GradArgs& a, uint32_t i)
+{
+    int64_t at;
+    if (a.flatTokens) {
+        at = int64_t(i) * a.tokenSeq;
+    } else {
+        const uint32_t b = a.perBatch(i);
+        at = int64_t(b) * a.tokenBatch + int64_t(i - b * a.perBatch.d) * a.tokenSeq;
+    }
+    const int64_t r = rowOfToken<Tok>(a.tokens, at, a.first, a.rows);
+    return r < 0 ? uint32_t(a.rows) : uint32_t(r);
+}
+
+struct SortShared {
+    uint32_t count[kSortWarps * kMaxBins];  // [warp][bin]
+    uint32_t base[kMaxBins];
+    uint32_t scan[33];
+};
+
+/** Each key's place among the tile's keys of its digit, in item order (a warp's items are
+ *  its 256 neighbours, item k of lane l the 32 k + l-th); ``total`` is bin threadIdx.x's
+ *  count. Leaves the per-warp counts scanned over the warps. */
+__device__ __forceinline__ void rankTile(const uint32_t (&digit)[kSortItems], uint32_t (&rank)[kSortItems],
+    uint32_t& total, uint32_t bins, SortShared& s)
+{
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    for (uint32_t i = threadIdx.x; i < kSortWarps * bins; i += kSortThreads)
+        s.count[i] = 0;
+    __syncthreads();
+    uint32_t* mine = s.count + warp * bins;
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t peers = __match_any_sync(kFull, digit[k]);
+        const uint32_t before = mine[digit[k]];
+        __syncwarp();
+        if (lane == uint32_t(__ffs(peers)) - 1u)
+            mine[digit[k]] = before + __popc(peers);
+        __syncwarp();
+        rank[k] = before + __popc(peers & ((1u << lane) - 1u));
+    }
+    __syncthreads();
+    total = 0;
+    if (threadIdx.x < bins) {
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+            const uint32_t c = s.count[w * bins + threadIdx.x];
+            s.count[w * bins + threadIdx.x] = total;
+            total += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k)
+        rank[k] += mine[digit[k]];
+}
+
+/** Zero the rows [row0, row1) whose bit in ``present`` (bit r - bit0) is clear, a warp per row. */
+template <class Out>
+__device__ __forceinline__ void zeroAbsent(const GradArgs& a, const uint32_t* present, uint32_t bit0, uint32_t row0,
+    uint32_t row1)
+{
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (uint32_t r = row0 + warp; r < row1; r += warps) {
+        if ((present[(r - bit0) >> 5] >> ((r - bit0) & 31u)) & 1u)
+            continue;
+        Out* row = reinterpret_cast<Out*>(a.table) + int64_t(r) * a.tableStride;
+        if (a.zeroWide) {
+            uint4* w = reinterpret_cast<uint4*>(row);
+            const uint32_t words = a.dim * uint32_t(sizeof(Out)) / 16u;
+            for (uint32_t i = lane; i < words; i += 32u)
+                w[i] = make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            for (uint32_t i = lane; i < a.dim; i += 32u)
+                row[i] = fromFloat<Out>(0.0f);
+        }
+    }
+}
+
+/** Up to one tile of tokens: CTA 0 sorts them in shared memory; the others zero the rows
+ *  without a token, each finding those of its rows that have one by reading all the ids. */
+template <class Out, class Tok>
+__global__ __launch_bounds__(kSortThreads) void sortTileKernel(GradArgs a)
+{
+    extern __shared__ __align__(16) unsigned char raw[];
+    if (blockIdx.x != 0) {
+        uint32_t* present = reinterpret_cast<uint32_t*>(raw);
+        const uint32_t words = a.zeroRows / 32u;
+        for (int64_t row0 = int64_t(blockIdx.x - 1) * a.zeroRows; row0 < a.rows;
+             row0 += int64_t(gridDim.x - 1) * a.zeroRows) {
+            const uint32_t row1 = uint32_t(min(row0 + int64_t(a.zeroRows), a.rows));
+            for (uint32_t i = threadIdx.x; i < words; i += kSortThreads)
+                present[i] = 0;
+            __syncthreads();
+            for (uint32_t i = threadIdx.x; i < a.n; i += kSortThreads) {
+                const uint32_t key = keyOfToken<Tok>(a, i);
+                if (key >= uint32_t(row0) && key < row1)
+                    atomicOr(present + ((key - uint32_t(row0)) >> 5), 1u << ((key - uint32_t(row0)) & 31u));
+            }
+            __syncthreads();
+            zeroAbsent<Out>(a, present, uint32_t(row0), uint32_t(row0), row1);
+            __syncthreads();
+        }
+        return;
+    }
+    SortShared& s = *reinterpret_cast<SortShared*>(raw);
+    uint32_t* keyAt = reinterpret_cast<uint32_t*>(raw + sizeof(SortShared));
+    uint32_t* posAt = keyAt + kSortTile;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t item0 = warp * (32u * kSortItems) + lane;
+    uint32_t key[kSortItems], pos[kSortItems], digit[kSortItems], rank[kSortItems];
+    if (threadIdx.x == 0)
+        *a.listCount = 0;
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        pos[k] = item0 + 32u * k;
+        key[k] = pos[k] < a.n ? keyOfToken<Tok>(a, pos[k]) : kNoKey;
+    }
+    const uint32_t top = a.shift;  // the bits that tell the rows apart
+    for (uint32_t shift = 0; shift < top; shift += a.digitBits) {
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k)
+            digit[k] = (key[k] >> shift) & (a.bins - 1u);
+        uint32_t total = 0, all = 0;
+        rankTile(digit, rank, total, a.bins, s);
+        const uint32_t base = blockExclusiveSum(total, all, s.scan);
+        if (threadIdx.x < a.bins)
+            s.base[threadIdx.x] = base;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            const uint32_t to = s.base[digit[k]] + rank[k];
+            keyAt[to] = key[k];
+            posAt[to] = pos[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortItems; ++k) {
+            key[k] = keyAt[item0 + 32u * k];
+            pos[k] = posAt[item0 + 32u * k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t i = item0 + 32u * k;
+        if (i < a.n) {
+            a.keyOut[i] = key[k];
+            a.posOut[i] = pos[k];
+        }
+    }
+}
+
+/** A tile's digit counts of the first pass, and the rows that have a token. */
+template <class Tok>
+__global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
+{
+    __shared__ uint32_t count[kMaxBins];
+    if (threadIdx.x < a.bins)
+        count[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t i = blockIdx.x * kSortTile + uint32_t(k) * kSortThreads + threadIdx.x;
+        if (i < a.n) {
+            const uint32_t key = keyOfToken<Tok>(a, i);
+            atomicAdd(count + (key & (a.bins - 1u)), 1u);
+            if (a.present != nullptr && key < uint32_t(a.rows)) {
+                const uint32_t bit = 1u << (key & 31u);
+                if ((*const_cast<volatile uint32_t*>(a.present + (key >> 5)) & bit) == 0)  // a frequent id: once
+                    atomicOr(a.present + (key >> 5), bit);
+            }
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < a.bins)
+        a.hist[size_t(blockIdx.x) * a.bins + threadIdx.x] = count[threadIdx.x];
+}
+
+/** One pass over one tile: a bin's first place is the keys of lower bins plus those of its
+ *  own in earlier tiles, added up from every tile's counts by the bin's thread. */
+template <bool First, class Tok>
+__global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
+{
+    extern __shared__ __align__(16) unsigned char raw[];
+    SortShared& s = *reinterpret_cast<SortShared*>(raw);
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t item0 = blockIdx.x * kSortTile + warp * (32u * kSortItems) + lane;
+    uint32_t key[kSortItems], pos[kSortItems], digit[kSortItems], rank[kSortItems];
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        const uint32_t i = item0 + 32u * k;
+        key[k] = kNoKey;
+        pos[k] = i;
+        if (i < a.n) {
+            key[k] = First ? keyOfToken<Tok>(a, i) : a.keyIn[i];
+            if (!First)
+                pos[k] = a.posIn[i];
+        }
+        digit[k] = (key[k] >> a.shift) & (a.bins - 1u);
+    }
+    uint32_t before = 0, total = 0;
+    if (threadIdx.x < a.bins) {
+        const uint32_t* column = a.hist + threadIdx.x;
+#pragma unroll 8
+        for (uint32_t t = 0; t < a.tiles; ++t) {
+            const uint32_t c = __ldcg(column + size_t(t) * a.bins);
+            total += c;
+            before += t < blockIdx.x ? c : 0u;
+        }
+    }
+    uint32_t all = 0, own = 0;
+    const uint32_t base = blockExclusiveSum(total, all, s.scan) + before;
+    rankTile(digit, rank, own, a.bins, s);
+    if (threadIdx.x < a.bins)
+        s.base[threadIdx.x] = base;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        if (item0 + 32u * k < a.n) {
+            const uint32_t to = s.base[digit[k]] + rank[k];
+            a.keyOut[to] = key[k];
+            a.posOut[to] = pos[k];
+            if (a.nextHist != nullptr)
+                atomicAdd(a.nextHist + size_t(to / kSortTile) * a.bins
+                        + ((key[k] >> (a.shift + a.digitBits)) & (a.bins - 1u)),
+                    1u);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ gradient: sums
+
+constexpr int kSumThreads = 256;
+constexpr uint32_t kRowsInFlight = 8;
+
+/** Columns of a piece: N neighbours (Wide: one 16-byte load of the values), or N columns
+ *  ``group`` apart, element by element, for rows of odd length, alignment or stride. */
+template <bool Wide, int N>
+__device__ __forceinline__ uint32_t columnOf(const GradArgs& a, uint32_t slice, uint32_t lane, int e)
+{
+    return Wide ? (slice * a.group + lane) * N + e : (slice * N + e) * a.group + lane;
+}
+
+template <class In, class Out, bool Wide, int N>
+__device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32_t slice, uint32_t lane,
+    const float (&acc)[N])
+{
+    Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
+    if constexpr (Wide) {
+        Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + columnOf<true, N>(a, slice, lane, 0));
+        Pack<Out, N> p;
+        if (a.accumulate)
+            p = *at;
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+            p.e[e] = fromFloat<Out>(a.accumulate ? toFloat(p.e[e]) + a.scale * acc[e] : a.scale * acc[e]);
+        *at = p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t col = columnOf<false, N>(a, slice, lane, e);
+            if (col < a.dim)
+                out[col] = fromFloat<Out>(a.accumulate ? toFloat(out[col]) + a.scale * acc[e] : a.scale * acc[e]);
+        }
+    }
+}
+
+template <bool Wide, int N>
+__device__ __forceinline__ void storePartial(const GradArgs& a, float* to, uint32_t chunk, uint32_t slice,
+    uint32_t lane, const float (&acc)[N])
+{
+    float* row = to + size_t(chunk) * a.width;
+    if constexpr (Wide) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4)
+            *reinterpret_cast<float4*>(row + columnOf<true, N>(a, slice, lane, e)) =
+                make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const uint32_t col = columnOf<false, N>(a, slice, lane, e);
+            if (col < a.dim)
+                row[col] = acc[e];
+        }
+    }
+}
+
+/** The runs of one chunk of the sorted order, by the lanes owning one slice of the columns;
+ *  the CTAs past ``sumBlocks`` zero rows. */
+template <class In, class Out, bool Wide, int N>
+__global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
+{
+    if (blockIdx.x >= a.sumBlocks) {
+        for (int64_t row0 = int64_t(blockIdx.x - a.sumBlocks) * a.zeroRows; row0 < a.rows;
+             row0 += int64_t(gridDim.x - a.sumBlocks) * a.zeroRows)
+            zeroAbsent<Out>(a, a.present, 0u, uint32_t(row0), uint32_t(min(row0 + int64_t(a.zeroRows), a.rows)));
+        return;
+    }
+    const uint64_t id = uint64_t(blockIdx.x) * kSumThreads + threadIdx.x;
+    const uint32_t lane = uint32_t(id) & (a.group - 1u);
+    const uint64_t which = id / a.group;  // a power of two
+    const uint32_t chunk = uint32_t(which / a.slices), slice = uint32_t(which % a.slices);
+    if (chunk >= a.chunks || (Wide && slice * a.group + lane >= a.pieces))
+        return;
+    const uint32_t begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
+    const uint32_t none = uint32_t(a.rows);
+    const In* values = reinterpret_cast<const In*>(a.values);
+    uint32_t current = __ldg(a.keys + begin);
+    if (current == none)
+        return;
+    bool fromBefore = begin > 0 && __ldg(a.keys + begin - 1) == current;
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        acc[e] = 0.0f;
+    for (uint32_t i0 = begin; i0 < end && current != none; i0 += kRowsInFlight) {
+        uint32_t key[kRowsInFlight];
+        Pack<In, N> got[kRowsInFlight];
+#pragma unroll
+        for (uint32_t u = 0; u < kRowsInFlight; ++u)
+            key[u] = i0 + u < end ? __ldg(a.keys + i0 + u) : kNoKey;
+#pragma unroll
+        for (uint32_t u = 0; u < kRowsInFlight; ++u) {
+            if (key[u] >= none)
+                continue;
+            const uint32_t t = __ldg(a.order + i0 + u);
+            int64_t at;
+            if (a.flatValues) {
+                at = int64_t(t) * a.valueSeq;
+            } else {
+                const uint32_t b = a.perBatch(t);
+                at = int64_t(b) * a.valueBatch + int64_t(t - b * a.perBatch.d) * a.valueSeq;
+            }
+            if constexpr (Wide) {
+                got[u] = *reinterpret_cast<const Pack<In, N>*>(values + at + columnOf<true, N>(a, slice, lane, 0));
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    const uint32_t col = columnOf<false, N>(a, slice, lane, e);
+                    if (col < a.dim)
+                        got[u].e[e] = values[at + int64_t(col) * a.valueDim];
+                    else
+                        got[u].e[e] = fromFloat<In>(0.0f);
+                }
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kRowsInFlight; ++u) {
+            if (key[u] == kNoKey)
+                break;
+            if (key[u] != current) {
+                if (fromBefore)
+                    storePartial<Wide, N>(a, a.head, chunk, slice, lane, acc);
+                else
+                    storeRow<In, Out, Wide, N>(a, current, slice, lane, acc);
+                fromBefore = false;
+                current = key[u];
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    acc[e] = 0.0f;
+                if (current == none)
+                    break;
+            }
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                acc[e] += toFloat(got[u].e[e]);
+        }
+    }
+    if (current == none)
+        return;
+    const bool goesOn = end < a.n && __ldg(a.keys + end) == current;
+    if (fromBefore) {
+        storePartial<Wide, N>(a, a.head, chunk, slice, lane, acc);
+    } else if (goesOn) {
+        storePartial<Wide, N>(a, a.tail, chunk, slice, lane, acc);
+        if (slice == 0 && lane == 0)
+            a.list[atomicAdd(a.listCount, 1u)] = chunk;  // any order: every run is joined on its own
+    } else {
+        storeRow<In, Out, Wide, N>(a, current, slice, lane, acc);
+    }
+}
+
+constexpr int kJoinThreads = 256;
+constexpr int kJoinWarps = kJoinThreads / 32;
+constexpr uint32_t kJoinColumns = 128;  // four per lane
+
+/** The rows whose runs cross chunks: eight warps each add a contiguous eighth of the run's
+ *  partials in chunk order, then the eight sums are added in order. */
+template <class Out>
+__global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
+{
+    __shared__ float4 part[kJoinWarps][32];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t blocks = (a.dim + kJoinColumns - 1) / kJoinColumns;
+    const uint64_t items = uint64_t(*a.listCount) * blocks;
+    for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const uint32_t chunk = a.list[item / blocks];
+        const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
+        const uint32_t key = __ldg(a.keys + (chunk + 1u) * a.chunk);
+        uint32_t m = 1;  // chunks after this one that the run reaches
+        for (;;) {
+            const uint32_t c = chunk + 1u + m + lane;
+            const bool in = c < a.chunks && __ldg(a.keys + c * a.chunk) == key;
+            const uint32_t reached = __ballot_sync(kFull, in);
+            m += __popc(reached);  // the keys are sorted: the set lanes are the first ones
+            if (reached != kFull)
+                break;
+        }
+        const uint32_t parts = m + 1u, each = (parts + kJoinWarps - 1) / kJoinWarps;
+        const uint32_t p0 = warp * each, p1 = min(p0 + each, parts);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (col < a.width) {
+#pragma unroll 8
+            for (uint32_t p = p0; p < p1; ++p) {
+                const float* row = (p == 0 ? a.tail : a.head) + size_t(chunk + p) * a.width;
+                const float4 v = *reinterpret_cast<const float4*>(row + col);
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            }
+        }
+        part[warp][lane] = sum;
+        __syncthreads();
+        if (warp == 0) {
+#pragma unroll
+            for (int w = 1; w < kJoinWarps; ++w) {
+                const float4 v = part[w][lane];
+                sum.x += v.x;
+                sum.y += v.y;
+                sum.z += v.z;
+                sum.w += v.w;
+            }
+            Out* out = reinterpret_cast<Out*>(a.table) + int64_t(key) * a.tableStride;
+            const float got[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (col + e < a.dim)
+                    out[col + e] = fromFloat<Out>(a.accumulate ? toFloat(out[col + e]) + a.scale * got[e]
+                                                               : a.scale * got[e]);
+        }
+        __syncthreads();
+    }
+}
+
+/** No tokens: every row is zero. */
+template <class Out>
+__global__ __launch_bounds__(kSumThreads) void zeroRowsKernel(GradArgs a)
+{
+    const uint32_t nothing[1] = {0};
+    for (int64_t r = int64_t(blockIdx.x); r < a.rows; r += gridDim.x)
+        if (threadIdx.x < 32)
+            zeroAbsent<Out>(a, nothing, uint32_t(r), uint32_t(r), uint32_t(r) + 1u);
+}
+
+// ------------------------------------------------------------------ host side
+
+uint64_t roundUp(uint64_t v, uint64_t to) { return (v + to - 1) / to * to; }
+
+/** What both entries refuse. */
+void checkEmbedding(const eagle_b200_embedding_desc& d, const char* who)
+{
+    const std::string w(who);
+    (void)elementBytes(d.table_type, who);
+    (void)elementBytes(d.values_type, who);
+    (void)indexBytes(d.token_type, who);
+    if (d.rows < 0 || d.rows > 0x7ffffffell)
+        invalid(w + ": rows must lie in [0, 2^31 - 2]");
+    if (d.dim < 0 || d.dim > (1ll << 24))
+        invalid(w + ": dim must lie in [0, 2^24]");
+    if (d.first < 0)
+        invalid(w + ": first must not be negative");
+    if (d.batch < 0 || d.seq < 0 || d.batch > 0x7fffffffll || d.seq > 0x7fffffffll || d.batch * d.seq > 0x7fffffffll)
+        invalid(w + ": batch * seq must lie in [0, 2^31 - 1]");
+    if (d.rows > 1 && d.table_stride < d.dim)
+        invalid(w + ": the table's rows overlap (table_stride below dim)");
+}
+
+/** One stride serves both token axes. */
+bool isFlat(int64_t batch, int64_t seq, int64_t outer, int64_t inner) { return batch <= 1 || outer == seq * inner; }
+
+template <class F>
+void withElement(uint32_t type, F&& f)
+{
+    if (type == EAGLE_B200_TYPE_F32)
+        f(float{});
+    else if (type == EAGLE_B200_TYPE_BF16)
+        f(__nv_bfloat16{});
+    else
+        f(__half{});
+}
+
+template <class F>
+void withIndex(uint32_t type, F&& f)
+{
+    if (type == EAGLE_B200_TYPE_I32)
+        f(int32_t{});
+    else
+        f(int64_t{});
+}
+
+template <class In, class Out, class Tok, int N>
+void launchLookup(LookupArgs a, int64_t dim, cudaStream_t s, const char* who)
+{
+    a.pieces = uint32_t(dim / N);
+    a.perRow = FastDiv(a.pieces);
+    const int64_t packs = a.n * int64_t(a.pieces);
+    // four packs a thread keep the memory busy; a plane too small to give every SM a few CTAs
+    // of those takes one each, so that more SMs share it
+    constexpr int kMany = N == 1 ? 8 : 4;
+    if (packs >= int64_t(smCount()) * 2 * kLookupThreads * kMany) {
+        const int64_t per = kLookupThreads * kMany;
+        lookupKernel<In, Out, Tok, N, kMany><<<gridOf((packs + per - 1) / per, who), kLookupThreads, 0, s>>>(a);
+    } else {
+        lookupKernel<In, Out, Tok, N, 1>
+            <<<gridOf((packs + kLookupThreads - 1) / kLookupThreads, who), kLookupThreads, 0, s>>>(a);
+    }
+    launchCheck(who);
+}
+
+void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
+{
+    const int inBytes = elementBytes(d.table_type, who), outBytes = elementBytes(d.values_type, who);
+    requireAddress(d.tokens, uint64_t(indexBytes(d.token_type, who)), who, "tokens");
+    requireAddress(d.values, uint64_t(outBytes), who, "values");
+    if (d.rows > 0)
+        requireAddress(d.table, uint64_t(inBytes), who, "table");
+    if (d.dim > 1 && d.value_strides[2] != 1)
+        invalid(std::string(who) + ": a vector's values must be contiguous");
+    LookupArgs a{};
+    a.table = reinterpret_cast<const void*>(d.table);
+    a.tokens = reinterpret_cast<const void*>(d.tokens);
+    a.values = reinterpret_cast<void*>(d.values);
+    a.rows = d.rows;
+    a.first = d.first;
+    a.tableStride = d.table_stride;
+    a.tokenBatch = d.token_strides[0];
+    a.tokenSeq = d.token_strides[1];
+    a.valueBatch = d.value_strides[0];
+    a.valueSeq = d.value_strides[1];
+    a.n = d.batch * d.seq;
+    a.perBatch = FastDiv(uint32_t(d.seq));
+    a.flat = isFlat(d.batch, d.seq, a.tokenBatch, a.tokenSeq) && isFlat(d.batch, d.seq, a.valueBatch, a.valueSeq);
+    a.scale = float(d.scale);
+    const cudaStream_t s = seamStream(d.stream);
+    withElement(d.table_type, [&](auto in) {
+        withElement(d.values_type, [&](auto out) {
+            withIndex(d.token_type, [&](auto tok) {
+                using In = decltype(in);
+                using Out = decltype(out);
+                using Tok = decltype(tok);
+                // a pack is 16 bytes of the narrower type; every row has to start on its words
+                constexpr int N = 16 / int(sizeof(In) < sizeof(Out) ? sizeof(In) : sizeof(Out));
+                const bool wide = d.dim % N == 0 && d.table % 16 == 0 && d.values % 16 == 0
+                    && d.table_stride * inBytes % 16 == 0 && d.value_strides[0] * outBytes % 16 == 0
+                    && d.value_strides[1] * outBytes % 16 == 0;
+                if (wide)
+                    launchLookup<In, Out, Tok, N>(a, d.dim, s, who);
+                else
+                    launchLookup<In, Out, Tok, 1>(a, d.dim, s, who);
+            });
+        });
+    });
+}
+
+/** How the gradient's sort, sums and scratch are laid out. */
+struct GradPlan {
+    uint32_t n = 0, bits = 0, passes = 0, digitBits = 0, bins = 0, tiles = 0;
+    bool wide = false;
+    uint32_t pieces = 0, group = 0, slices = 0, chunk = 0, chunks = 0, width = 0;
+    uint64_t present = 0, listCount = 0, hist = 0, zeroed = 0;  // offsets; [0, zeroed) is cleared
+    uint64_t firstHist = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, head = 0, tail = 0, bytes = 0;
+};
+
+GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
+{
+    GradPlan p;
+    p.n = uint32_t(d.batch * d.seq);
+    const int inBytes = elementBytes(d.values_type, who), outBytes = elementBytes(d.table_type, who);
+    // keys are 0 .. rows (rows: a token without a row)
+    while (p.bits < 32 && (uint64_t(d.rows) >> p.bits) != 0)
+        ++p.bits;
+    p.passes = (p.bits + 8) / 9;
+    p.digitBits = p.passes == 0 ? 0 : (p.bits + p.passes - 1) / p.passes;
+    p.bins = 1u << p.digitBits;
+    p.tiles = (p.n + kSortTile - 1) / kSortTile;
+    // 16-byte words of the values, if every vector and every row of the table starts on them
+    const int pack = 16 / inBytes;
+    const int64_t outWord = std::min(16, pack * outBytes);
+    p.wide = d.dim % pack == 0 && d.value_strides[2] == 1 && d.values % 16 == 0 && d.table % uint64_t(outWord) == 0
+        && d.value_strides[0] * inBytes % 16 == 0 && d.value_strides[1] * inBytes % 16 == 0
+        && d.table_stride * outBytes % outWord == 0;
+    p.pieces = p.wide ? uint32_t(d.dim / pack) : uint32_t((d.dim + 3) / 4);
+    p.group = 1;
+    while (p.group < 32 && p.group < p.pieces)
+        p.group *= 2;
+    p.slices = (p.pieces + p.group - 1) / p.group;
+    // the longest chunk that still leaves enough warps of 256 columns to hide the row loads: a
+    // longer one leaves fewer partials of runs that cross chunks. Of the sizes alone, not of
+    // types or alignment: it fixes the order of the sums, and the scratch the query asks for
+    p.chunk = 8;
+    while (p.chunk < 64 && uint64_t(p.n) * ((uint64_t(d.dim) + 255) / 256) / (p.chunk * 2) >= 4096)
+        p.chunk *= 2;
+    p.chunks = (p.n + p.chunk - 1) / p.chunk;
+    p.width = uint32_t(roundUp(uint64_t(d.dim), 4));
+    uint64_t at = 0;
+    auto take = [&](uint64_t bytes) {
+        const uint64_t was = at;
+        at += roundUp(bytes, 256);
+        return was;
+    };
+    p.present = take((uint64_t(d.rows) + 31) / 32 * 4);
+    p.listCount = take(4);
+    const uint64_t histBytes = uint64_t(p.tiles) * p.bins * 4;
+    p.hist = take(p.tiles > 1 && p.passes > 1 ? histBytes * (p.passes - 1) : 0);
+    p.zeroed = at;
+    p.firstHist = take(p.tiles > 1 ? histBytes : 0);
+    for (int k = 0; k < 2; ++k) {
+        p.key[k] = take(uint64_t(p.n) * 4);
+        p.pos[k] = take(uint64_t(p.n) * 4);
+    }
+    p.list = take(uint64_t(p.chunks) * 4);
+    p.head = take(uint64_t(p.chunks) * p.width * 4);
+    p.tail = take(uint64_t(p.chunks) * p.width * 4);
+    p.bytes = at;
+    return p;
+}
+
+template <class In, class Out, bool Wide>
+void launchSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const char* who)
+{
+    constexpr int N = Wide ? 16 / int(sizeof(In)) : 4;
+    sumKernel<In, Out, Wide, N><<<blocks, kSumThreads, 0, s>>>(a);
+    launchCheck(who);
+}
+
+void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
+{
+    const int inBytes = elementBytes(d.values_type, who), outBytes = elementBytes(d.table_type, who);
+    requireAddress(d.table, uint64_t(outBytes), who, "table");
+    const cudaStream_t s = seamStream(d.stream);
+    const bool accumulate = (d.flags & EAGLE_B200_EMBEDDING_ACCUMULATE) != 0;
+    GradArgs a{};
+    a.table = reinterpret_cast<void*>(d.table);
+    a.rows = d.rows;
+    a.first = d.first;
+    a.tableStride = d.table_stride;
+    a.dim = uint32_t(d.dim);
+    a.zeroWide = d.dim * outBytes % 16 == 0 && d.table % 16 == 0 && d.table_stride * outBytes % 16 == 0;
+    const int64_t sms = smCount();
+    if (p.n == 0) {
+        if (!accumulate) {
+            withElement(d.table_type, [&](auto out) {
+                zeroRowsKernel<decltype(out)><<<gridOf(std::min<int64_t>(d.rows, sms * 32), who), 32, 0, s>>>(a);
+                launchCheck(who);
+            });
+        }
+        return;
+    }
+    requireAddress(d.tokens, uint64_t(indexBytes(d.token_type, who)), who, "tokens");
+    requireAddress(d.values, uint64_t(inBytes), who, "values");
+    requireAddress(d.scratch, 256, who, "scratch");
+    char* scratch = reinterpret_cast<char*>(d.scratch);
+    auto words = [&](uint64_t off) { return reinterpret_cast<uint32_t*>(scratch + off); };
+    a.tokens = reinterpret_cast<const void*>(d.tokens);
+    a.values = reinterpret_cast<const void*>(d.values);
+    a.tokenBatch = d.token_strides[0];
+    a.tokenSeq = d.token_strides[1];
+    a.valueBatch = d.value_strides[0];
+    a.valueSeq = d.value_strides[1];
+    a.valueDim = d.value_strides[2];
+    a.perBatch = FastDiv(uint32_t(d.seq));
+    a.flatTokens = isFlat(d.batch, d.seq, a.tokenBatch, a.tokenSeq);
+    a.flatValues = isFlat(d.batch, d.seq, a.valueBatch, a.valueSeq);
+    a.accumulate = accumulate;
+    a.scale = float(d.scale);
+    a.n = p.n;
+    a.tiles = p.tiles;
+    a.bins = p.bins;
+    a.digitBits = p.digitBits;
+    a.chunk = p.chunk;
+    a.chunks = p.chunks;
+    a.group = p.group;
+    a.slices = p.slices;
+    a.pieces = p.pieces;
+    a.listCount = words(p.listCount);
+    a.list = words(p.list);
+    a.head = reinterpret_cast<float*>(scratch + p.head);
+    a.tail = reinterpret_cast<float*>(scratch + p.tail);
+    a.width = p.width;
+    const bool oneTile = p.tiles == 1;
+    a.present = accumulate || oneTile ? nullptr : words(p.present);
+    if (oneTile) {
+        a.keyOut = words(p.key[0]);
+        a.posOut = words(p.pos[0]);
+        a.shift = p.bits;
+        // each zeroing CTA takes an equal share of the rows, at most what 8 KB of bits hold
+        a.zeroRows = uint32_t(std::min<int64_t>(65536, int64_t(roundUp(uint64_t((d.rows + 2 * sms - 1) / (2 * sms)), 32))));
+        const int64_t zeroing = accumulate ? 0 : std::min<int64_t>(2 * sms, (d.rows + a.zeroRows - 1) / a.zeroRows);
+        const size_t shared = sizeof(SortShared) + size_t(kSortTile) * 8;
+        withElement(d.table_type, [&](auto out) {
+            withIndex(d.token_type, [&](auto tok) {
+                auto kernel = sortTileKernel<decltype(out), decltype(tok)>;
+                cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
+                kernel<<<gridOf(1 + zeroing, who), kSortThreads, shared, s>>>(a);
+                launchCheck(who);
+            });
+        });
+        a.keys = a.keyOut;
+        a.order = a.posOut;
+    } else {
+        cudaCheck(cudaMemsetAsync(scratch, 0, p.zeroed, s), who);
+        a.hist = words(p.firstHist);
+        withIndex(d.token_type, [&](auto tok) {
+            using Tok = decltype(tok);
+            histogramKernel<Tok><<<p.tiles, kSortThreads, 0, s>>>(a);
+            launchCheck(who);
+            for (uint32_t k = 0; k < p.passes; ++k) {
+                GradArgs b = a;
+                b.shift = k * p.digitBits;
+                b.hist = k == 0 ? words(p.firstHist) : words(p.hist) + size_t(k - 1) * p.tiles * p.bins;
+                b.nextHist = k + 1 < p.passes ? words(p.hist) + size_t(k) * p.tiles * p.bins : nullptr;
+                b.keyIn = words(p.key[(k + 1) & 1]);
+                b.posIn = words(p.pos[(k + 1) & 1]);
+                b.keyOut = words(p.key[k & 1]);
+                b.posOut = words(p.pos[k & 1]);
+                if (k == 0)
+                    passKernel<true, Tok><<<p.tiles, kSortThreads, sizeof(SortShared), s>>>(b);
+                else
+                    passKernel<false, Tok><<<p.tiles, kSortThreads, sizeof(SortShared), s>>>(b);
+                launchCheck(who);
+            }
+        });
+        a.keys = words(p.key[(p.passes + 1) & 1]);
+        a.order = words(p.pos[(p.passes + 1) & 1]);
+        a.zeroRows = 32;
+    }
+    const uint64_t lanes = uint64_t(p.chunks) * p.slices * p.group;
+    a.sumBlocks = gridOf(int64_t((lanes + kSumThreads - 1) / kSumThreads), who);
+    const int64_t zeroing = a.present == nullptr ? 0 : std::min<int64_t>(sms * 8, (d.rows + 31) / 32);
+    const unsigned blocks = gridOf(int64_t(a.sumBlocks) + zeroing, who);
+    withElement(d.values_type, [&](auto in) {
+        withElement(d.table_type, [&](auto out) {
+            if (p.wide)
+                launchSum<decltype(in), decltype(out), true>(a, blocks, s, who);
+            else
+                launchSum<decltype(in), decltype(out), false>(a, blocks, s, who);
+        });
+    });
+    if (p.chunks > 1) {
+        const int64_t items = int64_t(p.chunks - 1) * ((d.dim + kJoinColumns - 1) / kJoinColumns);
+        withElement(d.table_type, [&](auto out) {
+            joinKernel<decltype(out)><<<gridOf(std::min<int64_t>(items, sms * 4), who), kJoinThreads, 0, s>>>(a);
+            launchCheck(who);
+        });
+    }
+}
+
+}  // namespace
+}  // namespace eb
+
+using namespace eb;
+
+EB_API eagle_backend_status eagle_backend_x_b200_embedding(const eagle_b200_embedding_desc* desc)
+{
+    return guarded([&] {
+        const char* who = "eagle_backend_x_b200_embedding";
+        const eagle_b200_embedding_desc d = readDesc(desc, 0u, who);
+        checkEmbedding(d, who);
+        if (d.batch * d.seq == 0 || d.dim == 0)
+            return;
+        requireDevice();
+        DeviceScope scope(resolveDevice(d.device, d.values));
+        enqueueLookup(d, who);
+    });
+}
+
+EB_API eagle_backend_status eagle_backend_x_b200_embedding_grad(eagle_b200_embedding_desc* desc)
+{
+    return guarded([&] {
+        const char* who = "eagle_backend_x_b200_embedding_grad";
+        const eagle_b200_embedding_desc d = readDesc(desc, EAGLE_B200_EMBEDDING_ACCUMULATE, who);
+        if (desc->struct_size < sizeof d)
+            invalid(std::string(who) + ": struct_size too small for the query's answer");
+        checkEmbedding(d, who);
+        const GradPlan p = planGrad(d, who);
+        if (d.scratch == 0) {
+            desc->scratch_bytes = int64_t(p.bytes);
+            return;
+        }
+        if (d.rows == 0 || d.dim == 0)
+            return;
+        requireDevice();
+        DeviceScope scope(resolveDevice(d.device, d.table));
+        enqueueGrad(d, p, who);
+    });
+}

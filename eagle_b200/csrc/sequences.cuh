@@ -1,0 +1,112 @@
+// Shared pieces of the token-sequence operators (embedding.cu, paged.cu): element
+// conversions, division by a launch constant and the checks of their descs.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace eb {
+
+// ------------------------------------------------------------- launch-constant division
+
+/** Quotient by a divisor fixed at launch, for dividends below 2^31: with l = ceil(log2 d)
+ *  and m = floor(2^32 (2^l - d) / d) + 1, n / d = (mulhi(n, m) + n) >> l (Granlund and
+ *  Montgomery, "Division by invariant integers using multiplication", 1994). */
+struct FastDiv {
+    uint32_t d = 1, mul = 1, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t div)
+        : d(div)
+    {
+        while ((uint64_t(1) << shift) < div)
+            ++shift;
+        mul = uint32_t(((uint64_t(1) << 32) * ((uint64_t(1) << shift) - div)) / div + 1);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
+// ------------------------------------------------------------- elements
+
+template <class T>
+__device__ __forceinline__ float toFloat(T v);
+template <>
+__device__ __forceinline__ float toFloat<float>(float v)
+{
+    return v;
+}
+template <>
+__device__ __forceinline__ float toFloat<__nv_bfloat16>(__nv_bfloat16 v)
+{
+    return __bfloat162float(v);
+}
+template <>
+__device__ __forceinline__ float toFloat<__half>(__half v)
+{
+    return __half2float(v);
+}
+
+/** The one rounding of a result, to nearest even. */
+template <class T>
+__device__ __forceinline__ T fromFloat(float v);
+template <>
+__device__ __forceinline__ float fromFloat<float>(float v)
+{
+    return v;
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 fromFloat<__nv_bfloat16>(float v)
+{
+    return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half fromFloat<__half>(float v)
+{
+    return __float2half_rn(v);
+}
+
+/** N neighbouring elements, moved as words of up to 16 bytes. */
+template <class T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+    T e[N];
+};
+
+// ------------------------------------------------------------- host side
+
+inline int elementBytes(uint32_t type, const char* who)
+{
+    switch (type) {
+    case EAGLE_B200_TYPE_F32: return 4;
+    case EAGLE_B200_TYPE_BF16:
+    case EAGLE_B200_TYPE_F16: return 2;
+    default: unsupported(std::string(who) + ": element type " + std::to_string(type) + " is not F32, BF16 or F16");
+    }
+}
+
+inline int indexBytes(uint32_t type, const char* who)
+{
+    switch (type) {
+    case EAGLE_B200_TYPE_I32: return 4;
+    case EAGLE_B200_TYPE_I64: return 8;
+    default: unsupported(std::string(who) + ": index type " + std::to_string(type) + " is not I32 or I64");
+    }
+}
+
+/** ``p`` is an address whose elements of ``bytes`` are aligned. */
+inline void requireAddress(uint64_t p, uint64_t bytes, const char* who, const char* what)
+{
+    if (p == 0 || p % bytes != 0)
+        invalid(std::string(who) + ": " + what + " must be a device address aligned to " + std::to_string(bytes)
+            + " bytes");
+}
+
+/** A grid of ``want`` blocks, refused where it passes the launch limit. */
+inline unsigned gridOf(int64_t want, const char* who)
+{
+    if (want > 0x7fffffffll)
+        unsupported(std::string(who) + ": the call is larger than one launch holds");
+    return unsigned(want);
+}
+
+}  // namespace eb

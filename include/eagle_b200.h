@@ -888,6 +888,125 @@ eagle_backend_status eagle_backend_x_b200_engine_kernel_ms(eagle_b200_engine h, 
 eagle_backend_status eagle_backend_x_b200_probe_fp64(int32_t device, uint32_t kind, uint32_t ctas_per_sm,
     uint64_t stream, double* fma_per_s);
 
+/* ---- token sequences (this backend's additions; no counterpart in the reference) -- */
+
+/* What an until-done loop over token sequences does around its model: the embedding
+ * rows of a batch's tokens, the gradient of the table, the blocks of a paged cache that
+ * grown sequences take, and the cache slots of a pass's new tokens. All enqueue only,
+ * read nothing back and are capturable. */
+#define EAGLE_B200_TYPE_F32 0u
+#define EAGLE_B200_TYPE_BF16 1u
+#define EAGLE_B200_TYPE_F16 2u
+#define EAGLE_B200_TYPE_I32 3u
+#define EAGLE_B200_TYPE_I64 4u
+
+/* embedding_grad: add to the table's rows instead of writing all of them. */
+#define EAGLE_B200_EMBEDDING_ACCUMULATE 1u
+
+/* A table of ``rows`` x ``dim`` values, the row of token id ``first + r`` being row r
+ * (``first`` > 0: a contiguous shard of a larger table), ``batch`` x ``seq`` token ids,
+ * and one vector of ``dim`` values per token. Strides are in elements. */
+struct eagle_b200_embedding_desc {
+    uint32_t struct_size;
+    uint32_t flags;           /* embedding_grad: EAGLE_B200_EMBEDDING_ACCUMULATE */
+    int32_t device;           /* -1: the device owning the table */
+    uint32_t table_type;      /* F32, BF16 or F16 */
+    uint32_t values_type;     /* F32, BF16 or F16 */
+    uint32_t token_type;      /* I32 or I64 */
+    uint64_t table;           /* embedding reads it, embedding_grad writes it */
+    uint64_t tokens;
+    uint64_t values;          /* embedding writes them, embedding_grad reads them */
+    uint64_t scratch;         /* embedding_grad: scratch_bytes, 256-byte aligned; 0 is the query */
+    int64_t rows;             /* 0 <= rows <= 2^31 - 2 */
+    int64_t dim;              /* 0 <= dim <= 2^24 */
+    int64_t first;            /* >= 0 */
+    int64_t batch;            /* batch * seq <= 2^31 - 1 */
+    int64_t seq;
+    int64_t table_stride;     /* between rows, >= dim; a row's values are contiguous */
+    int64_t token_strides[2]; /* batch, seq */
+    int64_t value_strides[3]; /* batch, seq, dim (embedding: dim contiguous, vectors disjoint) */
+    double scale;             /* rounded to 32 bits */
+    uint64_t stream;
+    int64_t scratch_bytes;    /* out: embedding_grad's query */
+};
+
+/* eagle_backend_x_b200_embedding: values[b, s, :] = scale * table[token[b, s] - first, :],
+ * the product in 32 bits and rounded once to values_type. A token outside [first, first
+ * + rows) -- padding marked -1, a row of another shard -- gives a vector of zeros. One
+ * kernel; the outputs may not overlap the inputs. */
+eagle_backend_status eagle_backend_x_b200_embedding(const struct eagle_b200_embedding_desc* desc);
+
+/* eagle_backend_x_b200_embedding_grad: table[v, :] = scale * (the sum of values[b, s, :]
+ * over the tokens equal to first + v), zeros where there is none; with ACCUMULATE, that
+ * is added to the rows that have tokens and the others stay as they are. Tokens outside
+ * [first, first + rows) are left out, their values unread. The tokens are sorted
+ * (stable) and each row summed in 32 bits in token order, in runs of a length fixed by the
+ * sizes alone, so the bits depend on neither the launch nor the device's load; one
+ * rounding to table_type at the end. The values' strides may be anything, 0 (a broadcast
+ * gradient) included. Query with scratch == 0. */
+eagle_backend_status eagle_backend_x_b200_embedding_grad(struct eagle_b200_embedding_desc* desc);
+
+/* A paged cache: ``requests`` sequences whose tokens lie in blocks of ``block`` places;
+ * row r of ``table`` (int32[requests][width], row stride ``table_stride``) names request
+ * r's blocks in order of position. */
+struct eagle_b200_paged_desc {
+    uint32_t struct_size;
+    uint32_t flags;        /* 0 */
+    int32_t device;        /* -1: the device owning the table */
+    uint32_t length_type;  /* of lengths, start, fresh and positions: I32 or I64 */
+    uint32_t slot_type;    /* of slots: I32 or I64 */
+    uint32_t reserved0;
+    int64_t requests;      /* 0 <= requests <= 2^20 */
+    int64_t width;         /* blocks a row of the table holds, >= 0 */
+    int64_t table_stride;  /* >= width */
+    int64_t block;         /* >= 1; width * block <= 2^31 - 1 */
+    uint64_t table;
+    uint64_t terminated;   /* u8[requests] or 0: a set byte is a finished request */
+    uint64_t lengths;      /* block_tables: the length each request is to have room for */
+    uint64_t held;         /* block_tables: int32[requests], the blocks each has */
+    uint64_t pool;         /* block_tables: int32[pool_size], ids of free blocks */
+    uint64_t count;        /* block_tables: uint32, how many of the pool are valid */
+    int64_t pool_size;
+    uint64_t used;         /* block_tables: u8[used_size] or 0: the blocks in use */
+    int64_t used_size;
+    uint64_t blocks;       /* block_tables out: int32[requests], the blocks each has now */
+    uint64_t cells;        /* block_tables out: uint32[2] = {blocks taken, requests left short} */
+    uint64_t start;        /* slot_map: the position of each request's first new token */
+    uint64_t fresh;        /* slot_map: the new tokens of each request */
+    int64_t capacity;      /* slot_map: entries of slots, positions and token_requests */
+    uint64_t slots;        /* slot_map out: slot_type[capacity], 16-byte aligned */
+    uint64_t positions;    /* slot_map out: length_type[capacity], 16-byte aligned */
+    uint64_t token_requests; /* slot_map out: int32[capacity], 16-byte aligned */
+    uint64_t offsets;      /* slot_map out: int32[requests + 1] */
+    uint64_t scratch;      /* scratch_bytes, 16-byte aligned; 0 is the query */
+    uint64_t stream;
+    int64_t scratch_bytes; /* out: the query */
+};
+
+/* eagle_backend_x_b200_block_tables: every live request gets the blocks that
+ * ceil(length / block) needs past those it holds, in request order, from the front of
+ * the pool -- compact_device's (index_map, count) of the ``used`` mask, MASK_IS_DROP, is
+ * such a pool -- and their bytes in ``used`` are set. A request whose blocks do not all
+ * fit in what the requests before it left of the pool (those left short included), or
+ * that needs more than ``width``, keeps what it holds and is counted short; one that
+ * needs no more than it holds keeps its blocks. A terminated request gives its blocks
+ * back: their bytes in ``used`` are cleared and it then holds 0. Entries of ``table``
+ * past what a request holds are left as they were; ``held`` is not written. A count
+ * above pool_size (compact_device's report of a failure) is an empty pool. Negative
+ * lengths and holdings count as 0. Query with scratch == 0. */
+eagle_backend_status eagle_backend_x_b200_block_tables(struct eagle_b200_paged_desc* desc);
+
+/* eagle_backend_x_b200_slot_map: the new tokens of all live requests packed in request
+ * order: offsets[r] is where request r's begin (offsets[requests] their number,
+ * both at most 2^31 - 1), and the i-th of them has position start[r] + i, request r and
+ * slot table[r][position / block] * block + position % block; slot -1 where the position
+ * lies past the table's width (one past length_type's range wraps), the entry is
+ * negative or the slot does not fit slot_type.
+ * Entries past the last token get slot -1, position 0 and request -1; tokens past
+ * ``capacity`` are left out. Negative starts and counts count as 0. Query with
+ * scratch == 0. */
+eagle_backend_status eagle_backend_x_b200_slot_map(struct eagle_b200_paged_desc* desc);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,675 @@
+"""The token-sequence operators against plain implementations in 64 bits.
+
+Tolerances, with u(t) half the spacing of type t at 1 (2^-8 bf16, 2^-11 fp16, 2^-24 fp32)
+and s(t) half its smallest subnormal:
+
+* a looked-up value is one product in 32 bits and one rounding: u(fp32) |w| + u(out) |w|
+  (1 + u(fp32)) + s(out), w the product with the scale as rounded to 32 bits;
+* a gradient is a sum of m terms in 32 bits in some order, one product and one rounding: at
+  most (m - 1) u(fp32) / (1 - m u(fp32)) sum |x| for the sum, then as above, and one more
+  u(fp32) of the result where it is added to a row.
+
+Index operators are compared exactly."""
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def least(dtype):
+    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+
+
+def _gen(*seed):
+    return np.random.default_rng(list(seed))
+
+
+def _values(rng, shape, dtype):
+    return torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).to(dtype)
+
+
+def _close(got, want, tol):
+    got = got.double().cpu()
+    assert got.shape == want.shape
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), (int(bad.sum()), got[bad][:4], want[bad][:4])
+
+
+# ------------------------------------------------------------------------- lookup
+
+def _check_lookup(eb, table, tokens, *, scale=1.0, first=0, out=None, dtype=None):
+    got = eb.embedding(table, tokens, scale=scale, first=first, out=out, dtype=dtype)
+    if out is not None:
+        assert got is out
+    assert got.dtype == (dtype or (out.dtype if out is not None else table.dtype))
+    ids = tokens.cpu().long() - first
+    known = (ids >= 0) & (ids < table.shape[0]) & (tokens.cpu() >= first)
+    padded = torch.cat((table.cpu().double(), torch.zeros(1, table.shape[1], dtype=torch.float64)))
+    want = padded[torch.where(known, ids, table.shape[0])] * float(np.float32(scale))
+    u32 = half_step(torch.float32)
+    _close(got, want, want.abs() * (u32 + half_step(got.dtype) * (1 + u32)) + least(got.dtype))
+    return got
+
+
+@pytest.mark.parametrize("dim", (1, 2, 8, 33, 64, 777, 1024, 4100))
+@pytest.mark.parametrize("n", (1, 31, 1000))
+def test_lookup_sizes(eb, n, dim):
+    rng = _gen(1, n, dim)
+    table = _values(rng, (513, dim), torch.bfloat16).cuda()
+    ids = torch.from_numpy(rng.integers(-2, 516, n)).cuda()
+    _check_lookup(eb, table, ids, scale=dim ** 0.5)
+
+
+@pytest.mark.parametrize("source", FLOATS)
+@pytest.mark.parametrize("target", FLOATS)
+@pytest.mark.parametrize("ids_type", (torch.int32, torch.int64))
+def test_lookup_types(eb, source, target, ids_type):
+    rng = _gen(2)
+    table = _values(rng, (300, 264), source)
+    table[7, :5] = torch.tensor([0.0, -0.0, 1e-7, 3e4, 6e-8]).to(source)  # subnormal halves among them
+    ids = torch.from_numpy(rng.integers(0, 300, (3, 50))).to(ids_type)
+    ids[1, 3] = 7
+    _check_lookup(eb, table.cuda(), ids.cuda(), scale=0.37, dtype=target)
+
+
+def test_lookup_is_exact_without_a_scale(eb):
+    for dtype in FLOATS:
+        table = _values(_gen(3), (100, 40), dtype).cuda()
+        table[3, 0], table[3, 1], table[3, 2] = float("inf"), float("-inf"), float("nan")
+        ids = torch.arange(99, -1, -1).cuda()
+        got = eb.embedding(table, ids)
+        assert torch.equal(got.nan_to_num(5.0), table[ids].nan_to_num(5.0)) and got[96, 2].isnan()
+
+
+def test_lookup_strides(eb):
+    rng = _gen(4)
+    wide = _values(rng, (200, 96), torch.float16).cuda()
+    ids = torch.from_numpy(rng.integers(-1, 200, (12, 34))).cuda()
+    for table in (wide[:, 8:72], wide[:, 3:70], wide[::2], wide[50:51], wide[:, 5:6]):
+        for tokens in (ids, ids.t(), ids[:, ::3], ids[3], ids[0, 0], ids[:0], ids.view(3, 4, 34),
+                       ids[0].expand(5, 34), ids[:, :1].expand(12, 7)):
+            _check_lookup(eb, table, tokens.remainder(table.shape[0] + 1) - 1 if tokens.numel() else tokens)
+            _check_lookup(eb, table, tokens)
+    # an output inside a larger one, both token axes strided
+    room = torch.full((12, 40, 80), 7.0, dtype=torch.float16, device="cuda")
+    out = room[:, 2:36, 8:72]
+    _check_lookup(eb, wide[:, 8:72], ids, out=out)
+    room[:, 2:36, 8:72] = 7.0
+    assert bool((room == 7.0).all())
+    # the token axes the other way round
+    swapped = torch.empty(34, 12, 64, dtype=torch.float16, device="cuda").transpose(0, 1)
+    _check_lookup(eb, wide[:, 8:72], ids, out=swapped)
+    # three axes that do not join
+    with pytest.raises(ValueError, match="join"):
+        eb.embedding(wide, ids.view(3, 4, 34).transpose(0, 2))
+
+
+def test_lookup_of_a_shard(eb):
+    rng = _gen(5)
+    table = _values(rng, (1000, 128), torch.float32).cuda()
+    ids = torch.from_numpy(rng.integers(0, 1000, 777)).cuda()
+    parts = [eb.embedding(table[a:b], ids, first=a, scale=3.0) for a, b in ((0, 300), (300, 301), (301, 1000))]
+    assert torch.equal(parts[0] + parts[1] + parts[2], eb.embedding(table, ids, scale=3.0))
+    far = torch.tensor([2**62, -2**62, 2**63 - 1, -2**63, 5, 2**31 + 3], device="cuda")
+    got = _check_lookup(eb, table, far, first=2**31)
+    assert torch.equal(got[5], table[3]) and int((got != 0).any(1).sum()) == 1
+    assert not _check_lookup(eb, table, far, first=2**62 + 1).any()
+    assert not eb.embedding(table[:0], ids).any()
+
+
+def test_lookup_past_32_bits(eb):
+    """A table and an output of more than 2^31 elements each."""
+    rows, dim = 1_100_000, 2048
+    table = torch.zeros(rows, dim, dtype=torch.bfloat16, device="cuda")
+    last = torch.arange(rows - 64, rows, device="cuda")
+    table[last] = torch.randn(64, dim, device="cuda").to(torch.bfloat16)
+    ids = torch.full((rows,), -1, dtype=torch.int32, device="cuda")
+    ids[-64:] = last.flip(0).int()
+    got = eb.embedding(table, ids)
+    assert torch.equal(got[-64:], table[last.flip(0)]) and not got[:-64].any()
+
+
+# ------------------------------------------------------------------------- gradient
+
+def _check_gradient(eb, grad, tokens, rows, *, scale=1.0, first=0, out=None, dtype=None, accumulate=False):
+    before = out.double().cpu() if accumulate else None
+    got = eb.embedding_grad(grad, tokens, rows, scale=scale, first=first, out=out, dtype=dtype,
+                            accumulate=accumulate)
+    dim = grad.shape[-1]
+    ids = tokens.cpu().long().reshape(-1) - first
+    known = (ids >= 0) & (ids < rows) & (tokens.cpu().reshape(-1) >= first)
+    x = grad.cpu().double().reshape(-1, dim)
+    ids, x = ids[known], x[known]
+    total = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, ids, x)
+    size = torch.zeros(rows, dim, dtype=torch.float64).index_add_(0, ids, x.abs())
+    m = torch.bincount(ids, minlength=rows).double()[:, None]
+    s, u32 = float(np.float32(scale)), half_step(torch.float32)
+    summed = (m - 1).clamp(min=0) * u32 / (1 - m * u32) * size
+    want = total * s
+    tol = summed * abs(s) + u32 * (want.abs() + summed * abs(s))
+    if accumulate:
+        want = want + before
+        tol = tol * (1 + u32) + u32 * want.abs()
+    tol = tol + half_step(got.dtype) * (want.abs() + tol) + least(got.dtype)
+    _close(got, want, tol)
+    if accumulate:
+        untouched = torch.ones(rows, dtype=torch.bool)
+        untouched[ids] = False
+        assert torch.equal(got.cpu()[untouched].double(), before[untouched])
+    return got
+
+
+def _ids(rng, kind, n, rows):
+    if kind == "uniform":
+        return rng.integers(0, rows, n)
+    if kind == "skewed":  # the r-th most frequent about 1/r as often as the first, some padding
+        rank = np.minimum(np.exp(rng.random(n) * np.log(rows)).astype(np.int64) - 1, rows - 1).clip(0)
+        ids = rng.permutation(rows)[rank]
+        return np.where(rng.random(n) < 0.1, -1, ids)
+    if kind == "one":
+        return np.full(n, rows - 1)
+    if kind == "none":
+        return np.where(np.arange(n) % 2 == 0, -1, rows)
+    return np.arange(n)[::-1] % rows  # falling
+
+
+@pytest.mark.parametrize("kind", ("uniform", "skewed", "one", "none", "falling"))
+@pytest.mark.parametrize("n,rows,dim", [(0, 5, 8), (1, 1, 1), (1, 300, 64), (7, 3, 24), (65, 2, 520), (301, 8209, 40),
+                                        (4096, 511, 72), (4096, 512, 33), (4097, 513, 64), (9000, 40009, 777),
+                                        (20000, 1000, 128), (5000, 300000, 16)])
+def test_gradient_sizes(eb, n, rows, dim, kind):
+    rng = _gen(6, n, rows, dim)
+    grad = _values(rng, (n, dim), torch.bfloat16).cuda()
+    _check_gradient(eb, grad, torch.from_numpy(_ids(rng, kind, n, rows)).cuda(), rows, dtype=torch.float32)
+
+
+@pytest.mark.parametrize("source", FLOATS)
+@pytest.mark.parametrize("target", FLOATS)
+@pytest.mark.parametrize("accumulate", (False, True))
+@pytest.mark.parametrize("n,dim", [(700, 64), (700, 37), (9000, 136)])
+def test_gradient_types(eb, source, target, accumulate, n, dim):
+    rng = _gen(7, n)
+    rows = 350
+    grad = _values(rng, (n, dim), source).cuda()
+    ids = torch.from_numpy(_ids(rng, "skewed", n, rows)).int().cuda()
+    out = _values(rng, (rows, dim), target).cuda()
+    _check_gradient(eb, grad, ids, rows, scale=0.3, out=out, accumulate=accumulate)
+
+
+@pytest.mark.parametrize("n", (600, 6000))
+def test_gradient_strides(eb, n):
+    rng = _gen(8, n)
+    rows, dim = 97, 64
+    ids = torch.from_numpy(rng.integers(-1, rows, (6, n // 6))).cuda()
+    base = _values(rng, (n // 6, 6, 72), torch.float16).cuda()
+    for grad in (base[..., 8:72].transpose(0, 1), base[..., 3:67].transpose(0, 1),
+                 torch.ones((), dtype=torch.float16, device="cuda").expand(6, n // 6, dim),  # a sum's gradient
+                 base[:, 0, :64].unsqueeze(0).expand(6, n // 6, dim),
+                 base[0, :, :64].unsqueeze(1).expand(6, n // 6, dim),
+                 base[..., :1].transpose(0, 1).expand(6, n // 6, dim),
+                 torch.as_strided(base, (6, n // 6, dim), (1, 6, n))):
+        _check_gradient(eb, grad, ids, rows, dtype=torch.float32)
+    grad = base[..., 8:72].transpose(0, 1)
+    _check_gradient(eb, grad, ids.t().contiguous().t(), rows)
+    _check_gradient(eb, grad.reshape(2, 3, n // 6, dim), ids.view(2, 3, n // 6), rows)
+    # a table's gradient inside a larger plane; what lies around it stays
+    for columns in (slice(8, 72), slice(3, 67)):
+        room = torch.full((rows + 2, 80), 5.0, device="cuda")
+        _check_gradient(eb, grad, ids, rows, out=room[1:-1, columns])
+        room[1:-1, columns] = 5.0
+        assert bool((room == 5.0).all())
+
+
+def test_gradient_of_a_shard(eb):
+    rng = _gen(9)
+    grad = _values(rng, (6000, 48), torch.bfloat16).cuda()
+    ids = torch.from_numpy(rng.integers(0, 1000, 6000)).cuda()
+    whole = eb.embedding_grad(grad, ids, 1000, dtype=torch.float32)
+    for first, rows in ((0, 400), (400, 600), (999, 1), (5000, 30)):
+        part = _check_gradient(eb, grad, ids, rows, first=first, dtype=torch.float32)
+        if first < 1000:
+            assert torch.allclose(part, whole[first:first + rows], rtol=1e-5, atol=1e-4)
+    assert eb.embedding_grad(grad, ids, 0).shape == (0, 48)
+    assert eb.embedding_grad(grad[:, :0], ids, 7).shape == (7, 0)
+
+
+def test_gradient_ignores_what_padding_holds(eb):
+    for n in (500, 5000):
+        grad = torch.ones(n, 40, dtype=torch.bfloat16, device="cuda")
+        ids = torch.arange(n, device="cuda") % 7
+        ids[::3] = -1
+        grad[::3] = float("nan")
+        assert torch.equal(eb.embedding_grad(grad, ids, 9)[:, 0].float().cpu(),
+                           torch.bincount(ids[ids >= 0], minlength=9).float().bfloat16().float().cpu())
+        grad[4], ids[4] = float("inf"), 8
+        got = eb.embedding_grad(grad, ids, 9)
+        assert bool(got[8].isinf().all()) and bool(got[:8].isfinite().all())
+
+
+@pytest.mark.parametrize("n,dim", [(4000, 256), (30000, 264), (30000, 71)])
+def test_gradient_bits_do_not_depend_on_the_run(eb, n, dim):
+    """The same bits from a repeated call, a graph, misaligned memory and beside other work."""
+    rng = _gen(10, n)
+    rows = 5000
+    grad = _values(rng, (n, dim), torch.float32).cuda()
+    ids = torch.from_numpy(_ids(rng, "skewed", n, rows)).cuda()
+    want = eb.embedding_grad(grad, ids, rows).clone()
+    shifted = torch.empty(n, dim + 1, device="cuda")[:, 1:]
+    shifted.copy_(grad)
+    assert torch.equal(eb.embedding_grad(shifted, ids, rows), want)
+    call = eb.EmbeddingGrad(grad, ids, rows)
+    side = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    for _ in range(5):
+        with torch.cuda.stream(side):
+            busy @ busy
+        assert torch.equal(call(), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    call.out.fill_(-1.0)
+    graph.replay()
+    assert torch.equal(call.out, want)
+    ids.copy_(ids.flip(0))
+    grad.copy_(grad.flip(0))
+    graph.replay()
+    _check_gradient(eb, grad, ids, rows)
+    assert torch.equal(call.out, eb.embedding_grad(grad, ids, rows))
+
+
+def test_gradient_is_that_of_the_lookup(eb):
+    """Central differences of sum(y * c) in 32 bits; the function is linear, so they carry only roundings."""
+    rng = _gen(11)
+    table = _values(rng, (30, 16), torch.float32).cuda()
+    ids = torch.from_numpy(rng.integers(-1, 30, (4, 25))).cuda()
+    c = _values(rng, (4, 25, 16), torch.float32).cuda()
+    got = eb.embedding_grad(c, ids, 30, scale=1.5).double().cpu()
+
+    def value(t):
+        return float((eb.embedding(t, ids, scale=1.5).double() * c.double()).sum())
+
+    for v, k in ((0, 0), (3, 7), (29, 15), (11, 2)):
+        up, down = table.clone(), table.clone()
+        up[v, k] += 0.5
+        down[v, k] -= 0.5
+        step = float(up[v, k].double() - down[v, k].double())
+        # every looked-up value carries at most 2^-24 |1.5 w|, |w| < 6, times |c| < 6, in at most 100 terms
+        tol = 2 * 100 * 2**-24 * 9 * 6 / step + 1e-4
+        assert abs((value(up) - value(down)) / step - got[v, k]) <= tol
+
+
+def test_gradient_past_32_bits(eb):
+    n, dim, rows = 1_100_000, 2048, 3
+    grad = torch.ones(1, 1, dtype=torch.bfloat16, device="cuda").expand(n, dim)
+    ids = torch.zeros(n, dtype=torch.int32, device="cuda")
+    ids[-1000:] = 2
+    full = grad.contiguous()
+    full[-1000:] = 3.0
+    for g, last in ((grad, 1000.0), (full, 3000.0)):
+        got = eb.embedding_grad(g, ids, rows, dtype=torch.float32)
+        assert bool((got[0] == n - 1000).all()) and not got[1].any() and bool((got[2] == last).all())
+    wide = eb.embedding_grad(full[-2:], ids[-2:] * (n // 2), n + 1, dtype=torch.bfloat16)
+    assert bool((wide[n] == 6.0).all()) and not wide[:n].any()
+
+
+# ------------------------------------------------------------------------- block tables
+
+def _want_tables(lengths, held, table, pool, count, block, used, terminated):
+    """One request after the other, in whole numbers."""
+    table, used = table.copy(), None if used is None else used.copy()
+    width, asked, taken, short = table.shape[1], 0, 0, 0
+    count = count if 0 <= count <= len(pool) else 0
+    blocks = []
+    for r in range(len(lengths)):
+        have = min(max(int(held[r]), 0), width)
+        if terminated is not None and terminated[r]:
+            if used is not None:
+                for b in table[r, :have]:
+                    if 0 <= b < len(used):
+                        used[b] = 0
+            blocks.append(0)
+            continue
+        need = -(-max(int(lengths[r]), 0) // block)
+        more = max(0, need - have) if need <= width else 0
+        asked += more
+        if need > width or (more and asked > count):
+            short += 1
+            blocks.append(have)
+            continue
+        for j in range(more):
+            table[r, have + j] = pool[asked - more + j]
+            if used is not None and 0 <= pool[asked - more + j] < len(used):
+                used[pool[asked - more + j]] = 1
+        taken = asked if more else taken
+        blocks.append(max(need, have))
+    return table, used, np.array(blocks, np.int32), np.array([taken, short], np.int32)
+
+
+def _check_tables(eb, lengths, held, table, pool, count, block, used=None, terminated=None):
+    want = _want_tables(lengths, held, table, pool, count, block, used, terminated)
+    dev = [torch.from_numpy(np.ascontiguousarray(x)).cuda() for x in (lengths, held, table, pool)]
+    used_ = None if used is None else torch.from_numpy(used).cuda()
+    term = None if terminated is None else torch.from_numpy(terminated).cuda()
+    cell = torch.tensor([count], dtype=torch.int32, device="cuda")
+    call = eb.BlockTables(*dev, cell, block=block, used=used_, terminated=term)
+    for _ in range(2):  # a repeated call gives the same
+        blocks, cells = call()
+        assert np.array_equal(dev[2].cpu().numpy(), want[0])
+        assert used is None or np.array_equal(used_.cpu().numpy(), want[1])
+        assert np.array_equal(blocks.cpu().numpy(), want[2]) and np.array_equal(cells.cpu().numpy(), want[3])
+    return want
+
+
+@pytest.mark.parametrize("requests", (0, 1, 2, 33, 513, 8192, 8193, 20000))
+@pytest.mark.parametrize("block", (1, 16, 24))
+@pytest.mark.parametrize("dtype", (np.int32, np.int64))
+def test_tables(eb, requests, block, dtype):
+    rng = _gen(12, requests, block)
+    width = 20
+    for share, done in ((2.0, 0.0), (0.6, 0.2), (0.0, 1.0)):
+        held = rng.integers(0, width + 1, requests).astype(np.int32)
+        lengths = (held.astype(np.int64) * block + rng.integers(-2 * block, 3 * block, requests)).astype(dtype)
+        blocks = max(1, requests * width)
+        owner = rng.permutation(2 * blocks).astype(np.int32)
+        table = np.full((requests, width), -1, np.int32)
+        table[np.arange(width) < held[:, None]] = owner[:int(held.sum())]
+        used = np.zeros(2 * blocks, np.uint8)
+        used[owner[:int(held.sum())]] = 1
+        pool = np.flatnonzero(used == 0).astype(np.int32)
+        count = min(len(pool), int(requests * share))
+        _check_tables(eb, lengths, held, table, pool, count, block, used, rng.random(requests) < done)
+
+
+def test_tables_at_the_edges(eb):
+    i32 = np.int32
+    pool = np.arange(10, 20, dtype=i32)
+    table = np.full((4, 3), -7, i32)
+    zeros = np.zeros(4, i32)
+    for lengths, held, count in (
+            ([0, 0, 0, 0], [0, 0, 0, 0], 10), ([48, 49, 48, 0], [0, 0, 0, 3], 10),  # 49: past the row
+            ([48, 48, 48, 48], [0, 0, 0, 0], 10), ([48, 48, 48, 1], [0, 0, 0, 0], 9), ([16, 16, 16, 16], [1] * 4, 0),
+            ([-5, 2**31 - 1, 1, 1], [0, 0, 0, 0], 2), ([1, 1, 1, 1], [-3, 9, 3, 0], 4), ([48] * 4, [0] * 4, -1),
+            ([48] * 4, [0] * 4, 11), ([1] * 4, [0] * 4, 3)):
+        _check_tables(eb, np.array(lengths, i32), np.array(held, i32), table, pool, count, 16)
+    # ids outside the mask are handed out, and nothing is written for them
+    odd = np.array([5, -1, 100, 2**31 - 1, 0, 1], i32)
+    _check_tables(eb, np.array([48, 48, 0, 0], i32), zeros, table, odd, 6, 16, np.zeros(8, np.uint8))
+    # neither may a terminated request's row name what the mask does not have
+    rows = np.array([[3, -1, 2**31 - 1], [1, 2, 9], [0, 0, 0], [4, 4, 4]], i32)
+    _check_tables(eb, np.full(4, 40, np.int64), np.array([3, 2, 0, 99], i32), rows, pool[:0], 0, 16,
+                  np.ones(6, np.uint8), np.array([True, True, True, True]))
+    # width 0, and lengths in 64 bits past every row
+    _check_tables(eb, np.array([0, 1, 0, 2**62]), zeros, table[:, :0], pool, 10, 16)
+    _check_tables(eb, np.array([2**62, -2**62, 2**63 - 1, 5]), zeros, table, pool, 10, 16)
+
+
+def test_tables_in_a_wider_plane(eb):
+    plane = torch.full((5, 16), -1, dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([3, 70, 0, 33, 16], device="cuda")
+    held = torch.zeros(5, dtype=torch.int32, device="cuda")
+    pool = torch.arange(100, 150, dtype=torch.int32, device="cuda")
+    count = torch.tensor([50], dtype=torch.int32, device="cuda")
+    blocks, cells = eb.block_tables(lengths, held, plane[:, 3:9], pool, count, block=16)
+    assert blocks.tolist() == [1, 5, 0, 3, 1] and cells.tolist() == [10, 0]
+    assert plane[:, :3].eq(-1).all() and plane[:, 9:].eq(-1).all()
+    assert plane[1, 3:9].tolist() == [101, 102, 103, 104, 105, -1] and plane[3, 3:6].tolist() == [106, 107, 108]
+
+
+# ------------------------------------------------------------------------- slots
+
+def _want_slots(table, start, fresh, capacity, block, terminated, bits=64):
+    slots, positions, requests = np.full(capacity, -1, np.int64), np.zeros(capacity, np.int64), \
+        np.full(capacity, -1, np.int32)
+    offsets, q = [0], 0
+    for r in range(len(start)):
+        n = 0 if terminated is not None and terminated[r] else max(int(fresh[r]), 0)
+        inside = max(0, min(n, capacity - q))
+        p = max(int(start[r]), 0) + np.arange(inside, dtype=object)
+        for i, at in enumerate(p):
+            b = at // block
+            if b < table.shape[1] and table[r, b] >= 0 and int(table[r, b]) * block + at % block < 2 ** (bits - 1):
+                slots[q + i] = int(table[r, b]) * block + at % block
+        wrap = 2 ** (8 * start.dtype.itemsize)  # a position past its type wraps
+        positions[q:q + inside] = [(int(at) + wrap // 2) % wrap - wrap // 2 for at in p]
+        requests[q:q + inside] = r
+        q += n
+        offsets.append(min(q, 2**31 - 1))
+    return slots, positions, requests, np.array(offsets, np.int64)
+
+
+def _check_slots(eb, table, start, fresh, capacity, block, terminated=None, dtype=torch.int64):
+    want = _want_slots(table, start, fresh, capacity, block, terminated, 64 if dtype == torch.int64 else 32)
+    dev = [torch.from_numpy(np.ascontiguousarray(x)).cuda() for x in (table, start, fresh)]
+    term = None if terminated is None else torch.from_numpy(terminated).cuda()
+    got = eb.slot_map(*dev, capacity, block=block, terminated=term, dtype=dtype)
+    assert got[0].dtype == dtype and got[1].dtype == dev[1].dtype
+    for g, w, name in zip(got, want, ("slots", "positions", "requests", "offsets")):
+        assert np.array_equal(g.cpu().numpy().astype(np.int64), w), name
+
+
+@pytest.mark.parametrize("requests", (0, 1, 5, 513, 8192, 8193))
+@pytest.mark.parametrize("block", (1, 16, 24))
+@pytest.mark.parametrize("dtype,slot", [(np.int32, torch.int64), (np.int64, torch.int32)])
+def test_slots(eb, requests, block, dtype, slot):
+    rng = _gen(13, requests, block)
+    width = 12
+    table = rng.integers(-1, 1000, (requests, width)).astype(np.int32)
+    start = rng.integers(-2, width * block, requests).astype(dtype)
+    for kind, done in (("one", 0.1), ("ragged", 0.3), ("none", 0.0), ("ragged", 1.0)):
+        fresh = {"one": np.ones(requests), "none": np.zeros(requests),
+                 "ragged": rng.integers(-1, 9, requests) * (rng.random(requests) < 0.3)}[kind].astype(dtype)
+        total = int(fresh.clip(0).sum())
+        for capacity in {0, 1, total, max(0, total - 3), total + 5}:
+            _check_slots(eb, table, start, fresh, capacity, block, rng.random(requests) < done, slot)
+
+
+def test_slots_at_the_edges(eb):
+    table = np.array([[0, 7, 2**31 - 1], [-1, 5, 6], [2**30, 1, 1]], np.int32)
+    start = np.array([0, 3, 30])
+    fresh = np.array([60, 40, 2])
+    for slot in (torch.int32, torch.int64):  # slots past 2^31 fit one of the two
+        _check_slots(eb, table, start, fresh, 103, 16, None, slot)
+    for s in (2**62, 2**63 - 1, 2**31, -2**63):
+        _check_slots(eb, table, np.array([s if s < 2**63 - 8 else s - 40, 0, s if s < 2**62 else 3]), fresh, 103, 16)
+    # more tokens than an int32 counts: offsets stop there
+    _check_slots(eb, table, start, np.array([2**31, 5, 2**62]), 50, 16)
+    _check_slots(eb, table, start.astype(np.int32), np.array([2**31 - 1] * 3, np.int32), 50, 16)
+    # width 0
+    _check_slots(eb, table[:, :0], start, fresh, 20, 16)
+    # one long request between thousands without tokens
+    fresh = np.zeros(8000, np.int64)
+    fresh[[0, 4000, 7999]] = 3, 5000, 2
+    _check_slots(eb, np.arange(8000 * 4, dtype=np.int32).reshape(8000, 4), np.zeros(8000, np.int64), fresh, 5100, 2048)
+
+
+# ------------------------------------------------------------------------- refusals
+
+def test_refusals(eb):
+    dev = dict(device="cuda")
+    table = torch.zeros(10, 16, **dev)
+    ids = torch.zeros(4, dtype=torch.int64, **dev)
+    with pytest.raises(TypeError):
+        eb.embedding(table.double(), ids)
+    with pytest.raises(TypeError):
+        eb.embedding(table, ids.short())
+    with pytest.raises(TypeError):
+        eb.embedding(table, ids, dtype=torch.float64)
+    with pytest.raises(ValueError, match="CUDA"):
+        eb.embedding(table, ids.cpu())
+    for bad in (table.t(), table[0], table[:1].expand(10, 16)):
+        with pytest.raises(ValueError):
+            eb.embedding(bad, ids)
+    with pytest.raises(ValueError, match="first"):
+        eb.embedding(table, ids, first=-1)
+    with pytest.raises(ValueError, match="autograd"):
+        eb.embedding(table.clone().requires_grad_(), ids)
+    with torch.no_grad():
+        eb.embedding(table.clone().requires_grad_(), ids)
+    for out in (torch.zeros(4, 15, **dev), torch.zeros(16, 4, **dev).t(), torch.zeros(1, 16, **dev).expand(4, 16)):
+        with pytest.raises(ValueError):
+            eb.embedding(table, ids, out=out)
+    with pytest.raises(ValueError, match="overlaps"):
+        eb.embedding(table, ids, out=table[:4])
+    grad = torch.zeros(4, 16, **dev)
+    with pytest.raises(ValueError, match="shape"):
+        eb.embedding_grad(grad[:3], ids, 10)
+    with pytest.raises(ValueError, match="rows"):
+        eb.embedding_grad(grad, ids, -1)
+    with pytest.raises(ValueError, match="accumulate"):
+        eb.embedding_grad(grad, ids, 10, accumulate=True)
+    with pytest.raises(ValueError, match="overlaps"):
+        eb.embedding_grad(grad, ids, 4, out=grad)
+    with pytest.raises(ValueError, match="shape"):
+        eb.embedding_grad(grad, ids, 10, out=table[:9])
+    with pytest.raises(ValueError, match="autograd"):
+        eb.embedding_grad(grad.clone().requires_grad_(), ids, 10)
+    tables = torch.zeros(3, 4, dtype=torch.int32, **dev)
+    lengths = torch.zeros(3, dtype=torch.int32, **dev)
+    pool, count = torch.zeros(8, dtype=torch.int32, **dev), torch.zeros(1, dtype=torch.int32, **dev)
+    good = dict(lengths=lengths, held=lengths, table=tables, pool=pool, count=count, block=16)
+    eb.block_tables(**good)
+    for change, error in ((dict(lengths=lengths.float()), TypeError), (dict(held=lengths.long()), TypeError),
+                          (dict(lengths=lengths[:2]), ValueError), (dict(table=tables.t()), ValueError),
+                          (dict(table=tables.long()), TypeError), (dict(pool=pool[::2]), ValueError),
+                          (dict(count=pool), ValueError), (dict(block=0), ValueError),
+                          (dict(pool=tables[0]), ValueError), (dict(used=pool), TypeError),
+                          (dict(used=torch.zeros(3, 2, dtype=torch.bool, **dev)), ValueError),
+                          (dict(terminated=torch.zeros(2, dtype=torch.bool, **dev)), ValueError),
+                          (dict(block=2**31), ValueError), (dict(pool=pool.cpu()), ValueError)):
+        with pytest.raises(error):
+            eb.block_tables(**{**good, **change})
+    good = dict(table=tables, start=lengths, fresh=lengths, capacity=5, block=16)
+    eb.slot_map(**good)
+    for change, error in ((dict(fresh=lengths.long()), TypeError), (dict(capacity=-1), ValueError),
+                          (dict(capacity=2**31 - 1), ValueError), (dict(dtype=torch.int16), TypeError),
+                          (dict(block=-1), ValueError), (dict(terminated=lengths), TypeError),
+                          (dict(start=lengths[:2]), ValueError)):
+        with pytest.raises(error):
+            eb.slot_map(**{**good, **change})
+
+
+# ------------------------------------------------------------------------- streams, and all of them together
+
+def test_other_streams(eb):
+    rng = _gen(14)
+    table = _values(rng, (500, 64), torch.bfloat16).cuda()
+    ids = torch.from_numpy(rng.integers(0, 500, 6000)).cuda()
+    grad = _values(rng, (6000, 64), torch.bfloat16).cuda()
+    want = eb.embedding(table, ids), eb.embedding_grad(grad, ids, 500)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    late = torch.zeros_like(ids)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            busy @ busy
+        late.copy_(ids)
+    got = eb.embedding(table, late, stream=side), eb.embedding_grad(grad, late, 500, stream=side)
+    call = eb.EmbeddingGrad(grad, late, 500)
+    again = call(side)
+    side.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(again, want[1])
+
+
+def test_a_decode_loop_in_one_graph(eb):
+    """Free list, tables, slots and rows of a pass as one captured graph, replayed until every sequence has
+    ended: each token's cache slot is its own, and what a sequence wrote reads back through its table."""
+    rng = _gen(15)
+    requests, width, block, blocks, dim, rows = 40, 8, 4, 200, 64, 100
+    stop = torch.from_numpy(rng.integers(0, width * block + 1, requests)).int().cuda()
+    lengths = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    one = torch.ones(requests, dtype=torch.int32, device="cuda")
+    wanted = torch.empty_like(lengths)
+    held = torch.zeros(requests, dtype=torch.int32, device="cuda")
+    tables = torch.full((requests, width), -1, dtype=torch.int32, device="cuda")
+    used = torch.zeros(blocks, dtype=torch.bool, device="cuda")
+    terminated = stop == 0
+    weights = _values(rng, (rows, dim), torch.bfloat16).cuda()
+    cache = torch.zeros(blocks * block + 1, dim, dtype=torch.bfloat16, device="cuda")
+    tokens = torch.empty(48, dtype=torch.int32, device="cuda")
+    free = eb.Compactor(used)
+    grow = eb.BlockTables(wanted, held, tables, free.index_map, free.count, block=block, used=used,
+                          terminated=terminated)
+    spot = eb.SlotMap(tables, lengths, one, 48, block=block, terminated=terminated)
+    look = eb.Embedding(weights, tokens)
+
+    def step():
+        torch.add(lengths, 1, out=wanted)
+        free()
+        grow()
+        held.copy_(grow.blocks)
+        slots, positions, owner, _ = spot()
+        tokens.copy_(torch.where(owner < 0, -1, (owner * 7 + positions) % rows))
+        cache[torch.where(slots < 0, blocks * block, slots)] = look()
+        lengths.add_((~terminated).int())
+        terminated.logical_or_(lengths >= stop)
+
+    state = [x.clone() for x in (lengths, held, tables, used, terminated)]
+    step()  # warm up, then back to the start
+    for x, was in zip((lengths, held, tables, used, terminated), state):
+        x.copy_(was)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    done_at = {}
+    for n in range(width * block + 1):
+        before = terminated.cpu().numpy().copy()
+        graph.replay()
+        assert grow.cells[1].item() == 0
+        live = np.flatnonzero(~before)
+        slots = spot.slots.cpu().numpy()
+        assert len(set(slots[:len(live)])) == len(live) and (slots[len(live):] == -1).all()
+        assert (spot.requests.cpu().numpy()[:len(live)] == live).all()
+        rows_ = tables.cpu().numpy()
+        have = held.cpu().numpy()
+        names = [int(b) for r in live for b in rows_[r, :have[r]]]
+        assert len(set(names)) == len(names)  # no block has two owners
+        assert int(used.sum()) == len(names)
+        for r in np.flatnonzero(terminated.cpu().numpy() & ~before):
+            length = int(lengths[r])
+            assert length == int(stop[r])
+            at = [int(rows_[r, p // block]) * block + p % block for p in range(length)]
+            want = weights[(r * 7 + torch.arange(length, device="cuda")) % rows]
+            assert torch.equal(cache[at], want)
+            done_at[r] = n
+    graph.replay()
+    assert bool(terminated.all()) and not used.any() and not held.any()
+    assert len(done_at) == int((stop > 0).sum()) and not cache[-1].any()
+
+
+def test_a_training_step(eb):
+    """Rows looked up, a gradient through a plain layer, and the table's gradient accumulated over two batches:
+    what torch's own differentiation of the same formulas gives in 64 bits."""
+    rng = _gen(16)
+    rows, dim, scale = 700, 96, 96 ** 0.5
+    table = _values(rng, (rows, dim), torch.bfloat16).cuda()
+    total = torch.zeros(rows, dim, device="cuda")
+    exact = torch.zeros(rows, dim, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(exact)
+    m = 0
+    for seed in (0, 1):
+        ids = torch.from_numpy(_ids(_gen(17, seed), "skewed", 4 * 1500, rows)).view(4, 1500).cuda()
+        c = _values(_gen(18, seed), (4, 1500, dim), torch.bfloat16).cuda()
+        y = eb.embedding(table, ids, scale=scale)
+        dy = (c * torch.where(y > 0, 1.0, 0.0)).to(torch.bfloat16)  # of sum(c * relu(y)), exact
+        eb.embedding_grad(dy, ids, rows, scale=scale, out=total, accumulate=True)
+        leaf = table.double().requires_grad_()
+        known = (ids >= 0)[..., None]
+        out = torch.where(known, leaf[ids.clamp(min=0)] * float(np.float32(scale)), 0.0)
+        (out.relu() * c.double()).sum().backward()
+        exact += leaf.grad
+        size.index_add_(0, ids.clamp(min=0).flatten(), (dy.double() * known).abs().flatten(0, 1))
+        m += 6000
+    u = half_step(torch.float32)
+    tol = (m + 6) * u / (1 - m * u) * size * float(np.float32(scale))
+    assert bool(((total.double() - exact).abs() <= tol).all())

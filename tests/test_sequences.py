@@ -1,0 +1,157 @@
+"""The token-sequence operators without a GPU: their descs' layouts, the queries and every
+refusal that needs no device."""
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from eagle_b200 import _abi
+
+torch = pytest.importorskip("torch")
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "eagle_b200.h")
+
+
+@pytest.mark.parametrize("cname,ct", [("eagle_b200_embedding_desc", _abi.EmbeddingDesc),
+                                      ("eagle_b200_paged_desc", _abi.PagedDesc)])
+def test_layouts_match_the_header(tmp_path, cname, ct):
+    lines = ['#include <stddef.h>', '#include <stdio.h>', f'#include "{HEADER}"', "int main(void) {",
+             f'printf("%zu\\n", sizeof(struct {cname}));']
+    lines += [f'printf("%zu\\n", offsetof(struct {cname}, {name}));' for name, _ in ct._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c11", "-o", str(exe), str(src)], check=True)
+    got = [int(v) for v in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    assert got == [ctypes.sizeof(ct)] + [getattr(ct, name).offset for name, _ in ct._fields_]
+
+
+def _embedding(**fields):
+    d = _abi.new(_abi.EmbeddingDesc, table_type=_abi.TYPE_BF16, values_type=_abi.TYPE_BF16, token_type=_abi.TYPE_I64,
+                 table=1 << 20, tokens=1 << 20, values=1 << 20, rows=100, dim=64, batch=2, seq=8, table_stride=64,
+                 scale=1.0)
+    d.token_strides[:] = [8, 1]
+    d.value_strides[:] = [512, 64, 1]
+    for k, v in fields.items():
+        setattr(d, k, v)
+    return d
+
+
+def _paged(**fields):
+    d = _abi.new(_abi.PagedDesc, length_type=_abi.TYPE_I32, slot_type=_abi.TYPE_I64, requests=4, width=8,
+                 table_stride=8, block=16, pool_size=64, used_size=64, capacity=32)
+    for name in ("table", "lengths", "held", "pool", "count", "used", "blocks", "cells", "start", "fresh", "slots",
+                 "positions", "token_requests", "offsets"):
+        setattr(d, name, (1 << 20) + 4096 * (1 + len(name)))
+    for k, v in fields.items():
+        setattr(d, k, v)
+    return d
+
+
+BAD_EMBEDDING = [
+    (dict(table_type=9), _abi.UNSUPPORTED), (dict(values_type=_abi.TYPE_I32), _abi.UNSUPPORTED),
+    (dict(token_type=_abi.TYPE_F32), _abi.UNSUPPORTED), (dict(flags=2), _abi.UNSUPPORTED),
+    (dict(rows=-1), _abi.INVALID_ARGUMENT), (dict(rows=2**31 - 1), _abi.INVALID_ARGUMENT),
+    (dict(dim=-1), _abi.INVALID_ARGUMENT), (dict(dim=2**24 + 1), _abi.INVALID_ARGUMENT),
+    (dict(first=-1), _abi.INVALID_ARGUMENT), (dict(batch=-1), _abi.INVALID_ARGUMENT),
+    (dict(batch=2**16, seq=2**16), _abi.INVALID_ARGUMENT), (dict(batch=2**40, seq=2**40), _abi.INVALID_ARGUMENT),
+    (dict(table_stride=63), _abi.INVALID_ARGUMENT),
+]
+
+
+@pytest.mark.parametrize("fields,status", BAD_EMBEDDING)
+@pytest.mark.parametrize("entry", ["embedding", "embedding_grad"])
+def test_embedding_refuses(entry, fields, status):
+    d = _embedding(**fields)
+    assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == status
+    assert entry in _abi.last_error()
+
+
+def test_embedding_refuses_accumulate_and_a_short_desc():
+    d = _embedding(flags=_abi.EMBEDDING_ACCUMULATE)
+    assert _abi.lib().eagle_backend_x_b200_embedding(ctypes.byref(d)) == _abi.UNSUPPORTED
+    d = _embedding(struct_size=ctypes.sizeof(_abi.EmbeddingDesc) - 8)
+    assert _abi.lib().eagle_backend_x_b200_embedding_grad(ctypes.byref(d)) == _abi.INVALID_ARGUMENT
+
+
+def test_embedding_calls_without_work_need_no_device():
+    for fields in (dict(batch=0), dict(seq=0), dict(dim=0, table_stride=0)):
+        d = _embedding(**fields)
+        assert _abi.lib().eagle_backend_x_b200_embedding(ctypes.byref(d)) == _abi.OK
+
+
+def test_gradient_query_depends_on_sizes_alone():
+    def ask(**fields):
+        d = _embedding(**fields)
+        assert _abi.lib().eagle_backend_x_b200_embedding_grad(ctypes.byref(d)) == _abi.OK
+        return d.scratch_bytes
+
+    base = ask(batch=64, seq=1024, rows=5000)
+    assert base % 256 == 0 and base > 64 * 1024 * 16
+    for other in (dict(table=(1 << 20) + 2), dict(values=(1 << 20) + 2), dict(table_type=_abi.TYPE_F32),
+                  dict(values_type=_abi.TYPE_F32), dict(token_type=_abi.TYPE_I32), dict(table_stride=65),
+                  dict(flags=_abi.EMBEDDING_ACCUMULATE)):
+        assert ask(batch=64, seq=1024, rows=5000, **other) == base, other
+    assert ask(batch=64, seq=2048, rows=5000) > base
+
+
+BAD_PAGED = [
+    (dict(length_type=_abi.TYPE_F32), _abi.UNSUPPORTED), (dict(flags=1), _abi.UNSUPPORTED),
+    (dict(reserved0=1), _abi.INVALID_ARGUMENT), (dict(requests=-1), _abi.INVALID_ARGUMENT),
+    (dict(requests=2**20 + 1), _abi.INVALID_ARGUMENT), (dict(block=0), _abi.INVALID_ARGUMENT),
+    (dict(block=2**31), _abi.INVALID_ARGUMENT), (dict(width=-1), _abi.INVALID_ARGUMENT),
+    (dict(width=2**27, table_stride=2**27), _abi.INVALID_ARGUMENT), (dict(table_stride=7), _abi.INVALID_ARGUMENT),
+]
+
+
+@pytest.mark.parametrize("fields,status", BAD_PAGED)
+@pytest.mark.parametrize("entry", ["block_tables", "slot_map"])
+def test_paged_refuses(entry, fields, status):
+    d = _paged(**fields)
+    assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == status
+    assert entry in _abi.last_error()
+
+
+@pytest.mark.parametrize("entry,fields,status", [
+    ("block_tables", dict(pool_size=-1), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(pool_size=2**31 - 1), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(used_size=-1), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(scratch=1 << 20, count=0), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(scratch=1 << 20, held=0), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(scratch=1 << 20, lengths=(1 << 20) + 2), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(scratch=1 << 20, blocks=1 << 21, held=1 << 21), _abi.INVALID_ARGUMENT),
+    ("block_tables", dict(scratch=8), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(slot_type=_abi.TYPE_BF16), _abi.UNSUPPORTED),
+    ("slot_map", dict(capacity=-1), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(capacity=2**31 - 1), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(scratch=1 << 20, slots=(1 << 20) + 8), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(scratch=1 << 20, offsets=0), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(scratch=1 << 20, length_type=_abi.TYPE_I64, start=(1 << 20) + 4), _abi.INVALID_ARGUMENT),
+])
+def test_paged_refuses_its_own(entry, fields, status):
+    d = _paged(**fields)
+    assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == status
+
+
+def test_paged_queries():
+    for entry in ("block_tables", "slot_map"):
+        for requests, least in ((0, 0), (4, 0), (8192, 0), (8193, 4 * 8193), (2**20, 4 * 2**20)):
+            d = _paged(requests=requests)
+            assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == _abi.OK
+            assert d.scratch_bytes >= max(least, 16)
+
+
+def test_host_tensors_are_refused(eb):
+    table, ids = torch.zeros(4, 8), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        eb.embedding(table, ids)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        eb.embedding_grad(torch.zeros(3, 8), ids, 4)
+    tables = torch.zeros(2, 4, dtype=torch.int32)
+    lengths = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        eb.block_tables(lengths, lengths, tables, lengths, lengths[:1], block=16)
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        eb.slot_map(tables, lengths, lengths, 8, block=16)
