@@ -22,6 +22,8 @@
 // before, which knows where its keys land.
 #include "sequences.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #define EB_API extern "C" __attribute__((visibility("default")))
@@ -108,11 +110,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
 
 // ------------------------------------------------------------------ gradient: sort
 
-constexpr int kSortThreads = 512;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortItems = 8;
-constexpr uint32_t kSortTile = uint32_t(kSortThreads) * kSortItems;  // 4096 keys
-constexpr uint32_t kMaxBins = 512;                                  // 9 bits a pass, one bin per thread
+constexpr uint32_t kMaxBins = 512;        // 9 bits a pass
 constexpr uint32_t kNoKey = 0xffffffffu;  // behind the last key: every digit of it is the highest
 
 struct GradArgs {
@@ -130,10 +128,11 @@ struct GradArgs {
     uint32_t n;
     uint32_t dim;
     // sort
-    uint32_t tiles, bins, digitBits;
-    uint32_t* present;  // a bit per row that has a token
-    uint32_t* hist;     // this pass's digit counts, [tile][bin]
-    uint32_t* nextHist; // the next pass's, gathered by this one
+    uint32_t bits, bins, digitBits;
+    uint32_t tiles;
+    uint32_t* present;   // a bit per row that has a token
+    uint32_t* hist;      // this pass's digit counts, [tile][bin]
+    uint32_t* nextHist;  // the next pass's, gathered by this one
     const uint32_t* keyIn;
     const uint32_t* posIn;
     uint32_t* keyOut;
@@ -147,14 +146,14 @@ struct GradArgs {
     uint32_t slices;     // groups a row takes
     uint32_t pieces;     // packs (or columns) per row
     uint32_t sumBlocks;  // CTAs that sum; the others zero
-    uint32_t* listCount; // chunks whose last run goes on into the next
+    uint32_t* listCount; // chunks whose last run is joined
     uint32_t* list;
-    float* head;         // [chunk][width]: the part of a run that began in an earlier chunk
-    float* tail;         // [chunk][width]: the part of a run that goes on
-    uint32_t width;      // dim rounded up to 4
+    float* head;         // [chunk][width]: the part of a long run that began in an earlier chunk
+    float* tail;         // [chunk][width]: the part of a long run that goes on
+    uint32_t width;      // dim rounded up to 8
     // zeroing
-    uint32_t zeroRows;   // rows a zeroing CTA takes at a time
-    bool zeroWide;       // rows are whole aligned 16-byte words
+    int64_t rowBytes, strideBytes;
+    uint32_t zeroed;     // rows [0, zeroed) are zeroed, with tokens or without, beside the sort
 };
 
 template <class Tok>
@@ -171,143 +170,161 @@ __device__ __forceinline__ uint32_t keyOfToken(const GradArgs& a, uint32_t i)
     return r < 0 ? uint32_t(a.rows) : uint32_t(r);
 }
 
-struct SortShared {
-    uint32_t count[kSortWarps * kMaxBins];  // [warp][bin]
-    uint32_t base[kMaxBins];
-    uint32_t scan[33];
-};
+/** One warp zeroes row ``r``: whole 16-byte words, and bytes two at a time before and after. */
+__device__ __forceinline__ void zeroRow(const GradArgs& a, int64_t r)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    char* row = reinterpret_cast<char*>(a.table) + r * a.strideBytes;
+    char* end = row + a.rowBytes;
+    char* from = reinterpret_cast<char*>((reinterpret_cast<uint64_t>(row) + 15u) & ~uint64_t(15));
+    char* to = reinterpret_cast<char*>(reinterpret_cast<uint64_t>(end) & ~uint64_t(15));
+    if (from > to) {  // inside one word
+        from = end;
+        to = end;
+    }
+    for (char* p = from + lane * 16u; p < to; p += 32 * 16)
+        *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
+    for (char* p = row + lane * 2u; p < from; p += 64)
+        *reinterpret_cast<uint16_t*>(p) = 0;
+    for (char* p = to + lane * 2u; p < end; p += 64)
+        *reinterpret_cast<uint16_t*>(p) = 0;
+}
 
-/** Each key's place among the tile's keys of its digit, in item order (a warp's items are
- *  its 256 neighbours, item k of lane l the 32 k + l-th); ``total`` is bin threadIdx.x's
- *  count. Leaves the per-warp counts scanned over the warps. */
-__device__ __forceinline__ void rankTile(const uint32_t (&digit)[kSortItems], uint32_t (&rank)[kSortItems],
-    uint32_t& total, uint32_t bins, SortShared& s)
+/** The keys of one digit value before each item among a CTA's: items are ranked warp by
+ *  warp, by match_any among the 32 of a step and by the warp's running counts between steps
+ *  (item k of lane l is the warp's 32 k + l-th). ``count`` is [warp][bins], left scanned over
+ *  the warps; bin threadIdx.x's sum is returned. */
+template <int Warps, int Items>
+__device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint32_t shift, uint32_t (&rank)[Items],
+    uint32_t bins, uint16_t* count)
 {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    for (uint32_t i = threadIdx.x; i < kSortWarps * bins; i += kSortThreads)
-        s.count[i] = 0;
+    uint32_t* words = reinterpret_cast<uint32_t*>(count);
+    for (uint32_t i = threadIdx.x; i < Warps * bins / 2; i += Warps * 32)
+        words[i] = 0;
     __syncthreads();
-    uint32_t* mine = s.count + warp * bins;
+    uint16_t* mine = count + warp * bins;
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t peers = __match_any_sync(kFull, digit[k]);
-        const uint32_t before = mine[digit[k]];
+    for (int k = 0; k < Items; ++k) {
+        const uint32_t digit = (key[k] >> shift) & (bins - 1u);
+        const uint32_t peers = __match_any_sync(kFull, digit);
+        const uint32_t before = mine[digit];
         __syncwarp();
         if (lane == uint32_t(__ffs(peers)) - 1u)
-            mine[digit[k]] = before + __popc(peers);
+            mine[digit] = uint16_t(before + __popc(peers));
         __syncwarp();
         rank[k] = before + __popc(peers & ((1u << lane) - 1u));
     }
     __syncthreads();
-    total = 0;
+    uint32_t total = 0;
     if (threadIdx.x < bins) {
 #pragma unroll
-        for (int w = 0; w < kSortWarps; ++w) {
-            const uint32_t c = s.count[w * bins + threadIdx.x];
-            s.count[w * bins + threadIdx.x] = total;
+        for (int w = 0; w < Warps; ++w) {
+            const uint32_t c = count[w * bins + threadIdx.x];
+            count[w * bins + threadIdx.x] = uint16_t(total);
             total += c;
         }
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k)
-        rank[k] += mine[digit[k]];
+    for (int k = 0; k < Items; ++k)
+        rank[k] += mine[(key[k] >> shift) & (bins - 1u)];
+    return total;
 }
 
-/** Zero the rows [row0, row1) whose bit in ``present`` (bit r - bit0) is clear, a warp per row. */
-template <class Out>
-__device__ __forceinline__ void zeroAbsent(const GradArgs& a, const uint32_t* present, uint32_t bit0, uint32_t row0,
-    uint32_t row1)
-{
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    for (uint32_t r = row0 + warp; r < row1; r += warps) {
-        if ((present[(r - bit0) >> 5] >> ((r - bit0) & 31u)) & 1u)
-            continue;
-        Out* row = reinterpret_cast<Out*>(a.table) + int64_t(r) * a.tableStride;
-        if (a.zeroWide) {
-            uint4* w = reinterpret_cast<uint4*>(row);
-            const uint32_t words = a.dim * uint32_t(sizeof(Out)) / 16u;
-            for (uint32_t i = lane; i < words; i += 32u)
-                w[i] = make_uint4(0u, 0u, 0u, 0u);
-        } else {
-            for (uint32_t i = lane; i < a.dim; i += 32u)
-                row[i] = fromFloat<Out>(0.0f);
-        }
-    }
-}
+// ---- up to kClusterKeys: one cluster, the keys in its distributed shared memory
 
-/** Up to one tile of tokens: CTA 0 sorts them in shared memory; the others zero the rows
- *  without a token, each finding those of its rows that have one by reading all the ids. */
-template <class Out, class Tok>
-__global__ __launch_bounds__(kSortThreads) void sortTileKernel(GradArgs a)
+constexpr int kClusterThreads = 1024;
+constexpr int kClusterWarps = kClusterThreads / 32;
+constexpr int kClusterSize = 8;
+constexpr int kClusterItems = 16;
+constexpr uint32_t kClusterKeys = uint32_t(kClusterThreads) * kClusterSize * kClusterItems;  // 131072
+
+/** Cluster 0 sorts: every CTA holds 1024 * Items neighbouring keys in registers; a pass ranks
+ *  them, adds up the CTAs' digit counts over distributed shared memory and stores each key
+ *  and position straight into the CTA that has its place, two cluster barriers in all. The
+ *  other clusters meanwhile zero the first ``zeroed`` rows. */
+template <class Tok, int Items>
+__global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
-    if (blockIdx.x != 0) {
-        uint32_t* present = reinterpret_cast<uint32_t*>(raw);
-        const uint32_t words = a.zeroRows / 32u;
-        for (int64_t row0 = int64_t(blockIdx.x - 1) * a.zeroRows; row0 < a.rows;
-             row0 += int64_t(gridDim.x - 1) * a.zeroRows) {
-            const uint32_t row1 = uint32_t(min(row0 + int64_t(a.zeroRows), a.rows));
-            for (uint32_t i = threadIdx.x; i < words; i += kSortThreads)
-                present[i] = 0;
-            __syncthreads();
-            for (uint32_t i = threadIdx.x; i < a.n; i += kSortThreads) {
-                const uint32_t key = keyOfToken<Tok>(a, i);
-                if (key >= uint32_t(row0) && key < row1)
-                    atomicOr(present + ((key - uint32_t(row0)) >> 5), 1u << ((key - uint32_t(row0)) & 31u));
-            }
-            __syncthreads();
-            zeroAbsent<Out>(a, present, uint32_t(row0), uint32_t(row0), row1);
-            __syncthreads();
-        }
+    __shared__ uint32_t tileCount[kMaxBins], base[kMaxBins], scan[33];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
+    if (blockIdx.x >= ctas) {
+        for (int64_t r = int64_t(blockIdx.x - ctas) * kClusterWarps + (threadIdx.x >> 5); r < int64_t(a.zeroed);
+             r += int64_t(gridDim.x - ctas) * kClusterWarps)
+            zeroRow(a, r);
         return;
     }
-    SortShared& s = *reinterpret_cast<SortShared*>(raw);
-    uint32_t* keyAt = reinterpret_cast<uint32_t*>(raw + sizeof(SortShared));
-    uint32_t* posAt = keyAt + kSortTile;
+    uint64_t* at = reinterpret_cast<uint64_t*>(raw);  // key and position by place
+    uint16_t* count = reinterpret_cast<uint16_t*>(raw + size_t(kClusterThreads) * Items * 8);
+    constexpr uint32_t kTile = uint32_t(kClusterThreads) * Items;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t item0 = warp * (32u * kSortItems) + lane;
-    uint32_t key[kSortItems], pos[kSortItems], digit[kSortItems], rank[kSortItems];
-    if (threadIdx.x == 0)
+    const uint32_t item0 = warp * (32u * Items) + lane;
+    if (cta == 0 && threadIdx.x == 0)
         *a.listCount = 0;
+    if (a.present != nullptr)
+        for (int64_t w = int64_t(cta) * kClusterThreads + threadIdx.x; w < (a.rows + 31) / 32;
+             w += int64_t(ctas) * kClusterThreads)
+            a.present[w] = 0;
+    uint32_t key[Items], pos[Items], rank[Items];
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        pos[k] = item0 + 32u * k;
+    for (int k = 0; k < Items; ++k) {
+        pos[k] = cta * kTile + item0 + 32u * k;
         key[k] = pos[k] < a.n ? keyOfToken<Tok>(a, pos[k]) : kNoKey;
     }
-    const uint32_t top = a.shift;  // the bits that tell the rows apart
-    for (uint32_t shift = 0; shift < top; shift += a.digitBits) {
-#pragma unroll
-        for (int k = 0; k < kSortItems; ++k)
-            digit[k] = (key[k] >> shift) & (a.bins - 1u);
-        uint32_t total = 0, all = 0;
-        rankTile(digit, rank, total, a.bins, s);
-        const uint32_t base = blockExclusiveSum(total, all, s.scan);
+    for (uint32_t shift = 0; shift < a.bits; shift += a.digitBits) {
+        const uint32_t mine = rankItems<kClusterWarps, Items>(key, shift, rank, a.bins, count);
         if (threadIdx.x < a.bins)
-            s.base[threadIdx.x] = base;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kSortItems; ++k) {
-            const uint32_t to = s.base[digit[k]] + rank[k];
-            keyAt[to] = key[k];
-            posAt[to] = pos[k];
+            tileCount[threadIdx.x] = mine;
+        cluster.sync();
+        uint32_t before = 0, total = 0, all = 0;
+        if (threadIdx.x < a.bins) {
+            for (uint32_t c = 0; c < ctas; ++c) {
+                const uint32_t v = cluster.map_shared_rank(tileCount, c)[threadIdx.x];
+                total += v;
+                before += c < cta ? v : 0u;
+            }
         }
+        const uint32_t lower = blockExclusiveSum(total, all, scan);
+        if (threadIdx.x < a.bins)
+            base[threadIdx.x] = lower + before;
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kSortItems; ++k) {
-            key[k] = keyAt[item0 + 32u * k];
-            pos[k] = posAt[item0 + 32u * k];
+        for (int k = 0; k < Items; ++k) {
+            const uint32_t to = base[(key[k] >> shift) & (a.bins - 1u)] + rank[k];
+            cluster.map_shared_rank(at, to / kTile)[to % kTile] = (uint64_t(pos[k]) << 32) | key[k];
+        }
+        cluster.sync();
+#pragma unroll
+        for (int k = 0; k < Items; ++k) {
+            const uint64_t v = at[item0 + 32u * k];
+            key[k] = uint32_t(v);
+            pos[k] = uint32_t(v >> 32);
         }
     }
 #pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t i = item0 + 32u * k;
+    for (int k = 0; k < Items; ++k) {
+        const uint32_t i = cta * kTile + item0 + 32u * k;
+        const uint32_t left = __shfl_up_sync(kFull, key[k], 1);
         if (i < a.n) {
             a.keyOut[i] = key[k];
             a.posOut[i] = pos[k];
+            // cleared before the passes, whose barriers order that before this
+            if (a.present != nullptr && key[k] < uint32_t(a.rows) && (lane == 0 || left != key[k]))
+                atomicOr(a.present + (key[k] >> 5), 1u << (key[k] & 31u));
         }
     }
 }
+
+// ---- any number: a kernel a pass
+
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortItems = 8;
+constexpr uint32_t kSortTile = uint32_t(kSortThreads) * kSortItems;  // 4096 keys
 
 /** A tile's digit counts of the first pass, and the rows that have a token. */
 template <class Tok>
@@ -317,18 +334,22 @@ __global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
     if (threadIdx.x < a.bins)
         count[threadIdx.x] = 0;
     __syncthreads();
+    uint32_t key[kSortItems], word[kSortItems];
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const uint32_t i = blockIdx.x * kSortTile + uint32_t(k) * kSortThreads + threadIdx.x;
-        if (i < a.n) {
-            const uint32_t key = keyOfToken<Tok>(a, i);
-            atomicAdd(count + (key & (a.bins - 1u)), 1u);
-            if (a.present != nullptr && key < uint32_t(a.rows)) {
-                const uint32_t bit = 1u << (key & 31u);
-                if ((*const_cast<volatile uint32_t*>(a.present + (key >> 5)) & bit) == 0)  // a frequent id: once
-                    atomicOr(a.present + (key >> 5), bit);
-            }
-        }
+        key[k] = i < a.n ? keyOfToken<Tok>(a, i) : kNoKey;
+    }
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k)
+        word[k] = a.present != nullptr && key[k] < uint32_t(a.rows) ? __ldcg(a.present + (key[k] >> 5)) : ~0u;
+#pragma unroll
+    for (int k = 0; k < kSortItems; ++k) {
+        if (key[k] != kNoKey)
+            atomicAdd(count + (key[k] & (a.bins - 1u)), 1u);
+        const uint32_t bit = 1u << (key[k] & 31u);
+        if ((word[k] & bit) == 0)  // a frequent id's bit is mostly seen set
+            atomicOr(a.present + (key[k] >> 5), bit);
     }
     __syncthreads();
     if (threadIdx.x < a.bins)
@@ -340,11 +361,11 @@ __global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
 template <bool First, class Tok>
 __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
 {
-    extern __shared__ __align__(16) unsigned char raw[];
-    SortShared& s = *reinterpret_cast<SortShared*>(raw);
+    __shared__ uint16_t count[kSortWarps * kMaxBins];
+    __shared__ uint32_t base[kMaxBins], scan[33];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t item0 = blockIdx.x * kSortTile + warp * (32u * kSortItems) + lane;
-    uint32_t key[kSortItems], pos[kSortItems], digit[kSortItems], rank[kSortItems];
+    uint32_t key[kSortItems], pos[kSortItems], rank[kSortItems];
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const uint32_t i = item0 + 32u * k;
@@ -355,34 +376,35 @@ __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
             if (!First)
                 pos[k] = a.posIn[i];
         }
-        digit[k] = (key[k] >> a.shift) & (a.bins - 1u);
     }
-    uint32_t before = 0, total = 0;
+    uint32_t before = 0, total = 0, all = 0;
     if (threadIdx.x < a.bins) {
         const uint32_t* column = a.hist + threadIdx.x;
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t t = 0; t < a.tiles; ++t) {
             const uint32_t c = __ldcg(column + size_t(t) * a.bins);
             total += c;
             before += t < blockIdx.x ? c : 0u;
         }
     }
-    uint32_t all = 0, own = 0;
-    const uint32_t base = blockExclusiveSum(total, all, s.scan) + before;
-    rankTile(digit, rank, own, a.bins, s);
+    const uint32_t lower = blockExclusiveSum(total, all, scan);
     if (threadIdx.x < a.bins)
-        s.base[threadIdx.x] = base;
-    __syncthreads();
+        base[threadIdx.x] = lower + before;
+    (void)rankItems<kSortWarps, kSortItems>(key, a.shift, rank, a.bins, count);  // its barriers publish base
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
-        if (item0 + 32u * k < a.n) {
-            const uint32_t to = s.base[digit[k]] + rank[k];
+        const bool in = item0 + 32u * k < a.n;
+        const uint32_t to = base[(key[k] >> a.shift) & (a.bins - 1u)] + rank[k];
+        if (in) {
             a.keyOut[to] = key[k];
             a.posOut[to] = pos[k];
-            if (a.nextHist != nullptr)
-                atomicAdd(a.nextHist + size_t(to / kSortTile) * a.bins
-                        + ((key[k] >> (a.shift + a.digitBits)) & (a.bins - 1u)),
-                    1u);
+        }
+        if (a.nextHist != nullptr) {
+            // a frequent id's keys fall on one count: added together within the warp
+            const uint32_t next = (to / kSortTile) * a.bins + ((key[k] >> (a.shift + a.digitBits)) & (a.bins - 1u));
+            const uint32_t peers = __match_any_sync(kFull, in ? next : kNoKey);
+            if (in && lane == uint32_t(__ffs(peers)) - 1u)
+                atomicAdd(a.nextHist + next, uint32_t(__popc(peers)));
         }
     }
 }
@@ -392,21 +414,50 @@ __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
 constexpr int kSumThreads = 256;
 constexpr uint32_t kRowsInFlight = 8;
 
-/** Columns of a piece: N neighbours (Wide: one 16-byte load of the values), or N columns
- *  ``group`` apart, element by element, for rows of odd length, alignment or stride. */
-template <bool Wide, int N>
+/** How a lane's N columns lie: neighbours read as one aligned 16-byte word; neighbours in a
+ *  16-byte word of any alignment; or ``group`` apart, element by element, for values whose
+ *  last stride is not 1. */
+enum class Piece { Aligned, Shifted, Strided };
+
+template <Piece P, int N>
 __device__ __forceinline__ uint32_t columnOf(const GradArgs& a, uint32_t slice, uint32_t lane, int e)
 {
-    return Wide ? (slice * a.group + lane) * N + e : (slice * N + e) * a.group + lane;
+    return P == Piece::Strided ? (slice * N + e) * a.group + lane : (slice * a.group + lane) * N + e;
 }
 
-template <class In, class Out, bool Wide, int N>
+/** 16 bytes from any address of whole elements, of which ``valid`` bytes are wanted: the one or
+ *  two aligned words that hold them (each holds a wanted byte, so it lies in mapped memory),
+ *  shifted together. What lies past ``valid`` is unspecified. */
+__device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
+    const uint32_t skip = uint32_t(at) & 15u;
+    const uint4 lo = __ldg(word);
+    const uint4 hi = skip + valid > 16u ? __ldg(word + 1) : make_uint4(0u, 0u, 0u, 0u);
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (skip & 8u) {
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+            w[j] = w[j + 2];
+    }
+    if (skip & 4u) {
+#pragma unroll
+        for (int j = 0; j < 5; ++j)
+            w[j] = w[j + 1];
+    }
+    const uint32_t shift = (skip & 3u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
+        __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
+}
+
+template <class In, class Out, Piece P, int N>
 __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32_t slice, uint32_t lane,
     const float (&acc)[N])
 {
     Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
-    if constexpr (Wide) {
-        Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + columnOf<true, N>(a, slice, lane, 0));
+    if constexpr (P == Piece::Aligned) {
+        Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + columnOf<P, N>(a, slice, lane, 0));
         Pack<Out, N> p;
         if (a.accumulate)
             p = *at;
@@ -417,125 +468,196 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const uint32_t col = columnOf<false, N>(a, slice, lane, e);
+            const uint32_t col = columnOf<P, N>(a, slice, lane, e);
             if (col < a.dim)
                 out[col] = fromFloat<Out>(a.accumulate ? toFloat(out[col]) + a.scale * acc[e] : a.scale * acc[e]);
         }
     }
 }
 
-template <bool Wide, int N>
+template <Piece P, int N>
 __device__ __forceinline__ void storePartial(const GradArgs& a, float* to, uint32_t chunk, uint32_t slice,
     uint32_t lane, const float (&acc)[N])
 {
     float* row = to + size_t(chunk) * a.width;
-    if constexpr (Wide) {
+    if constexpr (P != Piece::Strided) {
 #pragma unroll
         for (int e = 0; e < N; e += 4)
-            *reinterpret_cast<float4*>(row + columnOf<true, N>(a, slice, lane, e)) =
+            *reinterpret_cast<float4*>(row + columnOf<P, N>(a, slice, lane, e)) =
                 make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const uint32_t col = columnOf<false, N>(a, slice, lane, e);
+            const uint32_t col = columnOf<P, N>(a, slice, lane, e);
             if (col < a.dim)
                 row[col] = acc[e];
         }
     }
 }
 
-/** The runs of one chunk of the sorted order, by the lanes owning one slice of the columns;
- *  the CTAs past ``sumBlocks`` zero rows. */
-template <class In, class Out, bool Wide, int N>
+/** Eight neighbours of an array of ``n`` from ``i`` (a multiple of 8) on; ``other`` past its end. */
+__device__ __forceinline__ void loadEight(uint32_t (&v)[kRowsInFlight], const uint32_t* from, uint32_t i, uint32_t n,
+    uint32_t other)
+{
+    if (i < n && n - i >= 8u) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(from + i));
+        const uint4 y = __ldg(reinterpret_cast<const uint4*>(from + i) + 1);
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+#pragma unroll
+        for (uint32_t u = 0; u < kRowsInFlight; ++u)
+            v[u] = i < n && u < n - i ? __ldg(from + i + u) : other;
+    }
+}
+
+/** The runs that start in one chunk of the sorted order, by the lanes owning one slice of the
+ *  columns; the CTAs past ``sumBlocks`` zero rows.
+ *
+ *  A run is long if two or more chunks begin inside it. A run that is not long is summed whole
+ *  by the chunk it starts in, up to a chunk's length past its end, and skipped by the next. A
+ *  long one leaves a partial in every chunk it touches. Which it is follows from the first keys
+ *  of the neighbouring chunks, so both sides of a boundary agree. The next eight ids and
+ *  positions are on their way while eight rows are. */
+template <class In, class Out, Piece P, int N>
 __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
 {
     if (blockIdx.x >= a.sumBlocks) {
-        for (int64_t row0 = int64_t(blockIdx.x - a.sumBlocks) * a.zeroRows; row0 < a.rows;
-             row0 += int64_t(gridDim.x - a.sumBlocks) * a.zeroRows)
-            zeroAbsent<Out>(a, a.present, 0u, uint32_t(row0), uint32_t(min(row0 + int64_t(a.zeroRows), a.rows)));
+        const uint32_t warp = threadIdx.x >> 5;
+        for (int64_t r = int64_t(a.zeroed) + int64_t(blockIdx.x - a.sumBlocks) * (kSumThreads / 32) + warp; r < a.rows;
+             r += int64_t(gridDim.x - a.sumBlocks) * (kSumThreads / 32))
+            if (((__ldg(a.present + (r >> 5)) >> (r & 31)) & 1u) == 0)
+                zeroRow(a, r);
         return;
     }
     const uint64_t id = uint64_t(blockIdx.x) * kSumThreads + threadIdx.x;
     const uint32_t lane = uint32_t(id) & (a.group - 1u);
     const uint64_t which = id / a.group;  // a power of two
     const uint32_t chunk = uint32_t(which / a.slices), slice = uint32_t(which % a.slices);
-    if (chunk >= a.chunks || (Wide && slice * a.group + lane >= a.pieces))
+    if (chunk >= a.chunks || (P != Piece::Strided && slice * a.group + lane >= a.pieces))
         return;
     const uint32_t begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
     const uint32_t none = uint32_t(a.rows);
     const In* values = reinterpret_cast<const In*>(a.values);
-    uint32_t current = __ldg(a.keys + begin);
-    if (current == none)
+    const uint32_t col0 = columnOf<P, N>(a, slice, lane, 0);
+    // the first key of the d-th chunk from this one
+    auto firstKey = [&](int d) {
+        const int64_t i = (int64_t(chunk) + d) * a.chunk;
+        return i >= 0 && i < int64_t(a.n) ? __ldg(a.keys + i) : kNoKey;
+    };
+    uint32_t key[kRowsInFlight], token[kRowsInFlight];
+    loadEight(key, a.keys, begin, a.n, kNoKey);
+    loadEight(token, a.order, begin, a.n, 0u);
+    const uint32_t first = key[0];
+    if (first >= none)
         return;
-    bool fromBefore = begin > 0 && __ldg(a.keys + begin - 1) == current;
+    uint32_t current = first, skipped = kNoKey;
+    bool fromBefore = false;
+    if (begin > 0 && __ldg(a.keys + begin - 1) == first) {
+        if (firstKey(-1) == first || firstKey(1) == first) {
+            fromBefore = true;
+        } else {
+            skipped = first;
+            current = kNoKey;  // no run yet
+        }
+    }
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e)
         acc[e] = 0.0f;
-    for (uint32_t i0 = begin; i0 < end && current != none; i0 += kRowsInFlight) {
-        uint32_t key[kRowsInFlight];
-        Pack<In, N> got[kRowsInFlight];
-#pragma unroll
-        for (uint32_t u = 0; u < kRowsInFlight; ++u)
-            key[u] = i0 + u < end ? __ldg(a.keys + i0 + u) : kNoKey;
+    uint32_t stop = end;
+    bool extending = false, done = false;
+    for (uint32_t i0 = begin; !done; i0 += kRowsInFlight) {
+        if (i0 >= stop) {
+            if (extending || current == kNoKey || end == a.n || __ldg(a.keys + end) != current)
+                break;
+            if (fromBefore)
+                break;
+            if (first == current && skipped == kNoKey)  // it starts with the chunk: the second chunk to begin in it
+                break;
+            if (firstKey(2) == current)
+                break;
+            extending = true;
+            stop = a.n - end < a.chunk ? a.n : end + a.chunk;
+        }
+        uint4 got[kRowsInFlight];
+        float apart[kRowsInFlight][P == Piece::Strided ? N : 1];
 #pragma unroll
         for (uint32_t u = 0; u < kRowsInFlight; ++u) {
-            if (key[u] >= none)
+            if (key[u] >= none || key[u] == skipped || (extending && key[u] != current))
                 continue;
-            const uint32_t t = __ldg(a.order + i0 + u);
             int64_t at;
             if (a.flatValues) {
-                at = int64_t(t) * a.valueSeq;
+                at = int64_t(token[u]) * a.valueSeq;
             } else {
-                const uint32_t b = a.perBatch(t);
-                at = int64_t(b) * a.valueBatch + int64_t(t - b * a.perBatch.d) * a.valueSeq;
+                const uint32_t b = a.perBatch(token[u]);
+                at = int64_t(b) * a.valueBatch + int64_t(token[u] - b * a.perBatch.d) * a.valueSeq;
             }
-            if constexpr (Wide) {
-                got[u] = *reinterpret_cast<const Pack<In, N>*>(values + at + columnOf<true, N>(a, slice, lane, 0));
-            } else {
+            if constexpr (P == Piece::Aligned)
+                got[u] = __ldg(reinterpret_cast<const uint4*>(values + at + col0));
+            else if constexpr (P == Piece::Shifted)
+                got[u] = loadShifted(values + at + col0, min(uint32_t(N), a.dim - col0) * uint32_t(sizeof(In)));
+            else {
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const uint32_t col = columnOf<false, N>(a, slice, lane, e);
-                    if (col < a.dim)
-                        got[u].e[e] = values[at + int64_t(col) * a.valueDim];
-                    else
-                        got[u].e[e] = fromFloat<In>(0.0f);
+                    const uint32_t col = columnOf<P, N>(a, slice, lane, e);
+                    apart[u][e] = col < a.dim ? toFloat(values[at + int64_t(col) * a.valueDim]) : 0.0f;
                 }
             }
         }
+        uint32_t nextKey[kRowsInFlight], nextToken[kRowsInFlight];
+        loadEight(nextKey, a.keys, i0 + kRowsInFlight, a.n, kNoKey);
+        loadEight(nextToken, a.order, i0 + kRowsInFlight, a.n, 0u);
 #pragma unroll
         for (uint32_t u = 0; u < kRowsInFlight; ++u) {
-            if (key[u] == kNoKey)
-                break;
+            if (done || key[u] == skipped)
+                continue;
             if (key[u] != current) {
+                if (extending) {
+                    done = true;
+                    continue;
+                }
                 if (fromBefore)
-                    storePartial<Wide, N>(a, a.head, chunk, slice, lane, acc);
-                else
-                    storeRow<In, Out, Wide, N>(a, current, slice, lane, acc);
+                    storePartial<P, N>(a, a.head, chunk, slice, lane, acc);
+                else if (current != kNoKey)
+                    storeRow<In, Out, P, N>(a, current, slice, lane, acc);
                 fromBefore = false;
                 current = key[u];
+                if (current >= none) {  // padding, or the end
+                    current = kNoKey;
+                    done = true;
+                    continue;
+                }
 #pragma unroll
                 for (int e = 0; e < N; ++e)
                     acc[e] = 0.0f;
-                if (current == none)
-                    break;
             }
+            if constexpr (P == Piece::Strided) {
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                acc[e] += toFloat(got[u].e[e]);
+                for (int e = 0; e < N; ++e)
+                    acc[e] += apart[u][e];
+            } else {
+                const Pack<In, N> p = *reinterpret_cast<const Pack<In, N>*>(&got[u]);
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    acc[e] += toFloat(p.e[e]);
+            }
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kRowsInFlight; ++u) {
+            key[u] = nextKey[u];
+            token[u] = nextToken[u];
         }
     }
-    if (current == none)
+    if (current == kNoKey)
         return;
-    const bool goesOn = end < a.n && __ldg(a.keys + end) == current;
     if (fromBefore) {
-        storePartial<Wide, N>(a, a.head, chunk, slice, lane, acc);
-    } else if (goesOn) {
-        storePartial<Wide, N>(a, a.tail, chunk, slice, lane, acc);
+        storePartial<P, N>(a, a.head, chunk, slice, lane, acc);
+    } else if (!extending && end < a.n && __ldg(a.keys + end) == current) {
+        storePartial<P, N>(a, a.tail, chunk, slice, lane, acc);
         if (slice == 0 && lane == 0)
             a.list[atomicAdd(a.listCount, 1u)] = chunk;  // any order: every run is joined on its own
     } else {
-        storeRow<In, Out, Wide, N>(a, current, slice, lane, acc);
+        storeRow<In, Out, P, N>(a, current, slice, lane, acc);
     }
 }
 
@@ -543,8 +665,8 @@ constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr uint32_t kJoinColumns = 128;  // four per lane
 
-/** The rows whose runs cross chunks: eight warps each add a contiguous eighth of the run's
- *  partials in chunk order, then the eight sums are added in order. */
+/** The rows of long runs: eight warps each add a contiguous eighth of the run's partials in
+ *  chunk order, then the eight sums are added in order. */
 template <class Out>
 __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
 {
@@ -603,13 +725,11 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
 }
 
 /** No tokens: every row is zero. */
-template <class Out>
 __global__ __launch_bounds__(kSumThreads) void zeroRowsKernel(GradArgs a)
 {
-    const uint32_t nothing[1] = {0};
-    for (int64_t r = int64_t(blockIdx.x); r < a.rows; r += gridDim.x)
-        if (threadIdx.x < 32)
-            zeroAbsent<Out>(a, nothing, uint32_t(r), uint32_t(r), uint32_t(r) + 1u);
+    for (int64_t r = int64_t(blockIdx.x) * (kSumThreads / 32) + (threadIdx.x >> 5); r < a.rows;
+         r += int64_t(gridDim.x) * (kSumThreads / 32))
+        zeroRow(a, r);
 }
 
 // ------------------------------------------------------------------ host side
@@ -725,7 +845,8 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
 /** How the gradient's sort, sums and scratch are laid out. */
 struct GradPlan {
     uint32_t n = 0, bits = 0, passes = 0, digitBits = 0, bins = 0, tiles = 0;
-    bool wide = false;
+    bool cluster = false;  // sorted by one cluster
+    Piece piece = Piece::Strided;
     uint32_t pieces = 0, group = 0, slices = 0, chunk = 0, chunks = 0, width = 0;
     uint64_t present = 0, listCount = 0, hist = 0, zeroed = 0;  // offsets; [0, zeroed) is cleared
     uint64_t firstHist = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, head = 0, tail = 0, bytes = 0;
@@ -742,26 +863,31 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     p.passes = (p.bits + 8) / 9;
     p.digitBits = p.passes == 0 ? 0 : (p.bits + p.passes - 1) / p.passes;
     p.bins = 1u << p.digitBits;
+    p.cluster = p.n <= kClusterKeys;
     p.tiles = (p.n + kSortTile - 1) / kSortTile;
-    // 16-byte words of the values, if every vector and every row of the table starts on them
+    // whole 16-byte words if every vector and every row of the table starts on them
     const int pack = 16 / inBytes;
     const int64_t outWord = std::min(16, pack * outBytes);
-    p.wide = d.dim % pack == 0 && d.value_strides[2] == 1 && d.values % 16 == 0 && d.table % uint64_t(outWord) == 0
-        && d.value_strides[0] * inBytes % 16 == 0 && d.value_strides[1] * inBytes % 16 == 0
-        && d.table_stride * outBytes % outWord == 0;
-    p.pieces = p.wide ? uint32_t(d.dim / pack) : uint32_t((d.dim + 3) / 4);
+    if (d.value_strides[2] == 1 || d.dim <= 1)
+        p.piece = d.dim % pack == 0 && d.values % 16 == 0 && d.table % uint64_t(outWord) == 0
+                && d.value_strides[0] * inBytes % 16 == 0 && d.value_strides[1] * inBytes % 16 == 0
+                && d.table_stride * outBytes % outWord == 0
+            ? Piece::Aligned
+            : Piece::Shifted;
+    const int64_t columns = p.piece == Piece::Strided ? 4 : pack;
+    p.pieces = uint32_t((d.dim + columns - 1) / columns);
     p.group = 1;
     while (p.group < 32 && p.group < p.pieces)
         p.group *= 2;
     p.slices = (p.pieces + p.group - 1) / p.group;
     // the longest chunk that still leaves enough warps of 256 columns to hide the row loads: a
-    // longer one leaves fewer partials of runs that cross chunks. Of the sizes alone, not of
-    // types or alignment: it fixes the order of the sums, and the scratch the query asks for
+    // longer one leaves fewer partials of long runs. Of the sizes alone, not of types or
+    // alignment: it fixes the order of the sums, and the scratch the query asks for
     p.chunk = 8;
     while (p.chunk < 64 && uint64_t(p.n) * ((uint64_t(d.dim) + 255) / 256) / (p.chunk * 2) >= 4096)
         p.chunk *= 2;
     p.chunks = (p.n + p.chunk - 1) / p.chunk;
-    p.width = uint32_t(roundUp(uint64_t(d.dim), 4));
+    p.width = uint32_t(roundUp(uint64_t(d.dim), 8));
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t was = at;
@@ -770,11 +896,11 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     };
     p.present = take((uint64_t(d.rows) + 31) / 32 * 4);
     p.listCount = take(4);
-    const uint64_t histBytes = uint64_t(p.tiles) * p.bins * 4;
-    p.hist = take(p.tiles > 1 && p.passes > 1 ? histBytes * (p.passes - 1) : 0);
+    const uint64_t histBytes = p.cluster ? 0 : uint64_t(p.tiles) * p.bins * 4;
+    p.hist = take(p.passes > 1 ? histBytes * (p.passes - 1) : 0);
     p.zeroed = at;
-    p.firstHist = take(p.tiles > 1 ? histBytes : 0);
-    for (int k = 0; k < 2; ++k) {
+    p.firstHist = take(histBytes);
+    for (int k = 0; k < (p.cluster ? 1 : 2); ++k) {
         p.key[k] = take(uint64_t(p.n) * 4);
         p.pos[k] = take(uint64_t(p.n) * 4);
     }
@@ -785,13 +911,35 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     return p;
 }
 
-template <class In, class Out, bool Wide>
+template <class In, class Out, Piece P>
 void launchSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const char* who)
 {
-    constexpr int N = Wide ? 16 / int(sizeof(In)) : 4;
-    sumKernel<In, Out, Wide, N><<<blocks, kSumThreads, 0, s>>>(a);
+    constexpr int N = P == Piece::Strided ? 4 : 16 / int(sizeof(In));
+    sumKernel<In, Out, P, N><<<blocks, kSumThreads, 0, s>>>(a);
     launchCheck(who);
 }
+
+template <class Tok, int Items>
+void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaStream_t s, const char* who)
+{
+    auto kernel = clusterSortKernel<Tok, Items>;
+    const size_t shared = size_t(kClusterThreads) * Items * 8 + size_t(kClusterWarps) * kMaxBins * 2;
+    cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim = {ctas, 1, 1};
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks, 1, 1);
+    config.blockDim = dim3(kClusterThreads, 1, 1);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    cudaCheck(cudaLaunchKernelEx(&config, kernel, a), who);
+}
+
+/** Bytes of rows that the SMs without part in a cluster's sort zero meanwhile. */
+constexpr int64_t kZeroedBesideSort = 32ll << 20;
 
 void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
 {
@@ -805,14 +953,13 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.first = d.first;
     a.tableStride = d.table_stride;
     a.dim = uint32_t(d.dim);
-    a.zeroWide = d.dim * outBytes % 16 == 0 && d.table % 16 == 0 && d.table_stride * outBytes % 16 == 0;
+    a.rowBytes = d.dim * outBytes;
+    a.strideBytes = d.table_stride * outBytes;
     const int64_t sms = smCount();
     if (p.n == 0) {
         if (!accumulate) {
-            withElement(d.table_type, [&](auto out) {
-                zeroRowsKernel<decltype(out)><<<gridOf(std::min<int64_t>(d.rows, sms * 32), who), 32, 0, s>>>(a);
-                launchCheck(who);
-            });
+            zeroRowsKernel<<<unsigned(std::min<int64_t>((d.rows + 7) / 8, sms * 8)), kSumThreads, 0, s>>>(a);
+            launchCheck(who);
         }
         return;
     }
@@ -834,6 +981,7 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.accumulate = accumulate;
     a.scale = float(d.scale);
     a.n = p.n;
+    a.bits = p.bits;
     a.tiles = p.tiles;
     a.bins = p.bins;
     a.digitBits = p.digitBits;
@@ -847,23 +995,35 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.head = reinterpret_cast<float*>(scratch + p.head);
     a.tail = reinterpret_cast<float*>(scratch + p.tail);
     a.width = p.width;
-    const bool oneTile = p.tiles == 1;
-    a.present = accumulate || oneTile ? nullptr : words(p.present);
-    if (oneTile) {
+    a.present = accumulate ? nullptr : words(p.present);
+    if (p.cluster) {
         a.keyOut = words(p.key[0]);
         a.posOut = words(p.pos[0]);
-        a.shift = p.bits;
-        // each zeroing CTA takes an equal share of the rows, at most what 8 KB of bits hold
-        a.zeroRows = uint32_t(std::min<int64_t>(65536, int64_t(roundUp(uint64_t((d.rows + 2 * sms - 1) / (2 * sms)), 32))));
-        const int64_t zeroing = accumulate ? 0 : std::min<int64_t>(2 * sms, (d.rows + a.zeroRows - 1) / a.zeroRows);
-        const size_t shared = sizeof(SortShared) + size_t(kSortTile) * 8;
-        withElement(d.table_type, [&](auto out) {
-            withIndex(d.token_type, [&](auto tok) {
-                auto kernel = sortTileKernel<decltype(out), decltype(tok)>;
-                cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
-                kernel<<<gridOf(1 + zeroing, who), kSortThreads, shared, s>>>(a);
-                launchCheck(who);
-            });
+        unsigned ctas = 1;
+        while (ctas < unsigned(kClusterSize) && ctas * unsigned(kClusterThreads) < p.n)
+            ctas *= 2;
+        // 1024 threads an SM: the SMs beside the cluster, in whole clusters
+        unsigned blocks = ctas;
+        if (!accumulate && a.rowBytes > 0) {
+            a.zeroed = uint32_t(std::min(d.rows, kZeroedBesideSort / a.rowBytes));
+            const int64_t want = (int64_t(a.zeroed) + kClusterWarps - 1) / kClusterWarps;
+            blocks += unsigned(std::min<int64_t>((want + ctas - 1) / ctas, sms / ctas - 1)) * ctas;
+            if (blocks == ctas)
+                a.zeroed = 0;
+        }
+        const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
+        withIndex(d.token_type, [&](auto tok) {
+            using Tok = decltype(tok);
+            if (perThread <= 1)
+                launchClusterSort<Tok, 1>(a, ctas, blocks, s, who);
+            else if (perThread <= 2)
+                launchClusterSort<Tok, 2>(a, ctas, blocks, s, who);
+            else if (perThread <= 4)
+                launchClusterSort<Tok, 4>(a, ctas, blocks, s, who);
+            else if (perThread <= 8)
+                launchClusterSort<Tok, 8>(a, ctas, blocks, s, who);
+            else
+                launchClusterSort<Tok, kClusterItems>(a, ctas, blocks, s, who);
         });
         a.keys = a.keyOut;
         a.order = a.posOut;
@@ -884,32 +1044,35 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
                 b.keyOut = words(p.key[k & 1]);
                 b.posOut = words(p.pos[k & 1]);
                 if (k == 0)
-                    passKernel<true, Tok><<<p.tiles, kSortThreads, sizeof(SortShared), s>>>(b);
+                    passKernel<true, Tok><<<p.tiles, kSortThreads, 0, s>>>(b);
                 else
-                    passKernel<false, Tok><<<p.tiles, kSortThreads, sizeof(SortShared), s>>>(b);
+                    passKernel<false, Tok><<<p.tiles, kSortThreads, 0, s>>>(b);
                 launchCheck(who);
             }
         });
         a.keys = words(p.key[(p.passes + 1) & 1]);
         a.order = words(p.pos[(p.passes + 1) & 1]);
-        a.zeroRows = 32;
     }
     const uint64_t lanes = uint64_t(p.chunks) * p.slices * p.group;
     a.sumBlocks = gridOf(int64_t((lanes + kSumThreads - 1) / kSumThreads), who);
-    const int64_t zeroing = a.present == nullptr ? 0 : std::min<int64_t>(sms * 8, (d.rows + 31) / 32);
+    const int64_t zeroing = a.present == nullptr ? 0 : std::min<int64_t>(sms * 8, (d.rows - a.zeroed + 7) / 8);
     const unsigned blocks = gridOf(int64_t(a.sumBlocks) + zeroing, who);
     withElement(d.values_type, [&](auto in) {
         withElement(d.table_type, [&](auto out) {
-            if (p.wide)
-                launchSum<decltype(in), decltype(out), true>(a, blocks, s, who);
+            using In = decltype(in);
+            using Out = decltype(out);
+            if (p.piece == Piece::Aligned)
+                launchSum<In, Out, Piece::Aligned>(a, blocks, s, who);
+            else if (p.piece == Piece::Shifted)
+                launchSum<In, Out, Piece::Shifted>(a, blocks, s, who);
             else
-                launchSum<decltype(in), decltype(out), false>(a, blocks, s, who);
+                launchSum<In, Out, Piece::Strided>(a, blocks, s, who);
         });
     });
     if (p.chunks > 1) {
-        const int64_t items = int64_t(p.chunks - 1) * ((d.dim + kJoinColumns - 1) / kJoinColumns);
+        const int64_t items = int64_t(p.chunks / 2) * ((d.dim + kJoinColumns - 1) / kJoinColumns);
         withElement(d.table_type, [&](auto out) {
-            joinKernel<decltype(out)><<<gridOf(std::min<int64_t>(items, sms * 4), who), kJoinThreads, 0, s>>>(a);
+            joinKernel<decltype(out)><<<unsigned(std::min<int64_t>(items, sms * 8)), kJoinThreads, 0, s>>>(a);
             launchCheck(who);
         });
     }
