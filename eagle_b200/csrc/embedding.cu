@@ -25,6 +25,8 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <mutex>
+#include <vector>
 
 #define EB_API extern "C" __attribute__((visibility("default")))
 
@@ -111,6 +113,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
 // ------------------------------------------------------------------ gradient: sort
 
 constexpr uint32_t kMaxBins = 512;        // 9 bits a pass
+constexpr uint32_t kWarpParts = 32;       // partials of a run that one warp joins
 constexpr uint32_t kNoKey = 0xffffffffu;  // behind the last key: every digit of it is the highest
 
 struct GradArgs {
@@ -146,8 +149,9 @@ struct GradArgs {
     uint32_t slices;     // groups a row takes
     uint32_t pieces;     // packs (or columns) per row
     uint32_t sumBlocks;  // CTAs that sum; the others zero
-    uint32_t* listCount; // chunks whose last run is joined
-    uint32_t* list;
+    uint32_t* listCount; // {runs of up to kWarpParts partials, of more}
+    uint32_t* list;      // the chunks they start in
+    uint32_t* longList;
     float* head;         // [chunk][width]: the part of a long run that began in an earlier chunk
     float* tail;         // [chunk][width]: the part of a long run that goes on
     uint32_t width;      // dim rounded up to 8
@@ -156,18 +160,26 @@ struct GradArgs {
     uint32_t zeroed;     // rows [0, zeroed) are zeroed, with tokens or without, beside the sort
 };
 
-template <class Tok>
-__device__ __forceinline__ uint32_t keyOfToken(const GradArgs& a, uint32_t i)
+/** The keys of Items tokens, ``step`` apart from ``from`` on (kNoKey past the last). No branch
+ *  stands between the loads, so all are in flight together. */
+template <class Tok, int Items>
+__device__ __forceinline__ void loadKeys(const GradArgs& a, uint32_t from, uint32_t step, uint32_t (&key)[Items])
 {
-    int64_t at;
-    if (a.flatTokens) {
-        at = int64_t(i) * a.tokenSeq;
-    } else {
-        const uint32_t b = a.perBatch(i);
-        at = int64_t(b) * a.tokenBatch + int64_t(i - b * a.perBatch.d) * a.tokenSeq;
+    const Tok* tokens = reinterpret_cast<const Tok*>(a.tokens);
+    Tok id[Items];
+#pragma unroll
+    for (int k = 0; k < Items; ++k) {
+        const uint32_t i = min(from + uint32_t(k) * step, a.n - 1u);
+        const uint32_t b = a.flatTokens ? 0u : a.perBatch(i);
+        id[k] = __ldg(tokens + int64_t(b) * a.tokenBatch + int64_t(i - b * a.perBatch.d) * a.tokenSeq);
     }
-    const int64_t r = rowOfToken<Tok>(a.tokens, at, a.first, a.rows);
-    return r < 0 ? uint32_t(a.rows) : uint32_t(r);
+#pragma unroll
+    for (int k = 0; k < Items; ++k) {
+        const uint64_t r = uint64_t(int64_t(id[k])) - uint64_t(a.first);  // first >= 0: no wrap above it
+        key[k] = int64_t(id[k]) >= a.first && r < uint64_t(a.rows) ? uint32_t(r) : uint32_t(a.rows);
+        if (from + uint32_t(k) * step >= a.n)
+            key[k] = kNoKey;
+    }
 }
 
 /** One warp zeroes row ``r``: whole 16-byte words, and bytes two at a time before and after. */
@@ -190,30 +202,40 @@ __device__ __forceinline__ void zeroRow(const GradArgs& a, int64_t r)
         *reinterpret_cast<uint16_t*>(p) = 0;
 }
 
-/** The keys of one digit value before each item among a CTA's: items are ranked warp by
- *  warp, by match_any among the 32 of a step and by the warp's running counts between steps
- *  (item k of lane l is the warp's 32 k + l-th). ``count`` is [warp][bins], left scanned over
- *  the warps; bin threadIdx.x's sum is returned. */
+/** The keys of the same digit before each item among a CTA's: items are ranked warp by warp,
+ *  among the 32 of a step by their lanes and between steps by the warp's running counts
+ *  (item k of lane l is the warp's 32 k + l-th). The lanes of one digit find one another in a
+ *  word of shared memory, each setting its own bit: match_any takes about 7 cycles per
+ *  different value and warp (200 for random digits) and a ballot per bit 110, this 40.
+ *  ``count`` and ``peers`` are [warp][bins] of shared memory; count is left scanned over the
+ *  warps, and bin threadIdx.x's sum is returned. */
 template <int Warps, int Items>
-__device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint32_t shift, uint32_t (&rank)[Items],
-    uint32_t bins, uint16_t* count)
+__device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint32_t shift, uint32_t bits,
+    uint32_t (&rank)[Items], uint16_t* count, uint32_t* peers)
 {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, bins = 1u << bits;
+    __syncthreads();  // whoever still reads this memory
     uint32_t* words = reinterpret_cast<uint32_t*>(count);
     for (uint32_t i = threadIdx.x; i < Warps * bins / 2; i += Warps * 32)
         words[i] = 0;
+    for (uint32_t i = threadIdx.x; i < Warps * bins; i += Warps * 32)
+        peers[i] = 0;
     __syncthreads();
     uint16_t* mine = count + warp * bins;
+    uint32_t* same = peers + warp * bins;
 #pragma unroll
     for (int k = 0; k < Items; ++k) {
         const uint32_t digit = (key[k] >> shift) & (bins - 1u);
-        const uint32_t peers = __match_any_sync(kFull, digit);
-        const uint32_t before = mine[digit];
+        atomicOr(same + digit, 1u << lane);
         __syncwarp();
-        if (lane == uint32_t(__ffs(peers)) - 1u)
-            mine[digit] = uint16_t(before + __popc(peers));
+        const uint32_t lanes = same[digit], before = mine[digit];
         __syncwarp();
-        rank[k] = before + __popc(peers & ((1u << lane) - 1u));
+        if (lane == uint32_t(__ffs(lanes)) - 1u) {
+            mine[digit] = uint16_t(before + __popc(lanes));
+            same[digit] = 0;
+        }
+        __syncwarp();
+        rank[k] = before + __popc(lanes & ((1u << lane) - 1u));
     }
     __syncthreads();
     uint32_t total = 0;
@@ -236,19 +258,23 @@ __device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint
 
 constexpr int kClusterThreads = 1024;
 constexpr int kClusterWarps = kClusterThreads / 32;
-constexpr int kClusterSize = 8;
-constexpr int kClusterItems = 16;
+constexpr int kClusterSize = 16;  // past the portable 8: asked for only where more than 8 are needed
+constexpr int kClusterItems = 8;
 constexpr uint32_t kClusterKeys = uint32_t(kClusterThreads) * kClusterSize * kClusterItems;  // 131072
+constexpr uint32_t kPortableKeys = kClusterKeys / 2;
+constexpr uint32_t kPeerBytes = uint32_t(kClusterWarps) * kMaxBins * 4;
 
 /** Cluster 0 sorts: every CTA holds 1024 * Items neighbouring keys in registers; a pass ranks
- *  them, adds up the CTAs' digit counts over distributed shared memory and stores each key
- *  and position straight into the CTA that has its place, two cluster barriers in all. The
- *  other clusters meanwhile zero the first ``zeroed`` rows. */
+ *  them, puts them in digit order in the CTA's own shared memory, adds up the CTAs' digit
+ *  counts over distributed shared memory and stores each key and position into the CTA that
+ *  has its place, neighbours mostly to neighbours; two cluster barriers in all. The other
+ *  clusters meanwhile zero the first ``zeroed`` rows. */
 template <class Tok, int Items>
 __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ uint32_t tileCount[kMaxBins], base[kMaxBins], scan[33];
+    __shared__ uint32_t local[kMaxBins];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
@@ -258,30 +284,46 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
             zeroRow(a, r);
         return;
     }
-    uint64_t* at = reinterpret_cast<uint64_t*>(raw);  // key and position by place
-    uint16_t* count = reinterpret_cast<uint16_t*>(raw + size_t(kClusterThreads) * Items * 8);
     constexpr uint32_t kTile = uint32_t(kClusterThreads) * Items;
+    uint64_t* at = reinterpret_cast<uint64_t*>(raw);  // key and position by place in the order
+    uint64_t* own = at + kTile;                       // by place among the CTA's
+    // the lanes' words take the memory of ``own``, empty while they are in use, if that is enough
+    uint32_t* peers = reinterpret_cast<uint32_t*>(kTile * 8 >= kPeerBytes ? own : own + kTile);
+    uint16_t* count = reinterpret_cast<uint16_t*>(
+        reinterpret_cast<char*>(own) + (kTile * 8 >= kPeerBytes ? kTile * 8 : kTile * 8 + kPeerBytes));
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t item0 = warp * (32u * Items) + lane;
-    if (cta == 0 && threadIdx.x == 0)
-        *a.listCount = 0;
+    if (cta == 0 && threadIdx.x < 2)
+        a.listCount[threadIdx.x] = 0;
     if (a.present != nullptr)
         for (int64_t w = int64_t(cta) * kClusterThreads + threadIdx.x; w < (a.rows + 31) / 32;
              w += int64_t(ctas) * kClusterThreads)
             a.present[w] = 0;
     uint32_t key[Items], pos[Items], rank[Items];
+    loadKeys<Tok, Items>(a, cta * kTile + item0, 32u, key);
 #pragma unroll
-    for (int k = 0; k < Items; ++k) {
+    for (int k = 0; k < Items; ++k)
         pos[k] = cta * kTile + item0 + 32u * k;
-        key[k] = pos[k] < a.n ? keyOfToken<Tok>(a, pos[k]) : kNoKey;
-    }
     for (uint32_t shift = 0; shift < a.bits; shift += a.digitBits) {
-        const uint32_t mine = rankItems<kClusterWarps, Items>(key, shift, rank, a.bins, count);
-        if (threadIdx.x < a.bins)
-            tileCount[threadIdx.x] = mine;
-        cluster.sync();
-        uint32_t before = 0, total = 0, all = 0;
+        const uint32_t mine = rankItems<kClusterWarps, Items>(key, shift, a.digitBits, rank, count, peers);
+        uint32_t all = 0;
+        const uint32_t first = blockExclusiveSum(mine, all, scan);
         if (threadIdx.x < a.bins) {
+            tileCount[threadIdx.x] = mine;
+            local[threadIdx.x] = first;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < Items; ++k)
+            own[local[(key[k] >> shift) & (a.bins - 1u)] + rank[k]] = (uint64_t(pos[k]) << 32) | key[k];
+        const uint64_t* from = own;
+        if (ctas == 1) {
+            __syncthreads();
+        } else {
+        cluster.sync();
+        uint32_t before = 0, total = 0;
+        if (threadIdx.x < a.bins) {
+#pragma unroll 8
             for (uint32_t c = 0; c < ctas; ++c) {
                 const uint32_t v = cluster.map_shared_rank(tileCount, c)[threadIdx.x];
                 total += v;
@@ -290,17 +332,21 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
         }
         const uint32_t lower = blockExclusiveSum(total, all, scan);
         if (threadIdx.x < a.bins)
-            base[threadIdx.x] = lower + before;
+            base[threadIdx.x] = lower + before - first;  // from a place among the CTA's to one in the order
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < Items; ++k) {
-            const uint32_t to = base[(key[k] >> shift) & (a.bins - 1u)] + rank[k];
-            cluster.map_shared_rank(at, to / kTile)[to % kTile] = (uint64_t(pos[k]) << 32) | key[k];
+            const uint32_t j = uint32_t(k) * kClusterThreads + threadIdx.x;
+            const uint64_t v = own[j];
+            const uint32_t to = base[(uint32_t(v) >> shift) & (a.bins - 1u)] + j;
+            cluster.map_shared_rank(at, to / kTile)[to % kTile] = v;
         }
         cluster.sync();
+        from = at;
+        }
 #pragma unroll
         for (int k = 0; k < Items; ++k) {
-            const uint64_t v = at[item0 + 32u * k];
+            const uint64_t v = from[item0 + 32u * k];
             key[k] = uint32_t(v);
             pos[k] = uint32_t(v >> 32);
         }
@@ -335,11 +381,7 @@ __global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
         count[threadIdx.x] = 0;
     __syncthreads();
     uint32_t key[kSortItems], word[kSortItems];
-#pragma unroll
-    for (int k = 0; k < kSortItems; ++k) {
-        const uint32_t i = blockIdx.x * kSortTile + uint32_t(k) * kSortThreads + threadIdx.x;
-        key[k] = i < a.n ? keyOfToken<Tok>(a, i) : kNoKey;
-    }
+    loadKeys<Tok, kSortItems>(a, blockIdx.x * kSortTile + threadIdx.x, kSortThreads, key);
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k)
         word[k] = a.present != nullptr && key[k] < uint32_t(a.rows) ? __ldcg(a.present + (key[k] >> 5)) : ~0u;
@@ -361,20 +403,23 @@ __global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
 template <bool First, class Tok>
 __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
 {
-    __shared__ uint16_t count[kSortWarps * kMaxBins];
+    extern __shared__ __align__(16) unsigned char raw[];
+    uint32_t* peers = reinterpret_cast<uint32_t*>(raw);
+    uint16_t* count = reinterpret_cast<uint16_t*>(peers + kSortWarps * kMaxBins);
     __shared__ uint32_t base[kMaxBins], scan[33];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t item0 = blockIdx.x * kSortTile + warp * (32u * kSortItems) + lane;
     uint32_t key[kSortItems], pos[kSortItems], rank[kSortItems];
+    if constexpr (First)
+        loadKeys<Tok, kSortItems>(a, item0, 32u, key);
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const uint32_t i = item0 + 32u * k;
-        key[k] = kNoKey;
-        pos[k] = i;
-        if (i < a.n) {
-            key[k] = First ? keyOfToken<Tok>(a, i) : a.keyIn[i];
-            if (!First)
-                pos[k] = a.posIn[i];
+        if constexpr (First) {
+            pos[k] = i;
+        } else {
+            key[k] = i < a.n ? __ldcg(a.keyIn + i) : kNoKey;
+            pos[k] = i < a.n ? __ldcg(a.posIn + i) : 0u;
         }
     }
     uint32_t before = 0, total = 0, all = 0;
@@ -390,7 +435,7 @@ __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
     const uint32_t lower = blockExclusiveSum(total, all, scan);
     if (threadIdx.x < a.bins)
         base[threadIdx.x] = lower + before;
-    (void)rankItems<kSortWarps, kSortItems>(key, a.shift, rank, a.bins, count);  // its barriers publish base
+    (void)rankItems<kSortWarps, kSortItems>(key, a.shift, a.digitBits, rank, count, peers);  // its barriers publish base
 #pragma unroll
     for (int k = 0; k < kSortItems; ++k) {
         const bool in = item0 + 32u * k < a.n;
@@ -400,11 +445,13 @@ __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
             a.posOut[to] = pos[k];
         }
         if (a.nextHist != nullptr) {
-            // a frequent id's keys fall on one count: added together within the warp
-            const uint32_t next = (to / kSortTile) * a.bins + ((key[k] >> (a.shift + a.digitBits)) & (a.bins - 1u));
-            const uint32_t peers = __match_any_sync(kFull, in ? next : kNoKey);
-            if (in && lane == uint32_t(__ffs(peers)) - 1u)
-                atomicAdd(a.nextHist + next, uint32_t(__popc(peers)));
+            // a frequent id's keys fall on one count: neighbours with the same one add together
+            const uint32_t next =
+                in ? (to / kSortTile) * a.bins + ((key[k] >> (a.shift + a.digitBits)) & (a.bins - 1u)) : kNoKey;
+            const uint32_t lead = __shfl_sync(kFull, next, 0);
+            const uint32_t equal = __ballot_sync(kFull, next == lead);
+            if (in && (next != lead || lane == uint32_t(__ffs(equal)) - 1u))
+                atomicAdd(a.nextHist + next, next == lead ? uint32_t(__popc(equal)) : 1u);
         }
     }
 }
@@ -419,22 +466,9 @@ constexpr uint32_t kRowsInFlight = 8;
  *  last stride is not 1. */
 enum class Piece { Aligned, Shifted, Strided };
 
-template <Piece P, int N>
-__device__ __forceinline__ uint32_t columnOf(const GradArgs& a, uint32_t slice, uint32_t lane, int e)
+/** The 16 bytes ``skip`` into 32 neighbouring ones. */
+__device__ __forceinline__ uint4 shiftWords(uint4 lo, uint4 hi, uint32_t skip)
 {
-    return P == Piece::Strided ? (slice * N + e) * a.group + lane : (slice * a.group + lane) * N + e;
-}
-
-/** 16 bytes from any address of whole elements, of which ``valid`` bytes are wanted: the one or
- *  two aligned words that hold them (each holds a wanted byte, so it lies in mapped memory),
- *  shifted together. What lies past ``valid`` is unspecified. */
-__device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
-{
-    const uint64_t at = reinterpret_cast<uint64_t>(p);
-    const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
-    const uint32_t skip = uint32_t(at) & 15u;
-    const uint4 lo = __ldg(word);
-    const uint4 hi = skip + valid > 16u ? __ldg(word + 1) : make_uint4(0u, 0u, 0u, 0u);
     uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     if (skip & 8u) {
 #pragma unroll
@@ -451,13 +485,27 @@ __device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
         __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
 }
 
+/** 16 bytes from any address of whole elements, of which ``valid`` bytes are wanted: the one or
+ *  two aligned words that hold them (each holds a wanted byte, so it lies in mapped memory),
+ *  shifted together. What lies past ``valid`` is unspecified. */
+__device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
+    const uint32_t skip = uint32_t(at) & 15u;
+    const uint4 lo = __ldg(word);
+    const uint4 hi = skip + valid > 16u ? __ldg(word + 1) : make_uint4(0u, 0u, 0u, 0u);
+    return shiftWords(lo, hi, skip);
+}
+
+/** The columns ``col0``, ``col0 + apart``, ... of a row; ``apart`` is 1 but for Strided pieces. */
 template <class In, class Out, Piece P, int N>
-__device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32_t slice, uint32_t lane,
+__device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32_t col0, uint32_t apart,
     const float (&acc)[N])
 {
     Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
     if constexpr (P == Piece::Aligned) {
-        Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + columnOf<P, N>(a, slice, lane, 0));
+        Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + col0);
         Pack<Out, N> p;
         if (a.accumulate)
             p = *at;
@@ -468,7 +516,7 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const uint32_t col = columnOf<P, N>(a, slice, lane, e);
+            const uint32_t col = col0 + uint32_t(e) * apart;
             if (col < a.dim)
                 out[col] = fromFloat<Out>(a.accumulate ? toFloat(out[col]) + a.scale * acc[e] : a.scale * acc[e]);
         }
@@ -476,19 +524,19 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
 }
 
 template <Piece P, int N>
-__device__ __forceinline__ void storePartial(const GradArgs& a, float* to, uint32_t chunk, uint32_t slice,
-    uint32_t lane, const float (&acc)[N])
+__device__ __forceinline__ void storePartial(const GradArgs& a, float* to, uint32_t chunk, uint32_t col0,
+    uint32_t apart, const float (&acc)[N])
 {
     float* row = to + size_t(chunk) * a.width;
     if constexpr (P != Piece::Strided) {
 #pragma unroll
         for (int e = 0; e < N; e += 4)
-            *reinterpret_cast<float4*>(row + columnOf<P, N>(a, slice, lane, e)) =
+            *reinterpret_cast<float4*>(row + col0 + e) =
                 make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const uint32_t col = columnOf<P, N>(a, slice, lane, e);
+            const uint32_t col = col0 + uint32_t(e) * apart;
             if (col < a.dim)
                 row[col] = acc[e];
         }
@@ -510,23 +558,236 @@ __device__ __forceinline__ void loadEight(uint32_t (&v)[kRowsInFlight], const ui
     }
 }
 
-/** The runs that start in one chunk of the sorted order, by the lanes owning one slice of the
- *  columns; the CTAs past ``sumBlocks`` zero rows.
- *
- *  A run is long if two or more chunks begin inside it. A run that is not long is summed whole
- *  by the chunk it starts in, up to a chunk's length past its end, and skipped by the next. A
- *  long one leaves a partial in every chunk it touches. Which it is follows from the first keys
- *  of the neighbouring chunks, so both sides of a boundary agree. The next eight ids and
- *  positions are on their way while eight rows are. */
+/** The rows past ``zeroed`` that have no token, by the warps of the CTAs past ``sumBlocks``. */
+__device__ __forceinline__ void zeroAbsent(const GradArgs& a)
+{
+    const uint32_t warps = blockDim.x >> 5;
+    for (int64_t r = int64_t(a.zeroed) + int64_t(blockIdx.x - a.sumBlocks) * warps + (threadIdx.x >> 5); r < a.rows;
+         r += int64_t(gridDim.x - a.sumBlocks) * warps)
+        if (((__ldg(a.present + (r >> 5)) >> (r & 31)) & 1u) == 0)
+            zeroRow(a, r);
+}
+
+/** Element offset of token ``t``'s vector. */
+__device__ __forceinline__ int64_t vectorOf(const GradArgs& a, uint32_t t)
+{
+    if (a.flatValues)
+        return int64_t(t) * a.valueSeq;
+    const uint32_t b = a.perBatch(t);
+    return int64_t(b) * a.valueBatch + int64_t(t - b * a.perBatch.d) * a.valueSeq;
+}
+
+/** Chunk ``chunk``'s last run, of row ``key``, is one to join. In any order: each is joined on its own. */
+__device__ __forceinline__ void listRun(const GradArgs& a, uint32_t chunk, uint32_t key)
+{
+    const uint64_t past = (uint64_t(chunk) + kWarpParts) * a.chunk;  // the first of one partial too many
+    if (past < a.n && __ldg(a.keys + past) == key)
+        a.longList[atomicAdd(a.listCount + 1, 1u)] = chunk;
+    else
+        a.list[atomicAdd(a.listCount, 1u)] = chunk;
+}
+
+// The sorted order is cut into chunks. A run is long if two or more chunks begin inside it. A
+// run that is not long is summed whole by the chunk it starts in, up to a chunk's length past
+// its end, and skipped by the next. A long one leaves a partial in every chunk it touches.
+// Which it is follows from the first keys of the neighbouring chunks, so both sides of a
+// boundary agree.
+
+// ---- wide contiguous rows: the copy engine brings them into shared memory
+
+constexpr int kBulkLanes = 128;                   // threads that add, 16 bytes of a row each
+constexpr int kBulkThreads = kBulkLanes + 32;     // and a warp that asks for the rows
+constexpr uint32_t kBulkSlab = kBulkLanes * 16;   // bytes of a row per CTA
+constexpr uint32_t kBulkSlot = kBulkSlab + 16;    // a piece of any alignment, in whole words
+constexpr uint32_t kBulkRows = 4;                 // rows per barrier
+constexpr uint32_t kBulkStages = 4;
+constexpr uint32_t kMaxChunk = 64;
+constexpr int64_t kBulkLeast = 1024;  // bytes of a row
+constexpr uint32_t kBulkWaits = 1u << 22;  // polls before a wait gives up
+
+struct BulkShared {
+    alignas(16) unsigned char row[kBulkStages][kBulkRows][kBulkSlot];
+    uint64_t full[kBulkStages], empty[kBulkStages];
+    uint32_t key[2 * kMaxChunk + 1], token[2 * kMaxChunk];
+};
+
+__device__ __forceinline__ void mbarArrive(uint64_t* bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(sharedAddr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void mbarExpect(uint64_t* bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(sharedAddr(bar)), "r"(bytes)
+                 : "memory");
+}
+
+__device__ __forceinline__ void bulkCopy(void* dst, const void* src, uint32_t bytes, uint64_t* bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     sharedAddr(dst)),
+        "l"(src), "r"(bytes), "r"(sharedAddr(bar))
+        : "memory");
+}
+
+/** One CTA sums the runs that start in one chunk over 2 KB of the columns. A warp asks the copy
+ *  engine for the rows, up to 16 ahead and each as the whole 16-byte words that hold it; four
+ *  warps add them from shared memory. So the memory is kept busy whatever the adding
+ *  threads wait for: 24 warps and 130 KB in flight an SM. */
+template <class In, class Out, bool Aligned>
+__global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
+{
+    constexpr int N = 16 / int(sizeof(In));
+    constexpr Piece P = Aligned ? Piece::Aligned : Piece::Shifted;
+    extern __shared__ __align__(16) unsigned char raw[];
+    if (blockIdx.x >= a.sumBlocks) {
+        zeroAbsent(a);
+        return;
+    }
+    BulkShared& s = *reinterpret_cast<BulkShared*>(raw);
+    const uint32_t chunk = blockIdx.x / a.slices, slab = blockIdx.x - chunk * a.slices;
+    const uint32_t begin = chunk * a.chunk, size = a.chunk, none = uint32_t(a.rows);
+    const uint32_t len = min(size, a.n - begin);
+    for (uint32_t i = threadIdx.x; i <= 2 * size; i += kBulkThreads) {
+        const bool in = i < a.n - begin;
+        s.key[i] = in ? __ldg(a.keys + begin + i) : kNoKey;
+        if (i < 2 * size)
+            s.token[i] = in ? __ldg(a.order + begin + i) : 0u;
+    }
+    const uint32_t left = begin > 0 ? __ldg(a.keys + begin - 1) : kNoKey;
+    const uint32_t before = begin > 0 ? __ldg(a.keys + begin - size) : kNoKey;  // the chunk before's first
+    if (threadIdx.x == 0) {
+        for (uint32_t k = 0; k < kBulkStages; ++k) {
+            mbarInit(&s.full[k], 1);
+            mbarInit(&s.empty[k], kBulkLanes / 32);
+        }
+    }
+    __syncthreads();
+    const uint32_t i = threadIdx.x, first = s.key[0];
+    if (first >= none)
+        return;
+    // the rows [r0, r1) of the chunk and the next that are summed here
+    const bool continued = begin > 0 && left == first;
+    const bool fromBefore = continued && (before == first || s.key[size] == first);
+    const uint32_t leading = uint32_t(__syncthreads_count(i < len && s.key[i] == first));
+    const uint32_t valid = uint32_t(__syncthreads_count(i < len && s.key[i] < none));
+    const uint32_t r0 = continued && !fromBefore ? leading : 0u;
+    if (r0 >= valid)
+        return;
+    const uint32_t last = s.key[valid - 1];
+    const bool goesOn = valid == size && s.key[size] == last;
+    const bool joined = goesOn && ((last == first && (!continued || fromBefore)) || s.key[2 * size] == last);
+    const uint32_t extra = uint32_t(__syncthreads_count(i < size && s.key[size + i] == last));
+    const uint32_t r1 = goesOn && !joined ? size + extra : valid;
+
+    const In* values = reinterpret_cast<const In*>(a.values);
+    const uint32_t slab0 = slab * (kBulkSlab / uint32_t(sizeof(In)));  // its first column
+    const uint32_t bytes = min(kBulkSlab, (a.dim - slab0) * uint32_t(sizeof(In)));
+    const uint32_t steps = (r1 - r0 + kBulkRows - 1) / kBulkRows;
+    if (threadIdx.x >= kBulkLanes) {
+        if (threadIdx.x == kBulkLanes) {
+            for (uint32_t j = 0; j < steps; ++j) {
+                const uint32_t stage = j % kBulkStages;
+                if (j >= kBulkStages && !mbarWait(&s.empty[stage], (j / kBulkStages - 1) & 1u, kBulkWaits))
+                    return;  // the adding warps gave up; they wait for what was asked for
+                const uint32_t rows = min(kBulkRows, r1 - r0 - j * kBulkRows);
+                const char* from[kBulkRows];
+                uint32_t size_[kBulkRows], sum = 0;
+#pragma unroll
+                for (uint32_t u = 0; u < kBulkRows; ++u) {
+                    if (u >= rows)
+                        break;
+                    const uint64_t p =
+                        reinterpret_cast<uint64_t>(values + vectorOf(a, s.token[r0 + j * kBulkRows + u]) + slab0);
+                    from[u] = reinterpret_cast<const char*>(p & ~uint64_t(15));
+                    size_[u] = Aligned ? bytes : (uint32_t(p & 15u) + bytes + 15u) & ~15u;
+                    sum += size_[u];
+                }
+                mbarExpect(&s.full[stage], sum);
+#pragma unroll
+                for (uint32_t u = 0; u < kBulkRows; ++u)
+                    if (u < rows)
+                        bulkCopy(s.row[stage][u], from[u], size_[u], &s.full[stage]);
+            }
+        }
+        return;
+    }
+    const uint32_t col0 = slab0 + threadIdx.x * N;
+    const bool active = col0 < a.dim;
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        acc[e] = 0.0f;
+    uint32_t current = s.key[r0];
+    bool partial = fromBefore;  // the run being summed began before: its sum is the chunk's head
+    for (uint32_t j = 0; j < steps; ++j) {
+        const uint32_t stage = j % kBulkStages, parity = (j / kBulkStages) & 1u;
+        if (!mbarWait(&s.full[stage], parity, kBulkWaits) && !mbarWait(&s.full[stage], parity, kBulkWaits)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                acc[e] = __int_as_float(0x7fc00000);  // rows that never came show
+        }
+        const uint32_t rows = min(kBulkRows, r1 - r0 - j * kBulkRows);
+#pragma unroll
+        for (uint32_t u = 0; u < kBulkRows; ++u) {
+            if (u >= rows)
+                break;
+            const uint32_t key = s.key[r0 + j * kBulkRows + u];
+            if (key != current) {
+                if (active) {
+                    if (partial)
+                        storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
+                    else
+                        storeRow<In, Out, P, N>(a, current, col0, 1u, acc);
+                }
+                partial = false;
+                current = key;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    acc[e] = 0.0f;
+            }
+            if (active) {
+                uint4 w;
+                if constexpr (Aligned) {
+                    w = *reinterpret_cast<const uint4*>(s.row[stage][u] + threadIdx.x * 16);
+                } else {
+                    const uint64_t p =
+                        reinterpret_cast<uint64_t>(values + vectorOf(a, s.token[r0 + j * kBulkRows + u]) + slab0);
+                    const uint4* at = reinterpret_cast<const uint4*>(s.row[stage][u] + threadIdx.x * 16);
+                    w = shiftWords(at[0], at[1], uint32_t(p) & 15u);
+                }
+                const Pack<In, N> v = *reinterpret_cast<const Pack<In, N>*>(&w);
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    acc[e] += toFloat(v.e[e]);
+            }
+        }
+        __syncwarp();
+        if ((threadIdx.x & 31u) == 0)
+            mbarArrive(&s.empty[stage]);
+    }
+    if (!active)
+        return;
+    if (partial) {
+        storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
+    } else if (joined) {
+        storePartial<P, N>(a, a.tail, chunk, col0, 1u, acc);
+        if (slab == 0 && threadIdx.x == 0)
+            listRun(a, chunk, current);
+    } else {
+        storeRow<In, Out, P, N>(a, current, col0, 1u, acc);
+    }
+}
+
+// ---- narrow or strided rows: loads into registers
+
+/** A chunk by the lanes owning one slice of the columns; the next eight ids and positions are on
+ *  their way while eight rows are. */
 template <class In, class Out, Piece P, int N>
 __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
 {
     if (blockIdx.x >= a.sumBlocks) {
-        const uint32_t warp = threadIdx.x >> 5;
-        for (int64_t r = int64_t(a.zeroed) + int64_t(blockIdx.x - a.sumBlocks) * (kSumThreads / 32) + warp; r < a.rows;
-             r += int64_t(gridDim.x - a.sumBlocks) * (kSumThreads / 32))
-            if (((__ldg(a.present + (r >> 5)) >> (r & 31)) & 1u) == 0)
-                zeroRow(a, r);
+        zeroAbsent(a);
         return;
     }
     const uint64_t id = uint64_t(blockIdx.x) * kSumThreads + threadIdx.x;
@@ -538,7 +799,8 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
     const uint32_t begin = chunk * a.chunk, end = min(begin + a.chunk, a.n);
     const uint32_t none = uint32_t(a.rows);
     const In* values = reinterpret_cast<const In*>(a.values);
-    const uint32_t col0 = columnOf<P, N>(a, slice, lane, 0);
+    const uint32_t apart = P == Piece::Strided ? a.group : 1u;
+    const uint32_t col0 = P == Piece::Strided ? slice * N * a.group + lane : (slice * a.group + lane) * N;
     // the first key of the d-th chunk from this one
     auto firstKey = [&](int d) {
         const int64_t i = (int64_t(chunk) + d) * a.chunk;
@@ -580,18 +842,12 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
             stop = a.n - end < a.chunk ? a.n : end + a.chunk;
         }
         uint4 got[kRowsInFlight];
-        float apart[kRowsInFlight][P == Piece::Strided ? N : 1];
+        float loose[kRowsInFlight][P == Piece::Strided ? N : 1];
 #pragma unroll
         for (uint32_t u = 0; u < kRowsInFlight; ++u) {
             if (key[u] >= none || key[u] == skipped || (extending && key[u] != current))
                 continue;
-            int64_t at;
-            if (a.flatValues) {
-                at = int64_t(token[u]) * a.valueSeq;
-            } else {
-                const uint32_t b = a.perBatch(token[u]);
-                at = int64_t(b) * a.valueBatch + int64_t(token[u] - b * a.perBatch.d) * a.valueSeq;
-            }
+            const int64_t at = vectorOf(a, token[u]);
             if constexpr (P == Piece::Aligned)
                 got[u] = __ldg(reinterpret_cast<const uint4*>(values + at + col0));
             else if constexpr (P == Piece::Shifted)
@@ -599,8 +855,8 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
             else {
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    const uint32_t col = columnOf<P, N>(a, slice, lane, e);
-                    apart[u][e] = col < a.dim ? toFloat(values[at + int64_t(col) * a.valueDim]) : 0.0f;
+                    const uint32_t col = col0 + uint32_t(e) * apart;
+                    loose[u][e] = col < a.dim ? toFloat(values[at + int64_t(col) * a.valueDim]) : 0.0f;
                 }
             }
         }
@@ -617,9 +873,9 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
                     continue;
                 }
                 if (fromBefore)
-                    storePartial<P, N>(a, a.head, chunk, slice, lane, acc);
+                    storePartial<P, N>(a, a.head, chunk, col0, apart, acc);
                 else if (current != kNoKey)
-                    storeRow<In, Out, P, N>(a, current, slice, lane, acc);
+                    storeRow<In, Out, P, N>(a, current, col0, apart, acc);
                 fromBefore = false;
                 current = key[u];
                 if (current >= none) {  // padding, or the end
@@ -634,7 +890,7 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
             if constexpr (P == Piece::Strided) {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    acc[e] += apart[u][e];
+                    acc[e] += loose[u][e];
             } else {
                 const Pack<In, N> p = *reinterpret_cast<const Pack<In, N>*>(&got[u]);
 #pragma unroll
@@ -651,59 +907,100 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
     if (current == kNoKey)
         return;
     if (fromBefore) {
-        storePartial<P, N>(a, a.head, chunk, slice, lane, acc);
+        storePartial<P, N>(a, a.head, chunk, col0, apart, acc);
     } else if (!extending && end < a.n && __ldg(a.keys + end) == current) {
-        storePartial<P, N>(a, a.tail, chunk, slice, lane, acc);
+        storePartial<P, N>(a, a.tail, chunk, col0, apart, acc);
         if (slice == 0 && lane == 0)
-            a.list[atomicAdd(a.listCount, 1u)] = chunk;  // any order: every run is joined on its own
+            listRun(a, chunk, current);
     } else {
-        storeRow<In, Out, P, N>(a, current, slice, lane, acc);
+        storeRow<In, Out, P, N>(a, current, col0, apart, acc);
     }
 }
+
+// ---- the rows of long runs
 
 constexpr int kJoinThreads = 256;
 constexpr int kJoinWarps = kJoinThreads / 32;
 constexpr uint32_t kJoinColumns = 128;  // four per lane
 
-/** The rows of long runs: eight warps each add a contiguous eighth of the run's partials in
- *  chunk order, then the eight sums are added in order. */
+/** The partials [p0, p1) of the run whose first is chunk ``chunk``'s tail, four columns from
+ *  ``col`` on, Ahead of them in flight, added in order. */
+template <int Ahead>
+__device__ __forceinline__ float4 addPartials(const GradArgs& a, uint32_t chunk, uint32_t p0, uint32_t p1, uint32_t col)
+{
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t p = p0; p < p1; p += Ahead) {
+        float4 v[Ahead];
+#pragma unroll
+        for (int u = 0; u < Ahead; ++u) {
+            // past the last: the last again, not added
+            const uint32_t q = min(p + uint32_t(u), p1 - 1u);
+            v[u] = __ldcg(reinterpret_cast<const float4*>((q == 0 ? a.tail : a.head) + size_t(chunk + q) * a.width + col));
+        }
+#pragma unroll
+        for (int u = 0; u < Ahead; ++u) {
+            if (p + uint32_t(u) < p1) {
+                sum.x += v[u].x;
+                sum.y += v[u].y;
+                sum.z += v[u].z;
+                sum.w += v[u].w;
+            }
+        }
+    }
+    return sum;
+}
+
+template <class Out>
+__device__ __forceinline__ void storeJoined(const GradArgs& a, uint32_t row, uint32_t col, float4 sum)
+{
+    Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
+    const float got[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < a.dim)
+            out[col + e] =
+                fromFloat<Out>(a.accumulate ? toFloat(out[col + e]) + a.scale * got[e] : a.scale * got[e]);
+}
+
+/** Rows of up to kWarpParts partials: a warp adds 128 columns of one, in chunk order. Rows of
+ *  more: the eight warps of a CTA add an eighth of its partials each, in chunk order, then the
+ *  eight sums in order. (A frequent id of ordinary text has tens of partials and there are a
+ *  few hundred of them: a CTA each, all columns in turn, took twice as long. A batch of one id
+ *  has thousands.) */
 template <class Out>
 __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
 {
     __shared__ float4 part[kJoinWarps][32];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t blocks = (a.dim + kJoinColumns - 1) / kJoinColumns;
-    const uint64_t items = uint64_t(*a.listCount) * blocks;
-    for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const uint32_t chunk = a.list[item / blocks];
+    const uint64_t longItems = uint64_t(a.listCount[1]) * blocks, items = uint64_t(a.listCount[0]) * blocks;
+    for (uint64_t item = blockIdx.x; item < longItems; item += gridDim.x) {
+        const uint32_t chunk = a.longList[item / blocks];
         const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
         const uint32_t key = __ldg(a.keys + (chunk + 1u) * a.chunk);
-        uint32_t m = 1;  // chunks after this one that the run reaches
-        for (;;) {
-            const uint32_t c = chunk + 1u + m + lane;
-            const bool in = c < a.chunks && __ldg(a.keys + c * a.chunk) == key;
-            const uint32_t reached = __ballot_sync(kFull, in);
-            m += __popc(reached);  // the keys are sorted: the set lanes are the first ones
-            if (reached != kFull)
-                break;
+        uint32_t m = 1;  // chunks after this one that the run reaches: the keys are sorted, so they are counted
+        for (uint32_t more = 4 * kJoinThreads; more == 4 * kJoinThreads;) {
+            bool in[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+                const uint64_t c = uint64_t(chunk) + 1u + m + u * kJoinThreads + threadIdx.x;
+                in[u] = c < a.chunks && __ldg(a.keys + c * a.chunk) == key;
+            }
+            more = 0;
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u)
+                more += uint32_t(__syncthreads_count(in[u]));
+            m += more;
         }
         const uint32_t parts = m + 1u, each = (parts + kJoinWarps - 1) / kJoinWarps;
         const uint32_t p0 = warp * each, p1 = min(p0 + each, parts);
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (col < a.width) {
-#pragma unroll 8
-            for (uint32_t p = p0; p < p1; ++p) {
-                const float* row = (p == 0 ? a.tail : a.head) + size_t(chunk + p) * a.width;
-                const float4 v = *reinterpret_cast<const float4*>(row + col);
-                sum.x += v.x;
-                sum.y += v.y;
-                sum.z += v.z;
-                sum.w += v.w;
-            }
-        }
-        part[warp][lane] = sum;
+        if (col < a.width && p0 < p1)
+            part[warp][lane] = addPartials<16>(a, chunk, p0, p1, col);
+        else
+            part[warp][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         __syncthreads();
-        if (warp == 0) {
+        if (warp == 0 && col < a.dim) {
+            float4 sum = part[0][lane];
 #pragma unroll
             for (int w = 1; w < kJoinWarps; ++w) {
                 const float4 v = part[w][lane];
@@ -712,15 +1009,19 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
                 sum.z += v.z;
                 sum.w += v.w;
             }
-            Out* out = reinterpret_cast<Out*>(a.table) + int64_t(key) * a.tableStride;
-            const float got[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < a.dim)
-                    out[col + e] = fromFloat<Out>(a.accumulate ? toFloat(out[col + e]) + a.scale * got[e]
-                                                               : a.scale * got[e]);
+            storeJoined<Out>(a, key, col, sum);
         }
         __syncthreads();
+    }
+    for (uint64_t item = uint64_t(blockIdx.x) * kJoinWarps + warp; item < items; item += uint64_t(gridDim.x) * kJoinWarps) {
+        const uint32_t chunk = a.list[item / blocks];
+        const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
+        const uint64_t next = uint64_t(chunk) + 1u + lane;
+        const uint32_t first = next < a.chunks ? __ldg(a.keys + next * a.chunk) : kNoKey;
+        const uint32_t key = __shfl_sync(kFull, first, 0);
+        const uint32_t parts = 1u + __popc(__ballot_sync(kFull, first == key));
+        if (col < a.width)
+            storeJoined<Out>(a, key, col, addPartials<8>(a, chunk, 0, parts, col));
     }
 }
 
@@ -842,14 +1143,51 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
     });
 }
 
+size_t clusterShared(int items)
+{
+    const size_t keys = size_t(kClusterThreads) * items * 8;
+    return 2 * keys + (keys >= kPeerBytes ? 0 : kPeerBytes) + size_t(kClusterWarps) * kMaxBins * 2;
+}
+
+/** Whether the current device holds a cluster of kClusterSize CTAs of the sort (kept per device). */
+bool largeClusters()
+{
+    static std::mutex mu;
+    static std::vector<int> known;  // 0: not asked, 1: no, 2: yes
+    int dev = 0;
+    cudaCheck(cudaGetDevice(&dev), "cudaGetDevice");
+    std::lock_guard<std::mutex> lock(mu);
+    if (int(known.size()) <= dev)
+        known.resize(size_t(dev) + 1, 0);
+    if (known[size_t(dev)] == 0) {
+        auto kernel = clusterSortKernel<int32_t, kClusterItems>;
+        cudaLaunchAttribute attr{};
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim = {unsigned(kClusterSize), 1, 1};
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(kClusterSize, 1, 1);
+        config.blockDim = dim3(kClusterThreads, 1, 1);
+        config.dynamicSmemBytes = clusterShared(kClusterItems);
+        config.attrs = &attr;
+        config.numAttrs = 1;
+        int clusters = 0;
+        const bool ok = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                            int(config.dynamicSmemBytes)) == cudaSuccess
+            && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess
+            && cudaOccupancyMaxActiveClusters(&clusters, kernel, &config) == cudaSuccess && clusters > 0;
+        (void)cudaGetLastError();
+        known[size_t(dev)] = ok ? 2 : 1;
+    }
+    return known[size_t(dev)] == 2;
+}
+
 /** How the gradient's sort, sums and scratch are laid out. */
 struct GradPlan {
     uint32_t n = 0, bits = 0, passes = 0, digitBits = 0, bins = 0, tiles = 0;
-    bool cluster = false;  // sorted by one cluster
     Piece piece = Piece::Strided;
     uint32_t pieces = 0, group = 0, slices = 0, chunk = 0, chunks = 0, width = 0;
     uint64_t present = 0, listCount = 0, hist = 0, zeroed = 0;  // offsets; [0, zeroed) is cleared
-    uint64_t firstHist = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, head = 0, tail = 0, bytes = 0;
+    uint64_t firstHist = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, longList = 0, head = 0, tail = 0, bytes = 0;
 };
 
 GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
@@ -863,7 +1201,6 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     p.passes = (p.bits + 8) / 9;
     p.digitBits = p.passes == 0 ? 0 : (p.bits + p.passes - 1) / p.passes;
     p.bins = 1u << p.digitBits;
-    p.cluster = p.n <= kClusterKeys;
     p.tiles = (p.n + kSortTile - 1) / kSortTile;
     // whole 16-byte words if every vector and every row of the table starts on them
     const int pack = 16 / inBytes;
@@ -895,16 +1232,18 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
         return was;
     };
     p.present = take((uint64_t(d.rows) + 31) / 32 * 4);
-    p.listCount = take(4);
-    const uint64_t histBytes = p.cluster ? 0 : uint64_t(p.tiles) * p.bins * 4;
+    p.listCount = take(8);
+    const bool portable = p.n <= kPortableKeys;  // the query's answer does not depend on the device
+    const uint64_t histBytes = portable ? 0 : uint64_t(p.tiles) * p.bins * 4;
     p.hist = take(p.passes > 1 ? histBytes * (p.passes - 1) : 0);
     p.zeroed = at;
     p.firstHist = take(histBytes);
-    for (int k = 0; k < (p.cluster ? 1 : 2); ++k) {
+    for (int k = 0; k < (portable ? 1 : 2); ++k) {
         p.key[k] = take(uint64_t(p.n) * 4);
         p.pos[k] = take(uint64_t(p.n) * 4);
     }
     p.list = take(uint64_t(p.chunks) * 4);
+    p.longList = take(uint64_t(p.chunks) * 4);
     p.head = take(uint64_t(p.chunks) * p.width * 4);
     p.tail = take(uint64_t(p.chunks) * p.width * 4);
     p.bytes = at;
@@ -919,12 +1258,23 @@ void launchSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const char* w
     launchCheck(who);
 }
 
+template <class In, class Out, bool Aligned>
+void launchBulkSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const char* who)
+{
+    auto kernel = bulkSumKernel<In, Out, Aligned>;
+    cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(BulkShared))), who);
+    kernel<<<blocks, kBulkThreads, sizeof(BulkShared), s>>>(a);
+    launchCheck(who);
+}
+
 template <class Tok, int Items>
 void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaStream_t s, const char* who)
 {
     auto kernel = clusterSortKernel<Tok, Items>;
-    const size_t shared = size_t(kClusterThreads) * Items * 8 + size_t(kClusterWarps) * kMaxBins * 2;
+    const size_t shared = clusterShared(Items);
     cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
+    if (ctas > 8)
+        cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), who);
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim = {ctas, 1, 1};
@@ -938,8 +1288,19 @@ void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaSt
     cudaCheck(cudaLaunchKernelEx(&config, kernel, a), who);
 }
 
-/** Bytes of rows that the SMs without part in a cluster's sort zero meanwhile. */
-constexpr int64_t kZeroedBesideSort = 32ll << 20;
+template <bool First, class Tok>
+void launchPass(const GradArgs& a, unsigned tiles, cudaStream_t s, const char* who)
+{
+    auto kernel = passKernel<First, Tok>;
+    const int shared = kSortWarps * int(kMaxBins) * 6;
+    cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared), who);
+    kernel<<<tiles, kSortThreads, shared, s>>>(a);
+    launchCheck(who);
+}
+
+/** Bytes of rows that the SMs without part in a cluster's sort zero meanwhile: what they write in
+ *  about the sort's time (9 us with one key a thread, 17 with two, 30 with eight). */
+constexpr int64_t zeroedBesideSort(unsigned perThread) { return (40ll + 20ll * perThread) << 20; }
 
 void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
 {
@@ -992,26 +1353,28 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.pieces = p.pieces;
     a.listCount = words(p.listCount);
     a.list = words(p.list);
+    a.longList = words(p.longList);
     a.head = reinterpret_cast<float*>(scratch + p.head);
     a.tail = reinterpret_cast<float*>(scratch + p.tail);
     a.width = p.width;
     a.present = accumulate ? nullptr : words(p.present);
-    if (p.cluster) {
+    if (p.n <= kPortableKeys || (p.n <= kClusterKeys && largeClusters())) {
         a.keyOut = words(p.key[0]);
         a.posOut = words(p.pos[0]);
         unsigned ctas = 1;
-        while (ctas < unsigned(kClusterSize) && ctas * unsigned(kClusterThreads) < p.n)
-            ctas *= 2;
+        // what one CTA holds needs no exchange; past that, as many as the cluster may have
+        if (p.n > uint32_t(kClusterThreads) * kClusterItems)
+            ctas = p.n <= kPortableKeys ? 8u : unsigned(kClusterSize);
+        const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
         // 1024 threads an SM: the SMs beside the cluster, in whole clusters
         unsigned blocks = ctas;
         if (!accumulate && a.rowBytes > 0) {
-            a.zeroed = uint32_t(std::min(d.rows, kZeroedBesideSort / a.rowBytes));
+            a.zeroed = uint32_t(std::min(d.rows, zeroedBesideSort(perThread) / a.rowBytes));
             const int64_t want = (int64_t(a.zeroed) + kClusterWarps - 1) / kClusterWarps;
             blocks += unsigned(std::min<int64_t>((want + ctas - 1) / ctas, sms / ctas - 1)) * ctas;
             if (blocks == ctas)
                 a.zeroed = 0;
         }
-        const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
         withIndex(d.token_type, [&](auto tok) {
             using Tok = decltype(tok);
             if (perThread <= 1)
@@ -1020,8 +1383,6 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
                 launchClusterSort<Tok, 2>(a, ctas, blocks, s, who);
             else if (perThread <= 4)
                 launchClusterSort<Tok, 4>(a, ctas, blocks, s, who);
-            else if (perThread <= 8)
-                launchClusterSort<Tok, 8>(a, ctas, blocks, s, who);
             else
                 launchClusterSort<Tok, kClusterItems>(a, ctas, blocks, s, who);
         });
@@ -1044,24 +1405,33 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
                 b.keyOut = words(p.key[k & 1]);
                 b.posOut = words(p.pos[k & 1]);
                 if (k == 0)
-                    passKernel<true, Tok><<<p.tiles, kSortThreads, 0, s>>>(b);
+                    launchPass<true, Tok>(b, p.tiles, s, who);
                 else
-                    passKernel<false, Tok><<<p.tiles, kSortThreads, 0, s>>>(b);
-                launchCheck(who);
+                    launchPass<false, Tok>(b, p.tiles, s, who);
             }
         });
         a.keys = words(p.key[(p.passes + 1) & 1]);
         a.order = words(p.pos[(p.passes + 1) & 1]);
     }
     const uint64_t lanes = uint64_t(p.chunks) * p.slices * p.group;
-    a.sumBlocks = gridOf(int64_t((lanes + kSumThreads - 1) / kSumThreads), who);
+    const bool bulk = p.piece != Piece::Strided && d.dim * inBytes >= kBulkLeast;
+    if (bulk) {
+        a.slices = uint32_t((d.dim * inBytes + kBulkSlab - 1) / kBulkSlab);
+        a.sumBlocks = gridOf(int64_t(p.chunks) * a.slices, who);
+    } else {
+        a.sumBlocks = gridOf(int64_t((lanes + kSumThreads - 1) / kSumThreads), who);
+    }
     const int64_t zeroing = a.present == nullptr ? 0 : std::min<int64_t>(sms * 8, (d.rows - a.zeroed + 7) / 8);
     const unsigned blocks = gridOf(int64_t(a.sumBlocks) + zeroing, who);
     withElement(d.values_type, [&](auto in) {
         withElement(d.table_type, [&](auto out) {
             using In = decltype(in);
             using Out = decltype(out);
-            if (p.piece == Piece::Aligned)
+            if (bulk && p.piece == Piece::Aligned)
+                launchBulkSum<In, Out, true>(a, blocks, s, who);
+            else if (bulk)
+                launchBulkSum<In, Out, false>(a, blocks, s, who);
+            else if (p.piece == Piece::Aligned)
                 launchSum<In, Out, Piece::Aligned>(a, blocks, s, who);
             else if (p.piece == Piece::Shifted)
                 launchSum<In, Out, Piece::Shifted>(a, blocks, s, who);
