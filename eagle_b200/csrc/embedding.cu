@@ -113,6 +113,8 @@ __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
 // ------------------------------------------------------------------ gradient: sort
 
 constexpr uint32_t kMaxBins = 512;        // 9 bits a pass
+constexpr int64_t kZeroUnit = 16384;      // bytes a CTA zeroes
+constexpr int64_t kZeroByWarp = 2048;     // bytes of a row that one warp zeroes
 constexpr uint32_t kWarpParts = 32;       // partials of a run that one warp joins
 constexpr uint32_t kNoKey = 0xffffffffu;  // behind the last key: every digit of it is the highest
 
@@ -157,7 +159,11 @@ struct GradArgs {
     uint32_t width;      // dim rounded up to 8
     // zeroing
     int64_t rowBytes, strideBytes;
-    uint32_t zeroed;     // rows [0, zeroed) are zeroed, with tokens or without, beside the sort
+    uint32_t zeroRows;    // rows in a unit
+    uint32_t zeroPieces;  // units in a row
+    int64_t zeroed;       // rows [0, zeroed) are zeroed, with tokens or without, beside the sort
+    int64_t zeroedBefore; // rows up to this are zeroed before the joins, the others beside them
+    uint32_t joinBlocks;  // CTAs that join; the others zero
 };
 
 /** The keys of Items tokens, ``step`` apart from ``from`` on (kNoKey past the last). No branch
@@ -182,24 +188,48 @@ __device__ __forceinline__ void loadKeys(const GradArgs& a, uint32_t from, uint3
     }
 }
 
-/** One warp zeroes row ``r``: whole 16-byte words, and bytes two at a time before and after. */
-__device__ __forceinline__ void zeroRow(const GradArgs& a, int64_t r)
+/** Zero the bytes [from, to), both even, with threads ``at``, ``at + step``, ...: whole 16-byte
+ *  words, and two bytes at a time before and after. */
+__device__ __forceinline__ void zeroBytes(char* from, char* to, uint32_t at, uint32_t step)
 {
-    const uint32_t lane = threadIdx.x & 31u;
-    char* row = reinterpret_cast<char*>(a.table) + r * a.strideBytes;
-    char* end = row + a.rowBytes;
-    char* from = reinterpret_cast<char*>((reinterpret_cast<uint64_t>(row) + 15u) & ~uint64_t(15));
-    char* to = reinterpret_cast<char*>(reinterpret_cast<uint64_t>(end) & ~uint64_t(15));
-    if (from > to) {  // inside one word
-        from = end;
-        to = end;
+    char* words = reinterpret_cast<char*>((reinterpret_cast<uint64_t>(from) + 15u) & ~uint64_t(15));
+    char* rest = reinterpret_cast<char*>(reinterpret_cast<uint64_t>(to) & ~uint64_t(15));
+    if (words > rest) {  // inside one word
+        words = to;
+        rest = to;
     }
-    for (char* p = from + lane * 16u; p < to; p += 32 * 16)
+    for (char* p = words + size_t(at) * 16u; p < rest; p += size_t(step) * 16u)
         *reinterpret_cast<uint4*>(p) = make_uint4(0u, 0u, 0u, 0u);
-    for (char* p = row + lane * 2u; p < from; p += 64)
+    for (char* p = from + size_t(at) * 2u; p < words; p += size_t(step) * 2u)
         *reinterpret_cast<uint16_t*>(p) = 0;
-    for (char* p = to + lane * 2u; p < end; p += 64)
+    for (char* p = rest + size_t(at) * 2u; p < to; p += size_t(step) * 2u)
         *reinterpret_cast<uint16_t*>(p) = 0;
+}
+
+/** Zero unit ``unit`` of the rows [row0, row1), of those whose bit in ``present`` is clear
+ *  (all if it is null): a unit is ``zeroRows`` rows or, of longer ones, a piece of kZeroUnit bytes. CTAs that
+ *  take neighbouring units one after the other write at 7 TB/s; a grid that strides over a
+ *  large plane, each warp a row, at 4. */
+__device__ __forceinline__ void zeroUnit(const GradArgs& a, const uint32_t* present, int64_t row0, int64_t row1,
+    uint64_t unit)
+{
+    char* table = reinterpret_cast<char*>(a.table);
+    const uint64_t which = unit / a.zeroPieces;
+    const int64_t piece = int64_t(unit - which * a.zeroPieces) * kZeroUnit;
+    const int64_t begin = row0 + int64_t(which) * a.zeroRows, end = min(begin + int64_t(a.zeroRows), row1);
+    auto absent = [&](int64_t r) {
+        return present == nullptr || ((__ldg(present + (r >> 5)) >> (r & 31)) & 1u) == 0;
+    };
+    if (a.rowBytes <= kZeroByWarp) {
+        for (int64_t r = begin + (threadIdx.x >> 5); r < end; r += blockDim.x >> 5)
+            if (absent(r))
+                zeroBytes(table + r * a.strideBytes, table + r * a.strideBytes + a.rowBytes, threadIdx.x & 31u, 32u);
+    } else {
+        for (int64_t r = begin; r < end; ++r)
+            if (absent(r))
+                zeroBytes(table + r * a.strideBytes + piece,
+                    table + r * a.strideBytes + min(piece + kZeroUnit, a.rowBytes), threadIdx.x, blockDim.x);
+    }
 }
 
 /** The keys of the same digit before each item among a CTA's: items are ranked warp by warp,
@@ -278,10 +308,20 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
+    letNextKernelStart();
     if (blockIdx.x >= ctas) {
-        for (int64_t r = int64_t(blockIdx.x - ctas) * kClusterWarps + (threadIdx.x >> 5); r < int64_t(a.zeroed);
-             r += int64_t(gridDim.x - ctas) * kClusterWarps)
-            zeroRow(a, r);
+        char* table = reinterpret_cast<char*>(a.table);
+        const uint32_t at = blockIdx.x - ctas, others = gridDim.x - ctas;
+        if (a.strideBytes == a.rowBytes) {  // one plane: every CTA 64 KB at a time
+            constexpr int64_t kPiece = 65536;
+            const int64_t bytes = a.zeroed * a.rowBytes;
+            for (int64_t from = at * kPiece; from < bytes; from += others * kPiece)
+                zeroBytes(table + from, table + min(from + kPiece, bytes), threadIdx.x, kClusterThreads);
+        } else {
+            for (int64_t r = int64_t(at) * kClusterWarps + (threadIdx.x >> 5); r < a.zeroed;
+                 r += int64_t(others) * kClusterWarps)
+                zeroBytes(table + r * a.strideBytes, table + r * a.strideBytes + a.rowBytes, threadIdx.x & 31u, 32u);
+        }
         return;
     }
     constexpr uint32_t kTile = uint32_t(kClusterThreads) * Items;
@@ -377,6 +417,7 @@ template <class Tok>
 __global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
 {
     __shared__ uint32_t count[kMaxBins];
+    letNextKernelStart();
     if (threadIdx.x < a.bins)
         count[threadIdx.x] = 0;
     __syncthreads();
@@ -404,6 +445,8 @@ template <bool First, class Tok>
 __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
+    letNextKernelStart();
+    waitForKernelBefore();
     uint32_t* peers = reinterpret_cast<uint32_t*>(raw);
     uint16_t* count = reinterpret_cast<uint16_t*>(peers + kSortWarps * kMaxBins);
     __shared__ uint32_t base[kMaxBins], scan[33];
@@ -558,16 +601,6 @@ __device__ __forceinline__ void loadEight(uint32_t (&v)[kRowsInFlight], const ui
     }
 }
 
-/** The rows past ``zeroed`` that have no token, by the warps of the CTAs past ``sumBlocks``. */
-__device__ __forceinline__ void zeroAbsent(const GradArgs& a)
-{
-    const uint32_t warps = blockDim.x >> 5;
-    for (int64_t r = int64_t(a.zeroed) + int64_t(blockIdx.x - a.sumBlocks) * warps + (threadIdx.x >> 5); r < a.rows;
-         r += int64_t(gridDim.x - a.sumBlocks) * warps)
-        if (((__ldg(a.present + (r >> 5)) >> (r & 31)) & 1u) == 0)
-            zeroRow(a, r);
-}
-
 /** Element offset of token ``t``'s vector. */
 __device__ __forceinline__ int64_t vectorOf(const GradArgs& a, uint32_t t)
 {
@@ -640,8 +673,10 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
     constexpr int N = 16 / int(sizeof(In));
     constexpr Piece P = Aligned ? Piece::Aligned : Piece::Shifted;
     extern __shared__ __align__(16) unsigned char raw[];
+    letNextKernelStart();
+    waitForKernelBefore();
     if (blockIdx.x >= a.sumBlocks) {
-        zeroAbsent(a);
+        zeroUnit(a, a.present, a.zeroed, a.zeroedBefore, blockIdx.x - a.sumBlocks);
         return;
     }
     BulkShared& s = *reinterpret_cast<BulkShared*>(raw);
@@ -786,8 +821,10 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
 template <class In, class Out, Piece P, int N>
 __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
 {
+    letNextKernelStart();
+    waitForKernelBefore();
     if (blockIdx.x >= a.sumBlocks) {
-        zeroAbsent(a);
+        zeroUnit(a, a.present, a.zeroed, a.zeroedBefore, blockIdx.x - a.sumBlocks);
         return;
     }
     const uint64_t id = uint64_t(blockIdx.x) * kSumThreads + threadIdx.x;
@@ -971,10 +1008,15 @@ template <class Out>
 __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
 {
     __shared__ float4 part[kJoinWarps][32];
+    waitForKernelBefore();
+    if (blockIdx.x >= a.joinBlocks) {
+        zeroUnit(a, a.present, a.zeroedBefore, a.rows, blockIdx.x - a.joinBlocks);
+        return;
+    }
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t blocks = (a.dim + kJoinColumns - 1) / kJoinColumns;
     const uint64_t longItems = uint64_t(a.listCount[1]) * blocks, items = uint64_t(a.listCount[0]) * blocks;
-    for (uint64_t item = blockIdx.x; item < longItems; item += gridDim.x) {
+    for (uint64_t item = blockIdx.x; item < longItems; item += a.joinBlocks) {
         const uint32_t chunk = a.longList[item / blocks];
         const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
         const uint32_t key = __ldg(a.keys + (chunk + 1u) * a.chunk);
@@ -1013,7 +1055,8 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
         }
         __syncthreads();
     }
-    for (uint64_t item = uint64_t(blockIdx.x) * kJoinWarps + warp; item < items; item += uint64_t(gridDim.x) * kJoinWarps) {
+    for (uint64_t item = uint64_t(blockIdx.x) * kJoinWarps + warp; item < items;
+         item += uint64_t(a.joinBlocks) * kJoinWarps) {
         const uint32_t chunk = a.list[item / blocks];
         const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
         const uint64_t next = uint64_t(chunk) + 1u + lane;
@@ -1028,9 +1071,7 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
 /** No tokens: every row is zero. */
 __global__ __launch_bounds__(kSumThreads) void zeroRowsKernel(GradArgs a)
 {
-    for (int64_t r = int64_t(blockIdx.x) * (kSumThreads / 32) + (threadIdx.x >> 5); r < a.rows;
-         r += int64_t(gridDim.x) * (kSumThreads / 32))
-        zeroRow(a, r);
+    zeroUnit(a, nullptr, 0, a.rows, blockIdx.x);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1254,8 +1295,7 @@ template <class In, class Out, Piece P>
 void launchSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const char* who)
 {
     constexpr int N = P == Piece::Strided ? 4 : 16 / int(sizeof(In));
-    sumKernel<In, Out, P, N><<<blocks, kSumThreads, 0, s>>>(a);
-    launchCheck(who);
+    launchBehind(sumKernel<In, Out, P, N>, blocks, kSumThreads, 0, s, a, who);
 }
 
 template <class In, class Out, bool Aligned>
@@ -1263,8 +1303,7 @@ void launchBulkSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const cha
 {
     auto kernel = bulkSumKernel<In, Out, Aligned>;
     cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(BulkShared))), who);
-    kernel<<<blocks, kBulkThreads, sizeof(BulkShared), s>>>(a);
-    launchCheck(who);
+    launchBehind(kernel, blocks, kBulkThreads, sizeof(BulkShared), s, a, who);
 }
 
 template <class Tok, int Items>
@@ -1294,13 +1333,15 @@ void launchPass(const GradArgs& a, unsigned tiles, cudaStream_t s, const char* w
     auto kernel = passKernel<First, Tok>;
     const int shared = kSortWarps * int(kMaxBins) * 6;
     cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared), who);
-    kernel<<<tiles, kSortThreads, shared, s>>>(a);
-    launchCheck(who);
+    launchBehind(kernel, tiles, kSortThreads, shared, s, a, who);
 }
 
 /** Bytes of rows that the SMs without part in a cluster's sort zero meanwhile: what they write in
- *  about the sort's time (9 us with one key a thread, 17 with two, 30 with eight). */
-constexpr int64_t zeroedBesideSort(unsigned perThread) { return (40ll + 20ll * perThread) << 20; }
+ *  about the sort's time, at 3.3 TB/s (7 us with one key a thread, 14 with two, 31 with eight). */
+constexpr int64_t zeroedBesideSort(unsigned perThread) { return (12ll + 12ll * perThread) << 20; }
+
+/** And those that the SMs without a join zero: what they write in about 8 us. */
+constexpr int64_t kZeroedBesideJoin = 32ll << 20;
 
 void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
 {
@@ -1316,10 +1357,13 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.dim = uint32_t(d.dim);
     a.rowBytes = d.dim * outBytes;
     a.strideBytes = d.table_stride * outBytes;
+    a.zeroRows = uint32_t(std::max<int64_t>(1, kZeroUnit / a.rowBytes));
+    a.zeroPieces = uint32_t((a.rowBytes + kZeroUnit - 1) / kZeroUnit);
+    auto unitsOf = [&](int64_t rows) { return (rows + a.zeroRows - 1) / a.zeroRows * a.zeroPieces; };
     const int64_t sms = smCount();
     if (p.n == 0) {
         if (!accumulate) {
-            zeroRowsKernel<<<unsigned(std::min<int64_t>((d.rows + 7) / 8, sms * 8)), kSumThreads, 0, s>>>(a);
+            zeroRowsKernel<<<gridOf(unitsOf(d.rows), who), kSumThreads, 0, s>>>(a);
             launchCheck(who);
         }
         return;
@@ -1368,11 +1412,13 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
         // 1024 threads an SM: the SMs beside the cluster, in whole clusters
         unsigned blocks = ctas;
-        if (!accumulate && a.rowBytes > 0) {
-            a.zeroed = uint32_t(std::min(d.rows, zeroedBesideSort(perThread) / a.rowBytes));
-            const int64_t want = (int64_t(a.zeroed) + kClusterWarps - 1) / kClusterWarps;
-            blocks += unsigned(std::min<int64_t>((want + ctas - 1) / ctas, sms / ctas - 1)) * ctas;
-            if (blocks == ctas)
+        if (!accumulate) {
+            a.zeroed = std::min(d.rows, zeroedBesideSort(perThread) / a.rowBytes);
+            const int64_t besides =
+                std::min<int64_t>((a.zeroed * a.rowBytes / 65536 + ctas) / ctas, sms / ctas - 1);
+            if (besides > 0)
+                blocks += unsigned(besides) * ctas;
+            else
                 a.zeroed = 0;
         }
         withIndex(d.token_type, [&](auto tok) {
@@ -1421,7 +1467,10 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     } else {
         a.sumBlocks = gridOf(int64_t((lanes + kSumThreads - 1) / kSumThreads), who);
     }
-    const int64_t zeroing = a.present == nullptr ? 0 : std::min<int64_t>(sms * 8, (d.rows - a.zeroed + 7) / 8);
+    a.zeroedBefore = d.rows;
+    if (a.present != nullptr && p.chunks > 1)
+        a.zeroedBefore = std::max(a.zeroed, d.rows - kZeroedBesideJoin / a.rowBytes);
+    const int64_t zeroing = a.present == nullptr ? 0 : unitsOf(a.zeroedBefore - a.zeroed);
     const unsigned blocks = gridOf(int64_t(a.sumBlocks) + zeroing, who);
     withElement(d.values_type, [&](auto in) {
         withElement(d.table_type, [&](auto out) {
@@ -1441,10 +1490,10 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     });
     if (p.chunks > 1) {
         const int64_t items = int64_t(p.chunks / 2) * ((d.dim + kJoinColumns - 1) / kJoinColumns);
-        withElement(d.table_type, [&](auto out) {
-            joinKernel<decltype(out)><<<unsigned(std::min<int64_t>(items, sms * 8)), kJoinThreads, 0, s>>>(a);
-            launchCheck(who);
-        });
+        a.joinBlocks = unsigned(std::min<int64_t>(items, sms * 8));
+        const unsigned all = gridOf(a.joinBlocks + (a.present == nullptr ? 0 : unitsOf(d.rows - a.zeroedBefore)), who);
+        withElement(d.table_type,
+            [&](auto out) { launchBehind(joinKernel<decltype(out)>, all, kJoinThreads, 0, s, a, who); });
     }
 }
 

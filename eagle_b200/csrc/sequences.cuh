@@ -72,6 +72,35 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
     T e[N];
 };
 
+// ------------------------------------------------------------- kernels in a row
+//
+// A call of several kernels launches each but the first while the one before it still runs
+// (programmatic dependent launch), so that its CTAs are in place when their turn comes. Such
+// a kernel touches no memory before ``waitForKernelBefore``, which returns once every kernel
+// before it has ended and its writes are visible; the one before lets it start with
+// ``letNextKernelStart``, early, which takes effect when all of its CTAs are running.
+
+__device__ __forceinline__ void waitForKernelBefore() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void letNextKernelStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+/** Launch ``kernel(args)``, which starts with waitForKernelBefore, behind another of the call's. */
+template <class Args>
+void launchBehind(void (*kernel)(Args), unsigned blocks, unsigned threads, size_t shared, cudaStream_t s,
+    const Args& args, const char* who)
+{
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(blocks, 1, 1);
+    config.blockDim = dim3(threads, 1, 1);
+    config.dynamicSmemBytes = shared;
+    config.stream = s;
+    config.attrs = &attr;
+    config.numAttrs = 1;
+    cudaCheck(cudaLaunchKernelEx(&config, kernel, args), who);
+}
+
 // ------------------------------------------------------------- host side
 
 inline int elementBytes(uint32_t type, const char* who)
