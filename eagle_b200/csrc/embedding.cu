@@ -44,6 +44,7 @@ struct LookupArgs {
     int64_t tokenBatch, tokenSeq;  // strides of the ids
     int64_t valueBatch, valueSeq;  // strides of the outputs
     int64_t n;                     // tokens
+    uint32_t dim;
     uint32_t pieces;               // packs per row
     FastDiv perRow;                // by pieces
     FastDiv perBatch;              // by seq
@@ -64,6 +65,18 @@ __device__ __forceinline__ int64_t rowOfToken(const void* tokens, int64_t at, in
     return r < uint64_t(rows) ? int64_t(r) : -1;
 }
 
+/** Where a thread's packs read and write: token t's row (-1: none) and output vector. */
+template <class Tok>
+__device__ __forceinline__ void placeOf(const LookupArgs& a, int64_t t, int64_t& row, int64_t& to)
+{
+    const uint32_t b = a.flat ? 0u : a.perBatch(uint32_t(t));
+    const int64_t s = t - int64_t(b) * a.perBatch.d;
+    row = rowOfToken<Tok>(a.tokens, int64_t(b) * a.tokenBatch + s * a.tokenSeq, a.first, a.rows);
+    to = int64_t(b) * a.valueBatch + s * a.valueSeq;
+}
+
+// Narrow rows: the packs of all of them in a row, so that no lane idles.
+
 /** ``Unroll`` packs of N values per thread, a CTA's width apart: neighbouring threads hold
  *  neighbouring packs of the flattened (token, column) plane, so loads and stores are
  *  whole lines whatever the row length, and short rows leave no lane idle. */
@@ -76,22 +89,17 @@ __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
     const In* table = reinterpret_cast<const In*>(a.table);
     Out* values = reinterpret_cast<Out*>(a.values);
     int64_t from[Unroll], to[Unroll];
+    bool inside[Unroll];
 #pragma unroll
     for (int u = 0; u < Unroll; ++u) {
         const uint32_t k = col0 + uint32_t(u) * kLookupThreads + threadIdx.x;
         const uint32_t down = a.perRow(k);
         const uint32_t col = (k - down * a.pieces) * N;
-        const int64_t t = row0 + down;
-        from[u] = -2;
-        to[u] = 0;
-        if (t < a.n) {
-            const uint32_t b = a.flat ? 0u : a.perBatch(uint32_t(t));
-            const int64_t s = t - int64_t(b) * a.perBatch.d;
-            const int64_t in = a.flat ? t : s;
-            const int64_t r = rowOfToken<Tok>(a.tokens, int64_t(b) * a.tokenBatch + in * a.tokenSeq, a.first, a.rows);
-            from[u] = r < 0 ? -1 : r * a.tableStride + col;
-            to[u] = int64_t(b) * a.valueBatch + in * a.valueSeq + col;
-        }
+        inside[u] = row0 + down < a.n;
+        int64_t row;
+        placeOf<Tok>(a, min(row0 + down, a.n - 1), row, to[u]);
+        from[u] = row < 0 ? -1 : row * a.tableStride + col;
+        to[u] += col;
     }
     Pack<In, N> got[Unroll];
 #pragma unroll
@@ -100,13 +108,160 @@ __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
             got[u] = *reinterpret_cast<const Pack<In, N>*>(table + from[u]);
 #pragma unroll
     for (int u = 0; u < Unroll; ++u) {
-        if (from[u] == -2)
+        if (!inside[u])
             continue;
         Pack<Out, N> out;
 #pragma unroll
         for (int e = 0; e < N; ++e)
             out.e[e] = fromFloat<Out>(from[u] >= 0 ? toFloat(got[u].e[e]) * a.scale : 0.0f);
         *reinterpret_cast<Pack<Out, N>*>(values + to[u]) = out;
+    }
+}
+
+/** The 16 bytes ``skip`` into 32 neighbouring ones. */
+__device__ __forceinline__ uint4 shiftWords(uint4 lo, uint4 hi, uint32_t skip)
+{
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (skip & 8u) {
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+            w[j] = w[j + 2];
+    }
+    if (skip & 4u) {
+#pragma unroll
+        for (int j = 0; j < 5; ++j)
+            w[j] = w[j + 1];
+    }
+    const uint32_t shift = (skip & 3u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
+        __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
+}
+
+/** 16 bytes from any address of whole elements, of which ``valid`` bytes are wanted: the one or
+ *  two aligned words that hold them (each holds a wanted byte, so it lies in mapped memory),
+ *  shifted together. What lies past ``valid`` is unspecified. */
+__device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
+    const uint32_t skip = uint32_t(at) & 15u;
+    const uint4 lo = __ldg(word);
+    const uint4 hi = skip + valid > 16u ? __ldg(word + 1) : make_uint4(0u, 0u, 0u, 0u);
+    return shiftWords(lo, hi, skip);
+}
+
+/** Rows of odd length or alignment: packs are cut where the output's 16-byte words begin, and the
+ *  row is read from wherever that falls as aligned words shifted together (element by
+ *  element, as the at most two incomplete packs of a row still are, took four times as long).
+ *  A row of dim values has up to ceil(dim / N) + 1 packs, the first ending at its first word. */
+template <class In, class Out, class Tok, int N, int Unroll>
+__global__ __launch_bounds__(kLookupThreads) void lookupShiftedKernel(LookupArgs a)
+{
+    const int64_t base = int64_t(blockIdx.x) * (kLookupThreads * Unroll);
+    const int64_t row0 = base / a.pieces;
+    const uint32_t col0 = uint32_t(base - row0 * a.pieces);
+    const In* table = reinterpret_cast<const In*>(a.table);
+    Out* values = reinterpret_cast<Out*>(a.values);
+    const int dim = int(a.dim);
+    const In* from[Unroll];
+    Out* to[Unroll];
+    int begin[Unroll];  // the pack's first column, of the row's dim
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u) {
+        const uint32_t k = col0 + uint32_t(u) * kLookupThreads + threadIdx.x;
+        const uint32_t down = a.perRow(k);
+        int64_t row, at;
+        placeOf<Tok>(a, min(row0 + down, a.n - 1), row, at);
+        to[u] = values + at;
+        from[u] = row < 0 ? nullptr : table + row * a.tableStride;
+        const int lead = int((0u - uint32_t(reinterpret_cast<uint64_t>(to[u]))) & 15u) / int(sizeof(Out));
+        begin[u] = row0 + down < a.n ? lead + (int(k - down * a.pieces) - 1) * N : dim;
+    }
+    constexpr int kWords = N * int(sizeof(In)) / 16;
+    uint4 got[Unroll][kWords];
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u)
+        if (from[u] != nullptr && begin[u] >= 0 && begin[u] + N <= dim)
+#pragma unroll
+            for (int w = 0; w < kWords; ++w)
+                got[u][w] = loadShifted(from[u] + begin[u] + w * (N / kWords), 16u);
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u) {
+        if (begin[u] >= 0 && begin[u] + N <= dim) {
+            const Pack<In, N>& in = *reinterpret_cast<const Pack<In, N>*>(&got[u]);
+            Pack<Out, N> out;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                out.e[e] = fromFloat<Out>(from[u] != nullptr ? toFloat(in.e[e]) * a.scale : 0.0f);
+            *reinterpret_cast<Pack<Out, N>*>(to[u] + begin[u]) = out;
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int col = begin[u] + e;
+                if (col >= 0 && col < dim)
+                    to[u][col] = fromFloat<Out>(from[u] != nullptr ? toFloat(from[u][col]) * a.scale : 0.0f);
+            }
+        }
+    }
+}
+
+// Wide rows: a warp takes 32 * Unroll packs of one row, so that the row, its addresses and its
+// alignment are worked out once for all of them (per pack, that took more time than the
+// bytes: 128 us against 210 at 65536 rows of 16 KB, and 8 against 20 at 10007 of 2002 bytes).
+
+/** ``Shifted``: packs are cut where the output's 16-byte words begin and read from wherever that
+ *  falls in the table; the up to N - 1 values before the first and after the last are taken
+ *  one to a lane. */
+template <class In, class Out, class Tok, int N, int Unroll, bool Shifted>
+__global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint64_t id = uint64_t(blockIdx.x) * (kLookupThreads / 32) + (threadIdx.x >> 5);
+    const int64_t t = int64_t(id / a.pieces);  // pieces: warps to a row
+    if (t >= a.n)
+        return;
+    const uint32_t segment = uint32_t(id - uint64_t(t) * a.pieces);
+    int64_t row, at;
+    placeOf<Tok>(a, t, row, at);
+    const In* from = reinterpret_cast<const In*>(a.table) + (row < 0 ? 0 : row * a.tableStride);
+    Out* to = reinterpret_cast<Out*>(a.values) + at;
+    uint32_t lead = 0;
+    if constexpr (Shifted)
+        lead = min(((0u - uint32_t(reinterpret_cast<uint64_t>(to))) & 15u) / uint32_t(sizeof(Out)), a.dim);
+    const uint32_t whole = (a.dim - lead) / N;
+    const uint32_t pack0 = segment * (32u * Unroll) + lane;
+    constexpr int kWords = N * int(sizeof(In)) / 16;
+    uint4 got[Unroll][kWords];
+    if (row >= 0) {
+#pragma unroll
+        for (int u = 0; u < Unroll; ++u) {
+            if (pack0 + 32u * u < whole) {
+                const In* p = from + lead + (pack0 + 32u * u) * N;
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) {
+                    if constexpr (Shifted)
+                        got[u][w] = loadShifted(p + w * (N / kWords), 16u);
+                    else
+                        got[u][w] = __ldg(reinterpret_cast<const uint4*>(p) + w);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < Unroll; ++u) {
+        if (pack0 + 32u * u < whole) {
+            const Pack<In, N>& in = *reinterpret_cast<const Pack<In, N>*>(&got[u]);
+            Pack<Out, N> out;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                out.e[e] = fromFloat<Out>(row >= 0 ? toFloat(in.e[e]) * a.scale : 0.0f);
+            *reinterpret_cast<Pack<Out, N>*>(to + lead + (pack0 + 32u * u) * N) = out;
+        }
+    }
+    if constexpr (Shifted) {
+        const uint32_t col = lane < 16u ? lane : lead + whole * N + lane - 16u;
+        if (segment == 0 && col < (lane < 16u ? lead : a.dim))
+            to[col] = fromFloat<Out>(row >= 0 ? toFloat(from[col]) * a.scale : 0.0f);
     }
 }
 
@@ -508,38 +663,6 @@ constexpr uint32_t kRowsInFlight = 8;
  *  16-byte word of any alignment; or ``group`` apart, element by element, for values whose
  *  last stride is not 1. */
 enum class Piece { Aligned, Shifted, Strided };
-
-/** The 16 bytes ``skip`` into 32 neighbouring ones. */
-__device__ __forceinline__ uint4 shiftWords(uint4 lo, uint4 hi, uint32_t skip)
-{
-    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    if (skip & 8u) {
-#pragma unroll
-        for (int j = 0; j < 6; ++j)
-            w[j] = w[j + 2];
-    }
-    if (skip & 4u) {
-#pragma unroll
-        for (int j = 0; j < 5; ++j)
-            w[j] = w[j + 1];
-    }
-    const uint32_t shift = (skip & 3u) * 8u;
-    return make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
-        __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
-}
-
-/** 16 bytes from any address of whole elements, of which ``valid`` bytes are wanted: the one or
- *  two aligned words that hold them (each holds a wanted byte, so it lies in mapped memory),
- *  shifted together. What lies past ``valid`` is unspecified. */
-__device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
-{
-    const uint64_t at = reinterpret_cast<uint64_t>(p);
-    const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
-    const uint32_t skip = uint32_t(at) & 15u;
-    const uint4 lo = __ldg(word);
-    const uint4 hi = skip + valid > 16u ? __ldg(word + 1) : make_uint4(0u, 0u, 0u, 0u);
-    return shiftWords(lo, hi, skip);
-}
 
 /** The columns ``col0``, ``col0 + apart``, ... of a row; ``apart`` is 1 but for Strided pieces. */
 template <class In, class Out, Piece P, int N>
@@ -1120,21 +1243,35 @@ void withIndex(uint32_t type, F&& f)
         f(int64_t{});
 }
 
-template <class In, class Out, class Tok, int N>
-void launchLookup(LookupArgs a, int64_t dim, cudaStream_t s, const char* who)
+template <class In, class Out, class Tok, int N, bool Shifted>
+void launchLookup(LookupArgs a, cudaStream_t s, const char* who)
 {
-    a.pieces = uint32_t(dim / N);
-    a.perRow = FastDiv(a.pieces);
-    const int64_t packs = a.n * int64_t(a.pieces);
-    // four packs a thread keep the memory busy; a plane too small to give every SM a few CTAs
-    // of those takes one each, so that more SMs share it
-    constexpr int kMany = N == 1 ? 8 : 4;
-    if (packs >= int64_t(smCount()) * 2 * kLookupThreads * kMany) {
-        const int64_t per = kLookupThreads * kMany;
-        lookupKernel<In, Out, Tok, N, kMany><<<gridOf((packs + per - 1) / per, who), kLookupThreads, 0, s>>>(a);
+    const int64_t packs = a.dim / N;
+    const int64_t sms = smCount();
+    if (packs >= 32) {
+        // four packs a lane keep the memory busy; a plane too small to give every SM a few CTAs
+        // of those takes one each, so that more SMs share it
+        const int unroll = a.n * packs >= sms * 2 * kLookupThreads * 4 ? 4 : 1;
+        a.pieces = uint32_t((packs + 32 * unroll - 1) / (32 * unroll));
+        const unsigned blocks = gridOf((a.n * a.pieces + kLookupThreads / 32 - 1) / (kLookupThreads / 32), who);
+        if (unroll == 1)
+            lookupWideKernel<In, Out, Tok, N, 1, Shifted><<<blocks, kLookupThreads, 0, s>>>(a);
+        else
+            lookupWideKernel<In, Out, Tok, N, 4, Shifted><<<blocks, kLookupThreads, 0, s>>>(a);
     } else {
-        lookupKernel<In, Out, Tok, N, 1>
-            <<<gridOf((packs + kLookupThreads - 1) / kLookupThreads, who), kLookupThreads, 0, s>>>(a);
+        a.pieces = Shifted ? (a.dim + N - 1) / N + 1 : a.dim / N;
+        a.perRow = FastDiv(a.pieces);
+        const int64_t all = a.n * int64_t(a.pieces);
+        const int unroll = all >= sms * 2 * kLookupThreads * 4 ? 4 : 1;
+        const unsigned blocks = gridOf((all + kLookupThreads * unroll - 1) / (kLookupThreads * unroll), who);
+        if (Shifted && unroll == 1)
+            lookupShiftedKernel<In, Out, Tok, N, 1><<<blocks, kLookupThreads, 0, s>>>(a);
+        else if (Shifted)
+            lookupShiftedKernel<In, Out, Tok, N, 4><<<blocks, kLookupThreads, 0, s>>>(a);
+        else if (unroll == 1)
+            lookupKernel<In, Out, Tok, N, 1><<<blocks, kLookupThreads, 0, s>>>(a);
+        else
+            lookupKernel<In, Out, Tok, N, 4><<<blocks, kLookupThreads, 0, s>>>(a);
     }
     launchCheck(who);
 }
@@ -1160,6 +1297,7 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
     a.valueBatch = d.value_strides[0];
     a.valueSeq = d.value_strides[1];
     a.n = d.batch * d.seq;
+    a.dim = uint32_t(d.dim);
     a.perBatch = FastDiv(uint32_t(d.seq));
     a.flat = isFlat(d.batch, d.seq, a.tokenBatch, a.tokenSeq) && isFlat(d.batch, d.seq, a.valueBatch, a.valueSeq);
     a.scale = float(d.scale);
@@ -1176,9 +1314,9 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
                     && d.table_stride * inBytes % 16 == 0 && d.value_strides[0] * outBytes % 16 == 0
                     && d.value_strides[1] * outBytes % 16 == 0;
                 if (wide)
-                    launchLookup<In, Out, Tok, N>(a, d.dim, s, who);
+                    launchLookup<In, Out, Tok, N, false>(a, s, who);
                 else
-                    launchLookup<In, Out, Tok, 1>(a, d.dim, s, who);
+                    launchLookup<In, Out, Tok, N, true>(a, s, who);
             });
         });
     });
