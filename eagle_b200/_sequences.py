@@ -21,6 +21,7 @@ No operator here records an autograd graph.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 
 from . import _abi
@@ -78,29 +79,40 @@ def _apart(out, what, *inputs):
                 raise ValueError(f"{what} overlaps an input")
 
 
+def _raw_stream(device):
+    """The handle of ``device``'s current stream."""
+    torch = _t()
+    global _current
+    if _current is None:  # the handle alone, where this torch offers it: a call a step makes every time
+        _current = getattr(torch._C, "_cuda_getCurrentRawStream",
+                           lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return _current(device.index)
+
+
+_current = None
+
+
 class _Call:
     """A prepared call: ``_desc`` and the C entry, enqueued on the tensors' device."""
 
     def _prepare(self, entry, desc, device, owned):
-        torch = _t()
         self.device = device
         self._entry = getattr(_abi.lib(), entry)
         self._desc = desc
         self._ref = ctypes.byref(desc)
         self._owned = owned  # allocated here, on this stream
-        self._home = torch.cuda.current_stream(device).cuda_stream
+        self._home = _raw_stream(device)
 
     def _enqueue(self, stream):
-        torch = _t()
         if stream is None:
-            handle = torch.cuda.current_stream(self.device).cuda_stream
+            handle = _raw_stream(self.device)
         else:
             if stream.device != self.device:
                 raise ValueError(f"the stream is on {stream.device}, the tensors on {self.device}")
             handle = stream.cuda_stream
         if handle != self._home:
             # the allocator may hand these out again once they are dropped: not before this stream is past the call
-            s = stream if stream is not None else torch.cuda.current_stream(self.device)
+            s = stream if stream is not None else _t().cuda.current_stream(self.device)
             for t in self._owned:
                 t.record_stream(s)
         self._desc.stream = handle
@@ -109,10 +121,9 @@ class _Call:
             _abi.check(status)
 
 
-def _on(stream, device):
+def _on(stream):
     """Allocations on ``stream``, where the call runs."""
-    torch = _t()
-    return torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(device))
+    return _t().cuda.stream(stream) if stream is not None else contextlib.nullcontext()
 
 
 def _query(entry, desc, device):
@@ -216,7 +227,7 @@ class Embedding(_Call):
 
 def embedding(table, tokens, *, scale: float = 1.0, first: int = 0, out=None, dtype=None, stream=None):
     """``scale * table[tokens - first]``, zeros for tokens the table has no row for (:class:`Embedding`)."""
-    with _on(stream, _cuda(table, "the table").device):
+    with _on(stream):
         return Embedding(table, tokens, scale=scale, first=first, out=out, dtype=dtype)(stream)
 
 
@@ -272,7 +283,7 @@ class EmbeddingGrad(_Call):
 def embedding_grad(grad, tokens, rows: int, *, scale: float = 1.0, first: int = 0, out=None, dtype=None,
                    accumulate: bool = False, stream=None):
     """The gradient of :func:`embedding`'s table from that of its output (:class:`EmbeddingGrad`)."""
-    with _on(stream, _cuda(grad, "grad").device):
+    with _on(stream):
         return EmbeddingGrad(grad, tokens, rows, scale=scale, first=first, out=out, dtype=dtype,
                              accumulate=accumulate)(stream)
 
@@ -360,7 +371,7 @@ class BlockTables(_Call):
 
 def block_tables(lengths, held, table, pool, count, *, block: int, used=None, terminated=None, stream=None):
     """Grow ``table`` to ``lengths`` from the free ``pool``: ``(blocks, cells)`` (:class:`BlockTables`)."""
-    with _on(stream, _cuda(table, "the table").device):
+    with _on(stream):
         return BlockTables(lengths, held, table, pool, count, block=block, used=used, terminated=terminated)(stream)
 
 
@@ -409,5 +420,5 @@ class SlotMap(_Call):
 
 def slot_map(table, start, fresh, capacity: int, *, block: int, terminated=None, dtype=None, stream=None):
     """The packed new tokens' ``(slots, positions, requests, offsets)`` (:class:`SlotMap`)."""
-    with _on(stream, _cuda(table, "the table").device):
+    with _on(stream):
         return SlotMap(table, start, fresh, capacity, block=block, terminated=terminated, dtype=dtype)(stream)

@@ -209,6 +209,14 @@ __global__ __launch_bounds__(kLookupThreads) void lookupShiftedKernel(LookupArgs
 // alignment are worked out once for all of them (per pack, that took more time than the
 // bytes: 128 us against 210 at 65536 rows of 16 KB, and 8 against 20 at 10007 of 2002 bytes).
 
+/** 32 bytes in one load (two of 16 bytes each touch every sector twice); ``p`` is 32-byte aligned. */
+__device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi)
+{
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
+                 : "l"(p));
+}
+
 /** ``Shifted``: packs are cut where the output's 16-byte words begin and read from wherever that
  *  falls in the table; the up to N - 1 values before the first and after the last are taken
  *  one to a lane. */
@@ -216,11 +224,11 @@ template <class In, class Out, class Tok, int N, int Unroll, bool Shifted>
 __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
 {
     const uint32_t lane = threadIdx.x & 31u;
-    const uint64_t id = uint64_t(blockIdx.x) * (kLookupThreads / 32) + (threadIdx.x >> 5);
-    const int64_t t = int64_t(id / a.pieces);  // pieces: warps to a row
+    const uint32_t id = blockIdx.x * (kLookupThreads / 32) + (threadIdx.x >> 5);
+    const int64_t t = a.perRow(id);  // pieces: warps to a row
     if (t >= a.n)
         return;
-    const uint32_t segment = uint32_t(id - uint64_t(t) * a.pieces);
+    const uint32_t segment = id - uint32_t(t) * a.pieces;
     int64_t row, at;
     placeOf<Tok>(a, t, row, at);
     const In* from = reinterpret_cast<const In*>(a.table) + (row < 0 ? 0 : row * a.tableStride);
@@ -241,8 +249,10 @@ __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
                 for (int w = 0; w < kWords; ++w) {
                     if constexpr (Shifted)
                         got[u][w] = loadShifted(p + w * (N / kWords), 16u);
-                    else
-                        got[u][w] = __ldg(reinterpret_cast<const uint4*>(p) + w);
+                    else if constexpr (kWords == 1)
+                        got[u][w] = __ldg(reinterpret_cast<const uint4*>(p));
+                    else if (w == 0)
+                        load32(p, got[u][0], got[u][kWords - 1]);
                 }
             }
         }
@@ -255,7 +265,10 @@ __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 out.e[e] = fromFloat<Out>(row >= 0 ? toFloat(in.e[e]) * a.scale : 0.0f);
-            *reinterpret_cast<Pack<Out, N>*>(to + lead + (pack0 + 32u * u) * N) = out;
+            uint4* words = reinterpret_cast<uint4*>(to + lead + (pack0 + 32u * u) * N);
+#pragma unroll
+            for (int w = 0; w < int(sizeof(out)) / 16; ++w)
+                __stcs(words + w, reinterpret_cast<const uint4*>(&out)[w]);  // L2 is for the table's rows
         }
     }
     if constexpr (Shifted) {
@@ -1253,7 +1266,11 @@ void launchLookup(LookupArgs a, cudaStream_t s, const char* who)
         // of those takes one each, so that more SMs share it
         const int unroll = a.n * packs >= sms * 2 * kLookupThreads * 4 ? 4 : 1;
         a.pieces = uint32_t((packs + 32 * unroll - 1) / (32 * unroll));
-        const unsigned blocks = gridOf((a.n * a.pieces + kLookupThreads / 32 - 1) / (kLookupThreads / 32), who);
+        a.perRow = FastDiv(a.pieces);
+        const int64_t warps = a.n * a.pieces;
+        if (warps > 0x7fffff00ll)
+            unsupported(std::string(who) + ": the call is larger than one launch holds");
+        const unsigned blocks = unsigned((warps + kLookupThreads / 32 - 1) / (kLookupThreads / 32));
         if (unroll == 1)
             lookupWideKernel<In, Out, Tok, N, 1, Shifted><<<blocks, kLookupThreads, 0, s>>>(a);
         else
@@ -1310,8 +1327,9 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
                 using Tok = decltype(tok);
                 // a pack is 16 bytes of the narrower type; every row has to start on its words
                 constexpr int N = 16 / int(sizeof(In) < sizeof(Out) ? sizeof(In) : sizeof(Out));
-                const bool wide = d.dim % N == 0 && d.table % 16 == 0 && d.values % 16 == 0
-                    && d.table_stride * inBytes % 16 == 0 && d.value_strides[0] * outBytes % 16 == 0
+                constexpr int64_t kInPack = N * int(sizeof(In));
+                const bool wide = d.dim % N == 0 && d.table % kInPack == 0 && d.values % 16 == 0
+                    && d.table_stride * inBytes % kInPack == 0 && d.value_strides[0] * outBytes % 16 == 0
                     && d.value_strides[1] * outBytes % 16 == 0;
                 if (wide)
                     launchLookup<In, Out, Tok, N, false>(a, s, who);

@@ -19,9 +19,10 @@
 namespace eb {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr uint32_t kScanInBlock = 8192;
-constexpr uint32_t kScanItems = kScanInBlock / kThreads;
+constexpr int kThreads = 1024;
+constexpr uint32_t kItems = 8;                           // requests a thread scans
+constexpr uint32_t kScanInBlock = kThreads * kItems;     // 8192
+constexpr uint32_t kWarps = kThreads / 32;
 
 struct PagedArgs {
     uint32_t requests;
@@ -56,51 +57,43 @@ __device__ __forceinline__ int64_t lengthAt(const void* p, uint32_t r)
     return v < 0 ? 0 : v;
 }
 
-__device__ __forceinline__ bool isLive(const PagedArgs& a, uint32_t r)
-{
-    return a.terminated == nullptr || __ldg(a.terminated + r) == 0;
-}
-
 // ------------------------------------------------------------------ what each request adds
 
-/** The blocks request r holds, clipped to its row. */
-__device__ __forceinline__ uint32_t heldOf(const PagedArgs& a, uint32_t r)
-{
-    const int64_t h = __ldg(a.held + r);
-    return uint32_t(h < 0 ? 0 : (h < a.width ? h : a.width));
-}
+/** A request's state: its reads do not wait for one another. */
+struct Blocks {
+    uint32_t held;   // clipped to the row
+    uint32_t need;   // width + 1 where the row cannot hold them
+    bool live;
+    bool wide;       // more than the row holds
 
-/** Blocks a live request's length needs; width + 1 where its row cannot hold them. */
-template <class Len>
-__device__ __forceinline__ uint32_t needOf(const PagedArgs& a, uint32_t r)
-{
-    if (!isLive(a, r))
-        return 0;
-    const int64_t length = lengthAt<Len>(a.lengths, r);
-    if (length > a.room)
-        return uint32_t(a.width) + 1u;
-    const uint32_t whole = a.perBlock(uint32_t(length));
-    return whole + (whole * a.perBlock.d != uint32_t(length) ? 1u : 0u);
-}
-
-struct NewBlocks {
     template <class Len>
-    static __device__ __forceinline__ uint32_t of(const PagedArgs& a, uint32_t r)
+    __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
     {
-        const uint32_t need = needOf<Len>(a, r), held = heldOf(a, r);
-        return need > uint32_t(a.width) || need <= held ? 0u : need - held;
+        const uint8_t ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
+        const int64_t length = lengthAt<Len>(a.lengths, r);
+        const int64_t h = __ldg(a.held + r);
+        held = uint32_t(h < 0 ? 0 : (h < a.width ? h : a.width));
+        live = ended == 0;
+        wide = live && length > a.room;
+        const uint32_t l = uint32_t(length < a.room ? length : a.room);
+        const uint32_t whole = a.perBlock(l);
+        need = live ? whole + (whole * a.perBlock.d != l ? 1u : 0u) : 0u;
     }
+    /** The blocks it asks for. */
+    __device__ __forceinline__ uint32_t adds() const { return wide || need <= held ? 0u : need - held; }
 };
 
-struct NewTokens {
+struct Tokens {
+    uint32_t fresh;
+
     template <class Len>
-    static __device__ __forceinline__ uint32_t of(const PagedArgs& a, uint32_t r)
+    __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
     {
-        if (!isLive(a, r))
-            return 0;
+        const uint8_t ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
         const int64_t f = lengthAt<Len>(a.fresh, r);
-        return uint32_t(f < 0x7fffffffll ? f : 0x7fffffffll);
+        fresh = ended != 0 ? 0u : uint32_t(f < 0x7fffffffll ? f : 0x7fffffffll);
     }
+    __device__ __forceinline__ uint32_t adds() const { return fresh; }
 };
 
 // ------------------------------------------------------------------ the scan
@@ -108,28 +101,32 @@ struct NewTokens {
 /** Sums past this read as this: no pool and no list is as long. */
 constexpr uint64_t kMost = 0x7fffffffull;
 
-/** The inclusive scan of What over requests [from, from + kScanInBlock) into ``upto`` (shared
- *  memory), on top of ``carry``; returns the new carry. */
+/** Requests [from, from + kScanInBlock): thread t reads ``items`` neighbours from ``t * items`` on
+ *  (as few as cover them), all at once; their inclusive sums on top of ``carry`` go to
+ *  ``upto``. Returns the new carry. */
 template <class What, class Len>
-__device__ __forceinline__ uint64_t scanBlock(const PagedArgs& a, uint32_t from, uint64_t carry, uint32_t* upto,
-    uint64_t* scratch)
+__device__ __forceinline__ uint64_t scanBlock(const PagedArgs& a, uint32_t from, uint64_t carry, What (&what)[kItems],
+    uint32_t* upto, uint64_t* scratch)
 {
     const uint32_t m = min(a.requests - from, kScanInBlock);
-    // as few items a thread as cover them, so that a small batch is not one thread's work
-    const uint32_t items = (m + kThreads - 1) / kThreads;
-    for (uint32_t i = threadIdx.x; i < m; i += kThreads)
-        upto[i] = What::template of<Len>(a, from + i);
-    __syncthreads();
-    const uint32_t first = threadIdx.x * items, last = min(first + items, m);
+    const uint32_t items = (m + kThreads - 1) / kThreads, first = threadIdx.x * items;
+#pragma unroll
+    for (uint32_t k = 0; k < kItems; ++k)
+        if (k < items && first + k < m)
+            what[k].template read<Len>(a, from + first + k);
     uint64_t mine = 0;
-    for (uint32_t i = first; i < last; ++i)
-        mine += upto[i];
+#pragma unroll
+    for (uint32_t k = 0; k < kItems; ++k)
+        if (k < items && first + k < m)
+            mine += what[k].adds();
     uint64_t total = 0;
     uint64_t sum = carry + blockExclusiveSum(mine, total, scratch);
-    for (uint32_t i = first; i < last; ++i) {
-        sum += upto[i];
-        upto[i] = uint32_t(sum < kMost ? sum : kMost);
-    }
+#pragma unroll
+    for (uint32_t k = 0; k < kItems; ++k)
+        if (k < items && first + k < m) {
+            sum += what[k].adds();
+            upto[first + k] = uint32_t(sum < kMost ? sum : kMost);
+        }
     __syncthreads();
     return carry + total;
 }
@@ -140,11 +137,13 @@ __global__ __launch_bounds__(kThreads) void scanKernel(PagedArgs a)
 {
     __shared__ uint32_t upto[kScanInBlock];
     __shared__ uint64_t scratch[33];
+    letNextKernelStart();
     if (threadIdx.x == 0 && a.cells != nullptr)
         a.cells[1] = 0;
     uint64_t carry = 0;
     for (uint32_t from = 0; from < a.requests; from += kScanInBlock) {
-        carry = scanBlock<What, Len>(a, from, carry, upto, scratch);
+        What what[kItems];
+        carry = scanBlock<What, Len>(a, from, carry, what, upto, scratch);
         for (uint32_t i = threadIdx.x; i < min(a.requests - from, kScanInBlock); i += kThreads)
             a.upto[from + i] = upto[i];
         __syncthreads();
@@ -166,51 +165,88 @@ __device__ __forceinline__ uint32_t requestOf(const uint32_t* upto, uint32_t req
     return low;
 }
 
+/** The same from a request ``r`` at or before it: mostly that one or the next; a row of requests
+ *  that add nothing is searched over. */
+__device__ __forceinline__ uint32_t requestFrom(const uint32_t* upto, uint32_t requests, uint32_t q, uint32_t r)
+{
+    if (r < requests && upto[r] <= q && ++r < requests && upto[r] <= q)
+        r = requestOf(upto, requests, q, r + 1u);
+    return r;
+}
+
 // ------------------------------------------------------------------ block tables
 
+constexpr uint32_t kEntries = 128;  // of the pool's front per warp and step: one search for all of them
+
+/** Every CTA scans the requests (or reads the scan from scratch) and takes its share of the
+ *  lists; the last one also writes what each request holds and the cells. */
 template <class Len, bool InBlock>
 __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 {
     __shared__ uint32_t sUpto[InBlock ? kScanInBlock : 1];
+    __shared__ uint32_t sGone[InBlock ? kScanInBlock / 32 : 1];  // a bit per terminated request
     __shared__ uint64_t scratch[33];
     __shared__ uint32_t sShort;
     const uint32_t* upto = InBlock ? sUpto : a.upto;
-    if (threadIdx.x == 0)
-        sShort = 0;
-    if constexpr (InBlock)
-        (void)scanBlock<NewBlocks, Len>(a, 0, 0, sUpto, scratch);
-    else
-        __syncthreads();
+    const bool returns = a.used != nullptr && a.terminated != nullptr;
+    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
+                   warps = gridDim.x * kWarps;
+    if constexpr (!InBlock)
+        waitForKernelBefore();
     const uint32_t given = __ldg(a.count);
     const uint32_t available = uint64_t(given) > uint64_t(a.poolSize) ? 0u : given;
-    // the sums never fall, so the requests that fit with new blocks are the first ones up to
+    if (threadIdx.x == 0)
+        sShort = 0;
+    Blocks what[kItems];
+    if constexpr (InBlock) {
+        for (uint32_t i = threadIdx.x; returns && i < (a.requests + 31) / 32; i += kThreads)
+            sGone[i] = 0;
+        (void)scanBlock<Blocks, Len>(a, 0, 0, what, sUpto, scratch);
+    } else {
+        __syncthreads();
+    }
+    // the sums never fall, so the requests that fit with new blocks are the first ones, up to
     // the last sum within the pool
     const uint32_t fitting = requestOf(upto, a.requests, available);
     const uint32_t taken = fitting == 0 ? 0u : upto[fitting - 1];
 
-    // what each request holds now, and who was left short; a CTA's share of them
+    const bool last = blockIdx.x == gridDim.x - 1;
     uint32_t missed = 0;
-    for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r < a.requests; r += gridDim.x * kThreads) {
-        const uint32_t held = heldOf(a, r), need = needOf<Len>(a, r);
-        uint32_t now = held;
-        if (!isLive(a, r))
-            now = 0;
-        else if (need > held && need <= uint32_t(a.width) && upto[r] <= available)
-            now = need;
-        else if (need > held)
-            ++missed;
-        a.blocks[r] = int32_t(now);
+    auto settle = [&](const Blocks& w, uint32_t r) {
+        const bool fits = !w.wide && (w.need <= w.held || upto[r] <= available);
+        a.blocks[r] = int32_t(!w.live ? 0u : (fits && w.need > w.held ? w.need : w.held));
+        missed += fits ? 0u : 1u;
+    };
+    if constexpr (InBlock) {
+        const uint32_t items = (a.requests + kThreads - 1) / kThreads, first = threadIdx.x * items;
+#pragma unroll
+        for (uint32_t k = 0; k < kItems; ++k) {
+            if (k < items && first + k < a.requests) {
+                if (last)
+                    settle(what[k], first + k);
+                if (returns && !what[k].live && what[k].held > 0)
+                    atomicOr(sGone + ((first + k) >> 5), 1u << ((first + k) & 31u));
+            }
+        }
+        __syncthreads();
+    } else {
+        for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r < a.requests; r += gridDim.x * kThreads) {
+            Blocks w;
+            w.read<Len>(a, r);
+            settle(w, r);
+        }
     }
 
     // the blocks of terminated requests, a warp per request
-    if (a.used != nullptr && a.terminated != nullptr) {
-        const uint32_t lane = threadIdx.x & 31u;
-        for (uint32_t r = (blockIdx.x * kThreads + threadIdx.x) >> 5; r < a.requests; r += gridDim.x * (kThreads / 32)) {
-            if (isLive(a, r))
+    if (returns) {
+        for (uint32_t r = warp; r < a.requests; r += warps) {
+            if (InBlock ? ((sGone[r >> 5] >> (r & 31u)) & 1u) == 0 : __ldg(a.terminated + r) == 0)
                 continue;
-            const uint32_t held = heldOf(a, r);
+            const int64_t h = __ldg(a.held + r);
+            const int64_t held = h < a.width ? h : a.width;
             const int32_t* row = a.table + int64_t(r) * a.tableStride;
-            for (uint32_t j = lane; j < held; j += 32u) {
+#pragma unroll 4
+            for (int64_t j = lane; j < held; j += 32) {
                 const int64_t id = row[j];
                 if (id >= 0 && id < a.usedSize)
                     a.used[id] = 0;
@@ -218,41 +254,43 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
         }
     }
 
-    // the pool's front, one entry per thread and step
-    for (uint32_t q = blockIdx.x * kThreads + threadIdx.x; q < taken; q += gridDim.x * kThreads) {
-        const uint32_t r = requestOf(upto, a.requests, q);
-        const uint32_t before = r == 0 ? 0u : upto[r - 1];
-        const int32_t id = __ldg(a.pool + q);
-        a.table[int64_t(r) * a.tableStride + heldOf(a, r) + (q - before)] = id;
-        if (a.used != nullptr && id >= 0 && int64_t(id) < a.usedSize)
-            a.used[id] = 1;
-    }
-
-    if constexpr (InBlock) {
-        // few enough requests for one CTA to count them all over again
-        if (blockIdx.x != gridDim.x - 1)
-            return;
-        missed = 0;
-        for (uint32_t r = threadIdx.x; r < a.requests; r += kThreads) {
-            const uint32_t held = heldOf(a, r), need = needOf<Len>(a, r);
-            if (need > held && (need > uint32_t(a.width) || upto[r] > available))
-                ++missed;
+    // the front of the pool
+    for (uint64_t q0 = uint64_t(warp) * kEntries; q0 < taken; q0 += uint64_t(warps) * kEntries) {
+        const uint32_t r0 = requestOf(upto, a.requests, uint32_t(q0));
+        int32_t id[kEntries / 32];
+#pragma unroll
+        for (uint32_t k = 0; k < kEntries / 32; ++k) {
+            const uint64_t q = q0 + 32u * k + lane;
+            id[k] = q < taken ? __ldg(a.pool + q) : -1;
+        }
+        uint32_t r = r0;
+#pragma unroll
+        for (uint32_t k = 0; k < kEntries / 32; ++k) {
+            const uint64_t q = q0 + 32u * k + lane;
+            if (q >= taken)
+                break;
+            r = requestFrom(upto, a.requests, uint32_t(q), r);
+            const uint32_t before = r == 0 ? 0u : upto[r - 1];
+            const int64_t h = __ldg(a.held + r);
+            a.table[int64_t(r) * a.tableStride + (h < 0 ? 0 : h) + (uint32_t(q) - before)] = id[k];
+            if (a.used != nullptr && id[k] >= 0 && int64_t(id[k]) < a.usedSize)
+                a.used[id[k]] = 1;
         }
     }
+
+    if (InBlock && !last)
+        return;
     missed = warpSum(missed);
-    if ((threadIdx.x & 31u) == 0 && missed != 0)
+    if (lane == 0 && missed != 0)
         atomicAdd(&sShort, missed);
     __syncthreads();
     if (threadIdx.x == 0) {
-        if constexpr (InBlock) {
+        if (last)
             a.cells[0] = taken;
+        if (InBlock)
             a.cells[1] = sShort;
-        } else {  // zeroed by the scan
-            if (blockIdx.x == 0)
-                a.cells[0] = taken;
-            if (sShort != 0)
-                atomicAdd(a.cells + 1, sShort);
-        }
+        else if (sShort != 0)  // zeroed by the scan
+            atomicAdd(a.cells + 1, sShort);
     }
 }
 
@@ -266,22 +304,27 @@ __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
     __shared__ uint32_t sUpto[InBlock ? kScanInBlock : 1];
     __shared__ uint64_t scratch[33];
     const uint32_t* upto = InBlock ? sUpto : a.upto;
-    if constexpr (InBlock)
-        (void)scanBlock<NewTokens, Len>(a, 0, 0, sUpto, scratch);
-    for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r <= a.requests; r += gridDim.x * kThreads)
-        a.offsets[r] = r == 0 ? 0 : int32_t(upto[r - 1]);
-    const uint64_t step = uint64_t(gridDim.x) * kThreads * kTokens;
-    for (uint64_t q0 = (uint64_t(blockIdx.x) * kThreads + threadIdx.x) * kTokens; q0 < a.capacity; q0 += step) {
-        uint32_t r = requestOf(upto, a.requests, uint32_t(q0));
+    if constexpr (InBlock) {
+        Tokens what[kItems];
+        (void)scanBlock<Tokens, Len>(a, 0, 0, what, sUpto, scratch);
+    } else {
+        waitForKernelBefore();
+    }
+    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
+                   warps = gridDim.x * kWarps;
+    for (uint64_t w0 = uint64_t(warp) * 32u * kTokens; w0 < a.capacity; w0 += uint64_t(warps) * 32u * kTokens) {
+        const uint32_t r0 = requestOf(upto, a.requests, uint32_t(w0));  // one search for the warp's tokens
+        const uint64_t q0 = w0 + lane * kTokens;
+        uint32_t r = r0;
+        if (q0 < a.capacity)
+            r = requestFrom(upto, a.requests, uint32_t(q0), r);
         Pack<Slot, kTokens> slot;
         Pack<Len, kTokens> position;
         Pack<int32_t, kTokens> request;
 #pragma unroll
         for (uint32_t k = 0; k < kTokens; ++k) {
             const uint32_t q = uint32_t(q0) + k;
-            // the next request is mostly the neighbour; a row of them without tokens is searched over
-            if (r < a.requests && upto[r] <= q && ++r < a.requests && upto[r] <= q)
-                r = requestOf(upto, a.requests, q, r + 1u);
+            r = requestFrom(upto, a.requests, q, r);
             slot.e[k] = Slot(-1);
             position.e[k] = 0;
             request.e[k] = -1;
@@ -314,6 +357,8 @@ __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
             }
         }
     }
+    for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r <= a.requests; r += gridDim.x * kThreads)
+        a.offsets[r] = r == 0 ? 0 : int32_t(upto[r - 1]);
 }
 
 // ------------------------------------------------------------------ host side
@@ -408,16 +453,16 @@ EB_API eagle_backend_status eagle_backend_x_b200_block_tables(eagle_b200_paged_d
         const cudaStream_t s = seamStream(d.stream);
         // the entries the call can write at most, an SM per CTA
         const int64_t most = std::max(std::min(d.pool_size, d.requests * d.width), d.requests);
-        const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(smCount(), (most + kThreads - 1) / kThreads));
+        const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(smCount(), (most + kWarps * kEntries - 1) / (kWarps * kEntries)));
         withLength(d.length_type, [&](auto len) {
             using Len = decltype(len);
             if (d.requests <= int64_t(kScanInBlock)) {
                 blockTablesKernel<Len, true><<<unsigned(grid), kThreads, 0, s>>>(a);
+                launchCheck(who);
             } else {
-                launchScan<NewBlocks, Len>(a, s, who);
-                blockTablesKernel<Len, false><<<unsigned(grid), kThreads, 0, s>>>(a);
+                launchScan<Blocks, Len>(a, s, who);
+                launchBehind(blockTablesKernel<Len, false>, unsigned(grid), kThreads, 0, s, a, who);
             }
-            launchCheck(who);
         });
     });
 }
@@ -469,11 +514,11 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
                 using Slot = decltype(slot);
                 if (d.requests <= int64_t(kScanInBlock)) {
                     slotMapKernel<Len, Slot, true><<<unsigned(grid), kThreads, 0, s>>>(a);
+                    launchCheck(who);
                 } else {
-                    launchScan<NewTokens, Len>(a, s, who);
-                    slotMapKernel<Len, Slot, false><<<unsigned(grid), kThreads, 0, s>>>(a);
+                    launchScan<Tokens, Len>(a, s, who);
+                    launchBehind(slotMapKernel<Len, Slot, false>, unsigned(grid), kThreads, 0, s, a, who);
                 }
-                launchCheck(who);
             });
         });
     });
