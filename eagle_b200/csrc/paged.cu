@@ -10,6 +10,8 @@
 // are bound by the launch and by one chain of dependent reads. Up to kScanInBlock
 // requests every CTA scans all of them itself into shared memory -- one launch, no wait on
 // another CTA; past it the scan is a kernel of its own (one CTA) that leaves it in scratch.
+// CTAs are of 256 threads where those scan the requests (2048), which starts and meets at
+// its barriers sooner than 1024.
 #include "sequences.cuh"
 
 #include <algorithm>
@@ -19,10 +21,9 @@
 namespace eb {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr uint32_t kItems = 8;                           // requests a thread scans
-constexpr uint32_t kScanInBlock = kThreads * kItems;     // 8192
-constexpr uint32_t kWarps = kThreads / 32;
+constexpr uint32_t kItems = 8;  // requests a thread scans
+constexpr int kSmall = 256, kLarge = 1024;
+constexpr uint32_t kScanInBlock = kLarge * kItems;  // 8192
 
 struct PagedArgs {
     uint32_t requests;
@@ -47,6 +48,7 @@ struct PagedArgs {
     void* positions;
     int32_t* tokenRequests;
     int32_t* offsets;
+    uint32_t pieces; // warps' shares of a row of the table
     uint32_t* upto;  // scratch: the inclusive scan (more than kScanInBlock requests)
 };
 
@@ -59,13 +61,13 @@ __device__ __forceinline__ int64_t lengthAt(const void* p, uint32_t r)
 
 // ------------------------------------------------------------------ what each request adds
 
-/** A request's state: its reads do not wait for one another. */
+/** A request's blocks: its reads do not wait for one another. */
 struct Blocks {
-    uint32_t held;   // clipped to the row
-    uint32_t need;   // width + 1 where the row cannot hold them
+    uint32_t held;  // clipped to the row
+    uint32_t need;  // width + 1 where the row cannot hold them
     bool live;
-    bool wide;       // more than the row holds
 
+    using Kept = uint2;  // {held, need}, the highest bit of held set where it is terminated
     template <class Len>
     __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
     {
@@ -74,77 +76,141 @@ struct Blocks {
         const int64_t h = __ldg(a.held + r);
         held = uint32_t(h < 0 ? 0 : (h < a.width ? h : a.width));
         live = ended == 0;
-        wide = live && length > a.room;
         const uint32_t l = uint32_t(length < a.room ? length : a.room);
         const uint32_t whole = a.perBlock(l);
-        need = live ? whole + (whole * a.perBlock.d != l ? 1u : 0u) : 0u;
+        need = length > a.room ? uint32_t(a.width) + 1u : whole + (whole * a.perBlock.d != l ? 1u : 0u);
+        need = live ? need : 0u;
     }
     /** The blocks it asks for. */
-    __device__ __forceinline__ uint32_t adds() const { return wide || need <= held ? 0u : need - held; }
+    __device__ __forceinline__ uint32_t adds(const PagedArgs& a) const
+    {
+        return need > uint32_t(a.width) || need <= held ? 0u : need - held;
+    }
+    __device__ __forceinline__ Kept kept() const { return make_uint2(held | (live ? 0u : 0x80000000u), need); }
+    static __device__ __forceinline__ Blocks of(Kept k)
+    {
+        Blocks b;
+        b.held = k.x & 0x7fffffffu;
+        b.live = (k.x >> 31) == 0;
+        b.need = k.y;
+        return b;
+    }
 };
 
+/** A request's new tokens. */
 struct Tokens {
     uint32_t fresh;
+    int64_t start;
 
+    using Kept = int64_t;
     template <class Len>
     __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
     {
         const uint8_t ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
         const int64_t f = lengthAt<Len>(a.fresh, r);
+        start = lengthAt<Len>(a.start, r);
         fresh = ended != 0 ? 0u : uint32_t(f < 0x7fffffffll ? f : 0x7fffffffll);
     }
-    __device__ __forceinline__ uint32_t adds() const { return fresh; }
+    __device__ __forceinline__ uint32_t adds(const PagedArgs&) const { return fresh; }
+    __device__ __forceinline__ Kept kept() const { return start; }
 };
 
 // ------------------------------------------------------------------ the scan
 
-/** Sums past this read as this: no pool and no list is as long. */
-constexpr uint64_t kMost = 0x7fffffffull;
+/** Sums past this read as this: no pool and no list is as long. So 32 bits hold them. */
+constexpr uint32_t kMost = 0x7fffffffu;
 
-/** Requests [from, from + kScanInBlock): thread t reads ``items`` neighbours from ``t * items`` on
- *  (as few as cover them), all at once; their inclusive sums on top of ``carry`` go to
- *  ``upto``. Returns the new carry. */
-template <class What, class Len>
-__device__ __forceinline__ uint64_t scanBlock(const PagedArgs& a, uint32_t from, uint64_t carry, What (&what)[kItems],
-    uint32_t* upto, uint64_t* scratch)
+__device__ __forceinline__ uint32_t addUpTo(uint32_t a, uint32_t b) { return min(a + b, kMost); }  // both at most kMost
+
+__device__ __forceinline__ uint32_t warpInclusive(uint32_t v)
 {
-    const uint32_t m = min(a.requests - from, kScanInBlock);
-    const uint32_t items = (m + kThreads - 1) / kThreads, first = threadIdx.x * items;
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (uint32_t off = 1; off < 32; off <<= 1) {
+        const uint32_t o = __shfl_up_sync(kFull, v, off);
+        if (lane >= off)
+            v = addUpTo(v, o);
+    }
+    return v;
+}
+
+constexpr uint32_t kMaxSegments = kItems * (kLarge / 32);
+
+/** Requests [from, from + Threads * kItems), Threads neighbours at a time (a thread reading its own
+ *  neighbours instead took 13 us for 8191 requests), all read at once: their inclusive sums on
+ *  top of ``carry`` go to ``upto`` and what they keep to ``kept``. Every warp scans its 32 of each
+ *  step, the first one those segments' sums. Returns the new carry. ``segment`` is kMaxSegments
+ *  + 1 words of shared memory. */
+template <int Threads, class What, class Len>
+__device__ __forceinline__ uint32_t scanBlock(const PagedArgs& a, uint32_t from, uint32_t carry, uint32_t* upto,
+    typename What::Kept* kept, uint32_t* segment)
+{
+    constexpr uint32_t kWarps = Threads / 32;
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    const uint32_t m = min(a.requests - from, uint32_t(Threads) * kItems);
+    const uint32_t items = (m + Threads - 1) / Threads;
+    What what[kItems];
+    uint32_t sum[kItems];
 #pragma unroll
     for (uint32_t k = 0; k < kItems; ++k)
-        if (k < items && first + k < m)
-            what[k].template read<Len>(a, from + first + k);
-    uint64_t mine = 0;
+        if (k < items && k * Threads + threadIdx.x < m)
+            what[k].template read<Len>(a, from + k * Threads + threadIdx.x);
 #pragma unroll
-    for (uint32_t k = 0; k < kItems; ++k)
-        if (k < items && first + k < m)
-            mine += what[k].adds();
-    uint64_t total = 0;
-    uint64_t sum = carry + blockExclusiveSum(mine, total, scratch);
-#pragma unroll
-    for (uint32_t k = 0; k < kItems; ++k)
-        if (k < items && first + k < m) {
-            sum += what[k].adds();
-            upto[first + k] = uint32_t(sum < kMost ? sum : kMost);
+    for (uint32_t k = 0; k < kItems; ++k) {
+        if (k < items) {
+            const uint32_t i = k * Threads + threadIdx.x;
+            sum[k] = 0;
+            if (i < m) {
+                sum[k] = what[k].adds(a);
+                if (kept != nullptr)
+                    kept[i] = what[k].kept();
+            }
+            sum[k] = warpInclusive(sum[k]);
+            if (lane == 31)
+                segment[k * kWarps + warp] = sum[k];
         }
+    }
     __syncthreads();
-    return carry + total;
+    if (warp == 0) {
+        constexpr uint32_t kEach = kItems * kWarps / 32;  // segments a lane adds up
+        uint32_t mine[kEach], total = 0;
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e) {
+            mine[e] = total;
+            const uint32_t s = lane * kEach + e;
+            total = addUpTo(total, s < items * kWarps ? segment[s] : 0u);
+        }
+        const uint32_t through = warpInclusive(total);
+        const uint32_t before = __shfl_up_sync(kFull, through, 1);
+        __syncwarp();
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e)
+            segment[lane * kEach + e] = addUpTo(carry, addUpTo(lane == 0 ? 0u : before, mine[e]));
+        if (lane == 31)
+            segment[kMaxSegments] = addUpTo(carry, through);
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < kItems; ++k)
+        if (k < items && k * Threads + threadIdx.x < m)
+            upto[k * Threads + threadIdx.x] = addUpTo(segment[k * kWarps + warp], sum[k]);
+    __syncthreads();
+    return segment[kMaxSegments];
 }
 
 /** The scan of any number of requests by one CTA, into scratch. */
 template <class What, class Len>
-__global__ __launch_bounds__(kThreads) void scanKernel(PagedArgs a)
+__global__ __launch_bounds__(kLarge) void scanKernel(PagedArgs a)
 {
     __shared__ uint32_t upto[kScanInBlock];
-    __shared__ uint64_t scratch[33];
+    __shared__ uint32_t segment[kMaxSegments + 1];
     letNextKernelStart();
     if (threadIdx.x == 0 && a.cells != nullptr)
         a.cells[1] = 0;
-    uint64_t carry = 0;
+    uint32_t carry = 0;
     for (uint32_t from = 0; from < a.requests; from += kScanInBlock) {
-        What what[kItems];
-        carry = scanBlock<What, Len>(a, from, carry, what, upto, scratch);
-        for (uint32_t i = threadIdx.x; i < min(a.requests - from, kScanInBlock); i += kThreads)
+        carry = scanBlock<kLarge, What, Len>(a, from, carry, upto, nullptr, segment);
+        for (uint32_t i = threadIdx.x; i < min(a.requests - from, kScanInBlock); i += kLarge)
             a.upto[from + i] = upto[i];
         __syncthreads();
     }
@@ -176,117 +242,112 @@ __device__ __forceinline__ uint32_t requestFrom(const uint32_t* upto, uint32_t r
 
 // ------------------------------------------------------------------ block tables
 
-constexpr uint32_t kEntries = 128;  // of the pool's front per warp and step: one search for all of them
+constexpr uint32_t kEntries = 512;  // of a request's new or returned blocks per warp
+constexpr int kAhead = 4;
 
-/** Every CTA scans the requests (or reads the scan from scratch) and takes its share of the
- *  lists; the last one also writes what each request holds and the cells. */
-template <class Len, bool InBlock>
-__global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
+/** A warp takes up to kEntries blocks of one request: those it gets are copied from the pool, and
+ *  those a terminated one gives back are cleared. (One search per entry of the pool's front
+ *  instead, 100 instructions per 32 entries against 15, took twice as long.) The requests are
+ *  spread over the CTAs for what they hold now, too. */
+template <class Len, int Threads, bool InBlock>
+__global__ __launch_bounds__(Threads) void blockTablesKernel(PagedArgs a)
 {
-    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : 1];
-    __shared__ uint32_t sGone[InBlock ? kScanInBlock / 32 : 1];  // a bit per terminated request
-    __shared__ uint64_t scratch[33];
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ uint32_t segment[kMaxSegments + 1];
     __shared__ uint32_t sShort;
+    constexpr uint32_t kCapacity = uint32_t(Threads) * kItems;
+    Blocks::Kept* kept = reinterpret_cast<Blocks::Kept*>(raw);
+    uint32_t* sUpto = reinterpret_cast<uint32_t*>(kept + kCapacity);
     const uint32_t* upto = InBlock ? sUpto : a.upto;
-    const bool returns = a.used != nullptr && a.terminated != nullptr;
-    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
-                   warps = gridDim.x * kWarps;
+    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * (Threads / 32) + (threadIdx.x >> 5),
+                   warps = gridDim.x * (Threads / 32);
     if constexpr (!InBlock)
         waitForKernelBefore();
     const uint32_t given = __ldg(a.count);
     const uint32_t available = uint64_t(given) > uint64_t(a.poolSize) ? 0u : given;
     if (threadIdx.x == 0)
         sShort = 0;
-    Blocks what[kItems];
-    if constexpr (InBlock) {
-        for (uint32_t i = threadIdx.x; returns && i < (a.requests + 31) / 32; i += kThreads)
-            sGone[i] = 0;
-        (void)scanBlock<Blocks, Len>(a, 0, 0, what, sUpto, scratch);
-    } else {
+    if constexpr (InBlock)
+        (void)scanBlock<Threads, Blocks, Len>(a, 0, 0, sUpto, kept, segment);
+    else
         __syncthreads();
-    }
-    // the sums never fall, so the requests that fit with new blocks are the first ones, up to
-    // the last sum within the pool
-    const uint32_t fitting = requestOf(upto, a.requests, available);
-    const uint32_t taken = fitting == 0 ? 0u : upto[fitting - 1];
+    auto request = [&](uint32_t r) {
+        Blocks b;
+        if constexpr (InBlock)
+            b = Blocks::of(kept[r]);
+        else
+            b.read<Len>(a, r);
+        return b;
+    };
 
+    const uint64_t tasks = uint64_t(a.requests) * a.pieces;
+    for (uint64_t task = warp; task < tasks; task += warps) {
+        const uint32_t r = a.pieces == 1 ? uint32_t(task) : uint32_t(task / a.pieces);
+        const uint32_t j0 = uint32_t(task - uint64_t(r) * a.pieces) * kEntries + lane;
+        const Blocks b = request(r);
+        int32_t* row = a.table + int64_t(r) * a.tableStride;
+        if (b.live) {
+            const uint32_t adds = b.adds(a), sum = upto[r];
+            if (j0 - lane >= adds || sum > available)
+                continue;
+            const int32_t* from = a.pool + (sum - adds);
+            for (uint32_t j = j0; j < min(j0 - lane + kEntries, adds); j += 32 * kAhead) {
+                int32_t id[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    id[u] = j + 32u * u < adds ? __ldg(from + j + 32u * u) : -1;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (j + 32u * u < adds) {
+                        row[b.held + j + 32u * u] = id[u];
+                        if (a.used != nullptr && id[u] >= 0 && int64_t(id[u]) < a.usedSize)
+                            a.used[id[u]] = 1;
+                    }
+                }
+            }
+        } else if (a.used != nullptr) {
+            for (uint32_t j = j0; j < min(j0 - lane + kEntries, b.held); j += 32 * kAhead) {
+                int32_t id[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    id[u] = j + 32u * u < b.held ? row[j + 32u * u] : -1;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (id[u] >= 0 && int64_t(id[u]) < a.usedSize)
+                        a.used[id[u]] = 0;
+            }
+        }
+    }
+
+    // what each request holds now; the last CTA counts those left short, over all of them where
+    // each CTA has them all, else its share of them
     const bool last = blockIdx.x == gridDim.x - 1;
     uint32_t missed = 0;
-    auto settle = [&](const Blocks& w, uint32_t r) {
-        const bool fits = !w.wide && (w.need <= w.held || upto[r] <= available);
-        a.blocks[r] = int32_t(!w.live ? 0u : (fits && w.need > w.held ? w.need : w.held));
-        missed += fits ? 0u : 1u;
+    auto fits = [&](const Blocks& b, uint32_t r) {
+        return b.need <= b.held || (b.need <= uint32_t(a.width) && upto[r] <= available);
     };
-    if constexpr (InBlock) {
-        const uint32_t items = (a.requests + kThreads - 1) / kThreads, first = threadIdx.x * items;
-#pragma unroll
-        for (uint32_t k = 0; k < kItems; ++k) {
-            if (k < items && first + k < a.requests) {
-                if (last)
-                    settle(what[k], first + k);
-                if (returns && !what[k].live && what[k].held > 0)
-                    atomicOr(sGone + ((first + k) >> 5), 1u << ((first + k) & 31u));
-            }
-        }
-        __syncthreads();
-    } else {
-        for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r < a.requests; r += gridDim.x * kThreads) {
-            Blocks w;
-            w.read<Len>(a, r);
-            settle(w, r);
-        }
+    for (uint32_t r = blockIdx.x * Threads + threadIdx.x; r < a.requests; r += gridDim.x * Threads) {
+        const Blocks b = request(r);
+        const bool ok = fits(b, r);
+        a.blocks[r] = int32_t(!b.live ? 0u : (ok && b.need > b.held ? b.need : b.held));
+        missed += !InBlock && !ok ? 1u : 0u;
     }
-
-    // the blocks of terminated requests, a warp per request
-    if (returns) {
-        for (uint32_t r = warp; r < a.requests; r += warps) {
-            if (InBlock ? ((sGone[r >> 5] >> (r & 31u)) & 1u) == 0 : __ldg(a.terminated + r) == 0)
-                continue;
-            const int64_t h = __ldg(a.held + r);
-            const int64_t held = h < a.width ? h : a.width;
-            const int32_t* row = a.table + int64_t(r) * a.tableStride;
-#pragma unroll 4
-            for (int64_t j = lane; j < held; j += 32) {
-                const int64_t id = row[j];
-                if (id >= 0 && id < a.usedSize)
-                    a.used[id] = 0;
-            }
-        }
-    }
-
-    // the front of the pool
-    for (uint64_t q0 = uint64_t(warp) * kEntries; q0 < taken; q0 += uint64_t(warps) * kEntries) {
-        const uint32_t r0 = requestOf(upto, a.requests, uint32_t(q0));
-        int32_t id[kEntries / 32];
-#pragma unroll
-        for (uint32_t k = 0; k < kEntries / 32; ++k) {
-            const uint64_t q = q0 + 32u * k + lane;
-            id[k] = q < taken ? __ldg(a.pool + q) : -1;
-        }
-        uint32_t r = r0;
-#pragma unroll
-        for (uint32_t k = 0; k < kEntries / 32; ++k) {
-            const uint64_t q = q0 + 32u * k + lane;
-            if (q >= taken)
-                break;
-            r = requestFrom(upto, a.requests, uint32_t(q), r);
-            const uint32_t before = r == 0 ? 0u : upto[r - 1];
-            const int64_t h = __ldg(a.held + r);
-            a.table[int64_t(r) * a.tableStride + (h < 0 ? 0 : h) + (uint32_t(q) - before)] = id[k];
-            if (a.used != nullptr && id[k] >= 0 && int64_t(id[k]) < a.usedSize)
-                a.used[id[k]] = 1;
-        }
-    }
-
     if (InBlock && !last)
         return;
+    if constexpr (InBlock)
+        for (uint32_t r = threadIdx.x; r < a.requests; r += Threads)
+            missed += fits(request(r), r) ? 0u : 1u;
     missed = warpSum(missed);
     if (lane == 0 && missed != 0)
         atomicAdd(&sShort, missed);
     __syncthreads();
     if (threadIdx.x == 0) {
-        if (last)
-            a.cells[0] = taken;
+        if (last) {
+            // the sums never fall, so the requests that fit with new blocks are the first ones,
+            // up to the last sum within the pool
+            const uint32_t fitting = requestOf(upto, a.requests, available);
+            a.cells[0] = fitting == 0 ? 0u : upto[fitting - 1];
+        }
         if (InBlock)
             a.cells[1] = sShort;
         else if (sShort != 0)  // zeroed by the scan
@@ -298,39 +359,41 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 
 constexpr uint32_t kTokens = 4;  // neighbouring tokens per thread and step
 
-template <class Len, class Slot, bool InBlock>
-__global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
+template <class Len, class Slot, int Threads, bool InBlock>
+__global__ __launch_bounds__(Threads) void slotMapKernel(PagedArgs a)
 {
-    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : 1];
-    __shared__ uint64_t scratch[33];
+    extern __shared__ __align__(16) unsigned char raw[];
+    __shared__ uint32_t segment[kMaxSegments + 1];
+    constexpr uint32_t kCapacity = uint32_t(Threads) * kItems;
+    int64_t* starts = reinterpret_cast<int64_t*>(raw);
+    uint32_t* sUpto = reinterpret_cast<uint32_t*>(starts + kCapacity);
     const uint32_t* upto = InBlock ? sUpto : a.upto;
-    if constexpr (InBlock) {
-        Tokens what[kItems];
-        (void)scanBlock<Tokens, Len>(a, 0, 0, what, sUpto, scratch);
-    } else {
+    if constexpr (InBlock)
+        (void)scanBlock<Threads, Tokens, Len>(a, 0, 0, sUpto, starts, segment);
+    else
         waitForKernelBefore();
-    }
-    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
-                   warps = gridDim.x * kWarps;
+    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * (Threads / 32) + (threadIdx.x >> 5),
+                   warps = gridDim.x * (Threads / 32);
     for (uint64_t w0 = uint64_t(warp) * 32u * kTokens; w0 < a.capacity; w0 += uint64_t(warps) * 32u * kTokens) {
-        const uint32_t r0 = requestOf(upto, a.requests, uint32_t(w0));  // one search for the warp's tokens
+        // one search for the warp's tokens, which are mostly one request's
+        uint32_t r = requestOf(upto, a.requests, uint32_t(w0));
+        const bool one = r < a.requests && uint64_t(upto[r]) >= w0 + 32u * kTokens;
         const uint64_t q0 = w0 + lane * kTokens;
-        uint32_t r = r0;
-        if (q0 < a.capacity)
-            r = requestFrom(upto, a.requests, uint32_t(q0), r);
         Pack<Slot, kTokens> slot;
         Pack<Len, kTokens> position;
         Pack<int32_t, kTokens> request;
 #pragma unroll
         for (uint32_t k = 0; k < kTokens; ++k) {
             const uint32_t q = uint32_t(q0) + k;
-            r = requestFrom(upto, a.requests, q, r);
+            if (!one)
+                r = requestFrom(upto, a.requests, q, r);
             slot.e[k] = Slot(-1);
             position.e[k] = 0;
             request.e[k] = -1;
             if (r < a.requests) {
                 const uint32_t before = r == 0 ? 0u : upto[r - 1];
-                const uint64_t p = uint64_t(lengthAt<Len>(a.start, r)) + (q - before);
+                const int64_t start = InBlock ? starts[r] : lengthAt<Len>(a.start, r);
+                const uint64_t p = uint64_t(start) + (q - before);
                 position.e[k] = Len(p);
                 request.e[k] = int32_t(r);
                 if (p < uint64_t(a.room)) {
@@ -357,7 +420,7 @@ __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
             }
         }
     }
-    for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r <= a.requests; r += gridDim.x * kThreads)
+    for (uint32_t r = blockIdx.x * Threads + threadIdx.x; r <= a.requests; r += gridDim.x * Threads)
         a.offsets[r] = r == 0 ? 0 : int32_t(upto[r - 1]);
 }
 
@@ -401,8 +464,30 @@ void withLength(uint32_t type, F&& f)
 template <class What, class Len>
 void launchScan(const PagedArgs& a, cudaStream_t s, const char* who)
 {
-    scanKernel<What, Len><<<1, kThreads, 0, s>>>(a);
+    scanKernel<What, Len><<<1, kLarge, 0, s>>>(a);
     launchCheck(who);
+}
+
+/** One kernel where each CTA holds all requests, in CTAs of the size that does; else behind the scan.
+ *  ``work``: what the threads share out, ``per`` to a thread; ``ctas`` an SM at most. */
+template <class Small, class Large, class Scanned>
+void launchPaged(const PagedArgs& a, Small small, Large large, Scanned scanned, size_t keptBytes, int64_t work,
+    int64_t per, int64_t ctas, cudaStream_t s, const char* who)
+{
+    auto grid = [&](int64_t threads) {
+        return unsigned(std::max<int64_t>(1, std::min(ctas * smCount(), (work + threads * per - 1) / (threads * per))));
+    };
+    if (a.requests <= uint32_t(kSmall) * kItems) {
+        small<<<grid(kSmall), kSmall, size_t(kSmall) * kItems * (keptBytes + 4), s>>>(a);
+        launchCheck(who);
+    } else if (a.requests <= kScanInBlock) {
+        const size_t shared = size_t(kLarge) * kItems * (keptBytes + 4);
+        cudaCheck(cudaFuncSetAttribute(large, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
+        large<<<grid(kLarge), kLarge, shared, s>>>(a);
+        launchCheck(who);
+    } else {
+        launchBehind(scanned, grid(kSmall), kSmall, 0, s, a, who);
+    }
 }
 
 }  // namespace
@@ -451,18 +536,14 @@ EB_API eagle_backend_status eagle_backend_x_b200_block_tables(eagle_b200_paged_d
         a.blocks = reinterpret_cast<int32_t*>(d.blocks);
         a.cells = reinterpret_cast<uint32_t*>(d.cells);
         const cudaStream_t s = seamStream(d.stream);
-        // the entries the call can write at most, an SM per CTA
-        const int64_t most = std::max(std::min(d.pool_size, d.requests * d.width), d.requests);
-        const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(smCount(), (most + kWarps * kEntries - 1) / (kWarps * kEntries)));
+        a.pieces = uint32_t(std::max<int64_t>(1, (d.width + kEntries - 1) / kEntries));
         withLength(d.length_type, [&](auto len) {
             using Len = decltype(len);
-            if (d.requests <= int64_t(kScanInBlock)) {
-                blockTablesKernel<Len, true><<<unsigned(grid), kThreads, 0, s>>>(a);
-                launchCheck(who);
-            } else {
+            if (d.requests > int64_t(kScanInBlock))
                 launchScan<Blocks, Len>(a, s, who);
-                launchBehind(blockTablesKernel<Len, false>, unsigned(grid), kThreads, 0, s, a, who);
-            }
+            launchPaged(a, blockTablesKernel<Len, kSmall, true>, blockTablesKernel<Len, kLarge, true>,
+                blockTablesKernel<Len, kSmall, false>, sizeof(Blocks::Kept), d.requests * a.pieces * 32, 1,
+                d.requests <= int64_t(kScanInBlock) ? 2 : 8, s, who);
         });
     });
 }
@@ -506,19 +587,15 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
         a.tokenRequests = reinterpret_cast<int32_t*>(d.token_requests);
         a.offsets = reinterpret_cast<int32_t*>(d.offsets);
         const cudaStream_t s = seamStream(d.stream);
-        const int64_t per = int64_t(kThreads) * kTokens;
-        const int64_t grid = std::max<int64_t>(1, std::min<int64_t>(2 * smCount(), (d.capacity + per - 1) / per));
         withLength(d.length_type, [&](auto len) {
             withLength(d.slot_type, [&](auto slot) {
                 using Len = decltype(len);
                 using Slot = decltype(slot);
-                if (d.requests <= int64_t(kScanInBlock)) {
-                    slotMapKernel<Len, Slot, true><<<unsigned(grid), kThreads, 0, s>>>(a);
-                    launchCheck(who);
-                } else {
+                if (d.requests > int64_t(kScanInBlock))
                     launchScan<Tokens, Len>(a, s, who);
-                    launchBehind(slotMapKernel<Len, Slot, false>, unsigned(grid), kThreads, 0, s, a, who);
-                }
+                launchPaged(a, slotMapKernel<Len, Slot, kSmall, true>, slotMapKernel<Len, Slot, kLarge, true>,
+                    slotMapKernel<Len, Slot, kSmall, false>, sizeof(Tokens::Kept), d.capacity, kTokens,
+                    d.requests <= int64_t(kScanInBlock) ? 2 : 8, s, who);
             });
         });
     });
