@@ -5,13 +5,12 @@
 //   slot_map      the scan of fresh_r packs the requests' new tokens; token i of request r
 //                 at position p = start_r + i has slot table[r][p / block] * block + p % block
 //
-// Both turn one number per request into a ragged list: a scan over the requests, then a
-// search of the scan per list entry. The lists are a few megabytes at most, so the calls
-// are bound by the launch and by one chain of dependent reads. Up to kScanInBlock
-// requests every CTA scans all of them itself into shared memory -- one launch, no wait on
-// another CTA; past it the scan is a kernel of its own (one CTA) that leaves it in scratch.
-// CTAs are of 256 threads where those scan the requests (2048), which starts and meets at
-// its barriers sooner than 1024.
+// Both turn one number per request into a ragged list by a scan over the requests. The lists
+// are a few megabytes at most, so the calls are bound by the launch and by one chain of
+// dependent reads. Up to kScanInBlock requests every CTA scans all of them itself into shared
+// memory: one launch, no wait on another CTA. Past it the scan is a kernel of its own, of one
+// CTA, that leaves it in scratch: 300 CTAs that each read 8191 requests took 7 us over
+// that, a CTA alone 3 and the start of a second kernel 1.
 #include "sequences.cuh"
 
 #include <algorithm>
@@ -22,8 +21,10 @@ namespace eb {
 namespace {
 
 constexpr uint32_t kItems = 8;  // requests a thread scans
-constexpr int kSmall = 256, kLarge = 1024;
-constexpr uint32_t kScanInBlock = kLarge * kItems;  // 8192
+constexpr int kThreads = 256, kScanThreads = 1024;
+constexpr uint32_t kScanInBlock = kThreads * kItems;    // 2048
+constexpr uint32_t kScanAtOnce = kScanThreads * kItems; // 8192
+constexpr uint32_t kWarps = kThreads / 32;
 
 struct PagedArgs {
     uint32_t requests;
@@ -61,7 +62,8 @@ __device__ __forceinline__ int64_t lengthAt(const void* p, uint32_t r)
 
 // ------------------------------------------------------------------ what each request adds
 
-/** A request's blocks: its reads do not wait for one another. */
+/** A request's blocks, from what is read of it (Raw: so that the reads of several are in flight
+ *  together). */
 struct Blocks {
     uint32_t held;  // clipped to the row
     uint32_t need;  // width + 1 where the row cannot hold them
@@ -69,13 +71,23 @@ struct Blocks {
 
     using Kept = uint2;  // {held, need}, the highest bit of held set where it is terminated
     template <class Len>
-    __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
+    struct Raw {
+        Len length;
+        int32_t held;
+        uint8_t ended;
+        __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
+        {
+            ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
+            length = __ldg(reinterpret_cast<const Len*>(a.lengths) + r);
+            held = __ldg(a.held + r);
+        }
+    };
+    template <class Len>
+    __device__ __forceinline__ void take(const PagedArgs& a, const Raw<Len>& raw)
     {
-        const uint8_t ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
-        const int64_t length = lengthAt<Len>(a.lengths, r);
-        const int64_t h = __ldg(a.held + r);
+        const int64_t length = raw.length < 0 ? 0 : int64_t(raw.length), h = raw.held;
         held = uint32_t(h < 0 ? 0 : (h < a.width ? h : a.width));
-        live = ended == 0;
+        live = raw.ended == 0;
         const uint32_t l = uint32_t(length < a.room ? length : a.room);
         const uint32_t whole = a.perBlock(l);
         need = length > a.room ? uint32_t(a.width) + 1u : whole + (whole * a.perBlock.d != l ? 1u : 0u);
@@ -104,12 +116,22 @@ struct Tokens {
 
     using Kept = int64_t;
     template <class Len>
-    __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
+    struct Raw {
+        Len fresh, start;
+        uint8_t ended;
+        __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
+        {
+            ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
+            fresh = __ldg(reinterpret_cast<const Len*>(a.fresh) + r);
+            start = __ldg(reinterpret_cast<const Len*>(a.start) + r);
+        }
+    };
+    template <class Len>
+    __device__ __forceinline__ void take(const PagedArgs&, const Raw<Len>& raw)
     {
-        const uint8_t ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
-        const int64_t f = lengthAt<Len>(a.fresh, r);
-        start = lengthAt<Len>(a.start, r);
-        fresh = ended != 0 ? 0u : uint32_t(f < 0x7fffffffll ? f : 0x7fffffffll);
+        const int64_t f = raw.fresh;
+        start = raw.start < 0 ? 0 : int64_t(raw.start);
+        fresh = raw.ended != 0 || f < 0 ? 0u : uint32_t(f < 0x7fffffffll ? f : 0x7fffffffll);
     }
     __device__ __forceinline__ uint32_t adds(const PagedArgs&) const { return fresh; }
     __device__ __forceinline__ Kept kept() const { return start; }
@@ -134,7 +156,7 @@ __device__ __forceinline__ uint32_t warpInclusive(uint32_t v)
     return v;
 }
 
-constexpr uint32_t kMaxSegments = kItems * (kLarge / 32);
+constexpr uint32_t kMaxSegments = kItems * (kScanThreads / 32);
 
 /** Requests [from, from + Threads * kItems), Threads neighbours at a time (a thread reading its own
  *  neighbours instead took 13 us for 8191 requests), all read at once: their inclusive sums on
@@ -145,40 +167,39 @@ template <int Threads, class What, class Len>
 __device__ __forceinline__ uint32_t scanBlock(const PagedArgs& a, uint32_t from, uint32_t carry, uint32_t* upto,
     typename What::Kept* kept, uint32_t* segment)
 {
-    constexpr uint32_t kWarps = Threads / 32;
+    constexpr uint32_t kOwn = Threads / 32;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t m = min(a.requests - from, uint32_t(Threads) * kItems);
     const uint32_t items = (m + Threads - 1) / Threads;
-    What what[kItems];
+    typename What::template Raw<Len> raw[kItems];
     uint32_t sum[kItems];
 #pragma unroll
     for (uint32_t k = 0; k < kItems; ++k)
-        if (k < items && k * Threads + threadIdx.x < m)
-            what[k].template read<Len>(a, from + k * Threads + threadIdx.x);
+        if (k < items)
+            raw[k].read(a, from + min(k * Threads + threadIdx.x, m - 1u));
 #pragma unroll
     for (uint32_t k = 0; k < kItems; ++k) {
         if (k < items) {
             const uint32_t i = k * Threads + threadIdx.x;
-            sum[k] = 0;
-            if (i < m) {
-                sum[k] = what[k].adds(a);
-                if (kept != nullptr)
-                    kept[i] = what[k].kept();
-            }
+            What what;
+            what.template take<Len>(a, raw[k]);
+            sum[k] = i < m ? what.adds(a) : 0u;
+            if (kept != nullptr && i < m)
+                kept[i] = what.kept();
             sum[k] = warpInclusive(sum[k]);
             if (lane == 31)
-                segment[k * kWarps + warp] = sum[k];
+                segment[k * kOwn + warp] = sum[k];
         }
     }
     __syncthreads();
     if (warp == 0) {
-        constexpr uint32_t kEach = kItems * kWarps / 32;  // segments a lane adds up
+        constexpr uint32_t kEach = kItems * kOwn / 32;  // segments a lane adds up
         uint32_t mine[kEach], total = 0;
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) {
             mine[e] = total;
             const uint32_t s = lane * kEach + e;
-            total = addUpTo(total, s < items * kWarps ? segment[s] : 0u);
+            total = addUpTo(total, s < items * kOwn ? segment[s] : 0u);
         }
         const uint32_t through = warpInclusive(total);
         const uint32_t before = __shfl_up_sync(kFull, through, 1);
@@ -193,24 +214,24 @@ __device__ __forceinline__ uint32_t scanBlock(const PagedArgs& a, uint32_t from,
 #pragma unroll
     for (uint32_t k = 0; k < kItems; ++k)
         if (k < items && k * Threads + threadIdx.x < m)
-            upto[k * Threads + threadIdx.x] = addUpTo(segment[k * kWarps + warp], sum[k]);
+            upto[k * Threads + threadIdx.x] = addUpTo(segment[k * kOwn + warp], sum[k]);
     __syncthreads();
     return segment[kMaxSegments];
 }
 
 /** The scan of any number of requests by one CTA, into scratch. */
 template <class What, class Len>
-__global__ __launch_bounds__(kLarge) void scanKernel(PagedArgs a)
+__global__ __launch_bounds__(kScanThreads) void scanKernel(PagedArgs a)
 {
-    __shared__ uint32_t upto[kScanInBlock];
+    __shared__ uint32_t upto[kScanAtOnce];
     __shared__ uint32_t segment[kMaxSegments + 1];
     letNextKernelStart();
     if (threadIdx.x == 0 && a.cells != nullptr)
         a.cells[1] = 0;
     uint32_t carry = 0;
-    for (uint32_t from = 0; from < a.requests; from += kScanInBlock) {
-        carry = scanBlock<kLarge, What, Len>(a, from, carry, upto, nullptr, segment);
-        for (uint32_t i = threadIdx.x; i < min(a.requests - from, kScanInBlock); i += kLarge)
+    for (uint32_t from = 0; from < a.requests; from += kScanAtOnce) {
+        carry = scanBlock<kScanThreads, What, Len>(a, from, carry, upto, nullptr, segment);
+        for (uint32_t i = threadIdx.x; i < min(a.requests - from, kScanAtOnce); i += kScanThreads)
             a.upto[from + i] = upto[i];
         __syncthreads();
     }
@@ -249,18 +270,16 @@ constexpr int kAhead = 4;
  *  those a terminated one gives back are cleared. (One search per entry of the pool's front
  *  instead, 100 instructions per 32 entries against 15, took twice as long.) The requests are
  *  spread over the CTAs for what they hold now, too. */
-template <class Len, int Threads, bool InBlock>
-__global__ __launch_bounds__(Threads) void blockTablesKernel(PagedArgs a)
+template <class Len, bool InBlock>
+__global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 {
-    extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ uint32_t segment[kMaxSegments + 1];
+    __shared__ uint32_t segment[InBlock ? kMaxSegments + 1 : 1];
     __shared__ uint32_t sShort;
-    constexpr uint32_t kCapacity = uint32_t(Threads) * kItems;
-    Blocks::Kept* kept = reinterpret_cast<Blocks::Kept*>(raw);
-    uint32_t* sUpto = reinterpret_cast<uint32_t*>(kept + kCapacity);
+    __shared__ Blocks::Kept kept[InBlock ? kScanInBlock : 1];
+    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : 1];
     const uint32_t* upto = InBlock ? sUpto : a.upto;
-    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * (Threads / 32) + (threadIdx.x >> 5),
-                   warps = gridDim.x * (Threads / 32);
+    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
+                   warps = gridDim.x * kWarps;
     if constexpr (!InBlock)
         waitForKernelBefore();
     const uint32_t given = __ldg(a.count);
@@ -268,15 +287,18 @@ __global__ __launch_bounds__(Threads) void blockTablesKernel(PagedArgs a)
     if (threadIdx.x == 0)
         sShort = 0;
     if constexpr (InBlock)
-        (void)scanBlock<Threads, Blocks, Len>(a, 0, 0, sUpto, kept, segment);
+        (void)scanBlock<kThreads, Blocks, Len>(a, 0, 0, sUpto, kept, segment);
     else
         __syncthreads();
     auto request = [&](uint32_t r) {
         Blocks b;
-        if constexpr (InBlock)
+        if constexpr (InBlock) {
             b = Blocks::of(kept[r]);
-        else
-            b.read<Len>(a, r);
+        } else {
+            Blocks::Raw<Len> raw;
+            raw.read(a, r);
+            b.take<Len>(a, raw);
+        }
         return b;
     };
 
@@ -326,7 +348,7 @@ __global__ __launch_bounds__(Threads) void blockTablesKernel(PagedArgs a)
     auto fits = [&](const Blocks& b, uint32_t r) {
         return b.need <= b.held || (b.need <= uint32_t(a.width) && upto[r] <= available);
     };
-    for (uint32_t r = blockIdx.x * Threads + threadIdx.x; r < a.requests; r += gridDim.x * Threads) {
+    for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r < a.requests; r += gridDim.x * kThreads) {
         const Blocks b = request(r);
         const bool ok = fits(b, r);
         a.blocks[r] = int32_t(!b.live ? 0u : (ok && b.need > b.held ? b.need : b.held));
@@ -335,7 +357,7 @@ __global__ __launch_bounds__(Threads) void blockTablesKernel(PagedArgs a)
     if (InBlock && !last)
         return;
     if constexpr (InBlock)
-        for (uint32_t r = threadIdx.x; r < a.requests; r += Threads)
+        for (uint32_t r = threadIdx.x; r < a.requests; r += kThreads)
             missed += fits(request(r), r) ? 0u : 1u;
     missed = warpSum(missed);
     if (lane == 0 && missed != 0)
@@ -359,21 +381,28 @@ __global__ __launch_bounds__(Threads) void blockTablesKernel(PagedArgs a)
 
 constexpr uint32_t kTokens = 4;  // neighbouring tokens per thread and step
 
-template <class Len, class Slot, int Threads, bool InBlock>
-__global__ __launch_bounds__(Threads) void slotMapKernel(PagedArgs a)
+/** ``Copied``: the scan is read from scratch into shared memory first (up to kScanAtOnce requests),
+ *  where a search is a tenth of the time. */
+template <class Len, class Slot, bool InBlock, bool Copied>
+__global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
 {
-    extern __shared__ __align__(16) unsigned char raw[];
-    __shared__ uint32_t segment[kMaxSegments + 1];
-    constexpr uint32_t kCapacity = uint32_t(Threads) * kItems;
-    int64_t* starts = reinterpret_cast<int64_t*>(raw);
-    uint32_t* sUpto = reinterpret_cast<uint32_t*>(starts + kCapacity);
-    const uint32_t* upto = InBlock ? sUpto : a.upto;
-    if constexpr (InBlock)
-        (void)scanBlock<Threads, Tokens, Len>(a, 0, 0, sUpto, starts, segment);
-    else
+    __shared__ uint32_t segment[InBlock ? kMaxSegments + 1 : 1];
+    __shared__ int64_t starts[InBlock ? kScanInBlock : 1];
+    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : (Copied ? kScanAtOnce : 1)];
+    const uint32_t* upto = InBlock || Copied ? sUpto : a.upto;
+    if constexpr (InBlock) {
+        (void)scanBlock<kThreads, Tokens, Len>(a, 0, 0, sUpto, starts, segment);
+    } else {
         waitForKernelBefore();
-    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * (Threads / 32) + (threadIdx.x >> 5),
-                   warps = gridDim.x * (Threads / 32);
+        if constexpr (Copied) {
+#pragma unroll 8
+            for (uint32_t i = threadIdx.x; i < a.requests; i += kThreads)
+                sUpto[i] = __ldcg(a.upto + i);
+            __syncthreads();
+        }
+    }
+    const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
+                   warps = gridDim.x * kWarps;
     for (uint64_t w0 = uint64_t(warp) * 32u * kTokens; w0 < a.capacity; w0 += uint64_t(warps) * 32u * kTokens) {
         // one search for the warp's tokens, which are mostly one request's
         uint32_t r = requestOf(upto, a.requests, uint32_t(w0));
@@ -382,14 +411,17 @@ __global__ __launch_bounds__(Threads) void slotMapKernel(PagedArgs a)
         Pack<Slot, kTokens> slot;
         Pack<Len, kTokens> position;
         Pack<int32_t, kTokens> request;
+        int64_t id[kTokens];
+        uint32_t within[kTokens];
 #pragma unroll
         for (uint32_t k = 0; k < kTokens; ++k) {
             const uint32_t q = uint32_t(q0) + k;
             if (!one)
                 r = requestFrom(upto, a.requests, q, r);
-            slot.e[k] = Slot(-1);
             position.e[k] = 0;
             request.e[k] = -1;
+            id[k] = -1;
+            within[k] = 0;
             if (r < a.requests) {
                 const uint32_t before = r == 0 ? 0u : upto[r - 1];
                 const int64_t start = InBlock ? starts[r] : lengthAt<Len>(a.start, r);
@@ -398,12 +430,15 @@ __global__ __launch_bounds__(Threads) void slotMapKernel(PagedArgs a)
                 request.e[k] = int32_t(r);
                 if (p < uint64_t(a.room)) {
                     const uint32_t b = a.perBlock(uint32_t(p));
-                    const int64_t id = __ldg(a.table + int64_t(r) * a.tableStride + b);
-                    const int64_t at = id * a.perBlock.d + (uint32_t(p) - b * a.perBlock.d);
-                    if (id >= 0 && int64_t(Slot(at)) == at)
-                        slot.e[k] = Slot(at);
+                    within[k] = uint32_t(p) - b * a.perBlock.d;
+                    id[k] = __ldg(a.table + int64_t(r) * a.tableStride + b);
                 }
             }
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kTokens; ++k) {
+            const int64_t at = id[k] * a.perBlock.d + within[k];
+            slot.e[k] = id[k] >= 0 && int64_t(Slot(at)) == at ? Slot(at) : Slot(-1);
         }
         if (q0 + kTokens <= a.capacity) {
             *reinterpret_cast<Pack<Slot, kTokens>*>(reinterpret_cast<Slot*>(a.slots) + q0) = slot;
@@ -420,7 +455,7 @@ __global__ __launch_bounds__(Threads) void slotMapKernel(PagedArgs a)
             }
         }
     }
-    for (uint32_t r = blockIdx.x * Threads + threadIdx.x; r <= a.requests; r += gridDim.x * Threads)
+    for (uint32_t r = blockIdx.x * kThreads + threadIdx.x; r <= a.requests; r += gridDim.x * kThreads)
         a.offsets[r] = r == 0 ? 0 : int32_t(upto[r - 1]);
 }
 
@@ -464,30 +499,14 @@ void withLength(uint32_t type, F&& f)
 template <class What, class Len>
 void launchScan(const PagedArgs& a, cudaStream_t s, const char* who)
 {
-    scanKernel<What, Len><<<1, kLarge, 0, s>>>(a);
+    scanKernel<What, Len><<<1, kScanThreads, 0, s>>>(a);
     launchCheck(who);
 }
 
-/** One kernel where each CTA holds all requests, in CTAs of the size that does; else behind the scan.
- *  ``work``: what the threads share out, ``per`` to a thread; ``ctas`` an SM at most. */
-template <class Small, class Large, class Scanned>
-void launchPaged(const PagedArgs& a, Small small, Large large, Scanned scanned, size_t keptBytes, int64_t work,
-    int64_t per, int64_t ctas, cudaStream_t s, const char* who)
+/** CTAs for ``threads`` threads' work, at most ``most`` an SM. */
+unsigned gridFor(int64_t threads, int64_t most)
 {
-    auto grid = [&](int64_t threads) {
-        return unsigned(std::max<int64_t>(1, std::min(ctas * smCount(), (work + threads * per - 1) / (threads * per))));
-    };
-    if (a.requests <= uint32_t(kSmall) * kItems) {
-        small<<<grid(kSmall), kSmall, size_t(kSmall) * kItems * (keptBytes + 4), s>>>(a);
-        launchCheck(who);
-    } else if (a.requests <= kScanInBlock) {
-        const size_t shared = size_t(kLarge) * kItems * (keptBytes + 4);
-        cudaCheck(cudaFuncSetAttribute(large, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
-        large<<<grid(kLarge), kLarge, shared, s>>>(a);
-        launchCheck(who);
-    } else {
-        launchBehind(scanned, grid(kSmall), kSmall, 0, s, a, who);
-    }
+    return unsigned(std::max<int64_t>(1, std::min(most * smCount(), (threads + kThreads - 1) / kThreads)));
 }
 
 }  // namespace
@@ -539,11 +558,14 @@ EB_API eagle_backend_status eagle_backend_x_b200_block_tables(eagle_b200_paged_d
         a.pieces = uint32_t(std::max<int64_t>(1, (d.width + kEntries - 1) / kEntries));
         withLength(d.length_type, [&](auto len) {
             using Len = decltype(len);
-            if (d.requests > int64_t(kScanInBlock))
+            const int64_t threads = d.requests * a.pieces * 32;  // a warp per request's share
+            if (d.requests <= int64_t(kScanInBlock)) {
+                blockTablesKernel<Len, true><<<gridFor(threads, 2), kThreads, 0, s>>>(a);
+                launchCheck(who);
+            } else {
                 launchScan<Blocks, Len>(a, s, who);
-            launchPaged(a, blockTablesKernel<Len, kSmall, true>, blockTablesKernel<Len, kLarge, true>,
-                blockTablesKernel<Len, kSmall, false>, sizeof(Blocks::Kept), d.requests * a.pieces * 32, 1,
-                d.requests <= int64_t(kScanInBlock) ? 2 : 8, s, who);
+                launchBehind(blockTablesKernel<Len, false>, gridFor(threads, 8), kThreads, 0, s, a, who);
+            }
         });
     });
 }
@@ -591,11 +613,17 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
             withLength(d.slot_type, [&](auto slot) {
                 using Len = decltype(len);
                 using Slot = decltype(slot);
-                if (d.requests > int64_t(kScanInBlock))
+                const int64_t threads = (d.capacity + kTokens - 1) / kTokens;
+                if (d.requests <= int64_t(kScanInBlock)) {
+                    slotMapKernel<Len, Slot, true, false><<<gridFor(threads, 4), kThreads, 0, s>>>(a);
+                    launchCheck(who);
+                } else {
                     launchScan<Tokens, Len>(a, s, who);
-                launchPaged(a, slotMapKernel<Len, Slot, kSmall, true>, slotMapKernel<Len, Slot, kLarge, true>,
-                    slotMapKernel<Len, Slot, kSmall, false>, sizeof(Tokens::Kept), d.capacity, kTokens,
-                    d.requests <= int64_t(kScanInBlock) ? 2 : 8, s, who);
+                    if (d.requests <= int64_t(kScanAtOnce))
+                        launchBehind(slotMapKernel<Len, Slot, false, true>, gridFor(threads, 6), kThreads, 0, s, a, who);
+                    else
+                        launchBehind(slotMapKernel<Len, Slot, false, false>, gridFor(threads, 8), kThreads, 0, s, a, who);
+                }
             });
         });
     });

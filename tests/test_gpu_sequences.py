@@ -369,7 +369,7 @@ def _check_tables(eb, lengths, held, table, pool, count, block, used=None, termi
     return want
 
 
-@pytest.mark.parametrize("requests", (0, 1, 2, 33, 513, 8192, 8193, 20000))
+@pytest.mark.parametrize("requests", (0, 1, 2, 33, 513, 2048, 2049, 8192, 8193, 20000))
 @pytest.mark.parametrize("block", (1, 16, 24))
 @pytest.mark.parametrize("dtype", (np.int32, np.int64))
 def test_tables(eb, requests, block, dtype):
@@ -456,7 +456,7 @@ def _check_slots(eb, table, start, fresh, capacity, block, terminated=None, dtyp
         assert np.array_equal(g.cpu().numpy().astype(np.int64), w), name
 
 
-@pytest.mark.parametrize("requests", (0, 1, 5, 513, 8192, 8193))
+@pytest.mark.parametrize("requests", (0, 1, 5, 513, 2048, 2049, 8192, 8193))
 @pytest.mark.parametrize("block", (1, 16, 24))
 @pytest.mark.parametrize("dtype,slot", [(np.int32, torch.int64), (np.int64, torch.int32)])
 def test_slots(eb, requests, block, dtype, slot):

@@ -137,7 +137,7 @@ def test_paged_refuses_its_own(entry, fields, status):
 
 def test_paged_queries():
     for entry in ("block_tables", "slot_map"):
-        for requests, least in ((0, 0), (4, 0), (8192, 0), (8193, 4 * 8193), (2**20, 4 * 2**20)):
+        for requests, least in ((0, 0), (4, 0), (2048, 0), (8193, 4 * 8193), (2**20, 4 * 2**20)):
             d = _paged(requests=requests)
             assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == _abi.OK
             assert d.scratch_bytes >= max(least, 16)
