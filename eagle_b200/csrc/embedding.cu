@@ -83,6 +83,8 @@ __device__ __forceinline__ void placeOf(const LookupArgs& a, int64_t t, int64_t&
 template <class In, class Out, class Tok, int N, int Unroll>
 __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
 {
+    letNextKernelStart();
+    waitForKernelBefore();
     const int64_t base = int64_t(blockIdx.x) * (kLookupThreads * Unroll);
     const int64_t row0 = base / a.pieces;
     const uint32_t col0 = uint32_t(base - row0 * a.pieces);
@@ -157,6 +159,8 @@ __device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
 template <class In, class Out, class Tok, int N, int Unroll>
 __global__ __launch_bounds__(kLookupThreads) void lookupShiftedKernel(LookupArgs a)
 {
+    letNextKernelStart();
+    waitForKernelBefore();
     const int64_t base = int64_t(blockIdx.x) * (kLookupThreads * Unroll);
     const int64_t row0 = base / a.pieces;
     const uint32_t col0 = uint32_t(base - row0 * a.pieces);
@@ -223,6 +227,8 @@ __device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi)
 template <class In, class Out, class Tok, int N, int Unroll, bool Shifted>
 __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
 {
+    letNextKernelStart();
+    waitForKernelBefore();
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t id = blockIdx.x * (kLookupThreads / 32) + (threadIdx.x >> 5);
     const int64_t t = a.perRow(id);  // pieces: warps to a row
@@ -477,6 +483,7 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t ctas = cluster.num_blocks(), cta = cluster.block_rank();
     letNextKernelStart();
+    waitForKernelBefore();
     if (blockIdx.x >= ctas) {
         char* table = reinterpret_cast<char*>(a.table);
         const uint32_t at = blockIdx.x - ctas, others = gridDim.x - ctas;
@@ -1144,6 +1151,7 @@ template <class Out>
 __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
 {
     __shared__ float4 part[kJoinWarps][32];
+    letNextKernelStart();
     waitForKernelBefore();
     if (blockIdx.x >= a.joinBlocks) {
         zeroUnit(a, a.present, a.zeroedBefore, a.rows, blockIdx.x - a.joinBlocks);
@@ -1272,9 +1280,9 @@ void launchLookup(LookupArgs a, cudaStream_t s, const char* who)
             unsupported(std::string(who) + ": the call is larger than one launch holds");
         const unsigned blocks = unsigned((warps + kLookupThreads / 32 - 1) / (kLookupThreads / 32));
         if (unroll == 1)
-            lookupWideKernel<In, Out, Tok, N, 1, Shifted><<<blocks, kLookupThreads, 0, s>>>(a);
+            launchBehind(lookupWideKernel<In, Out, Tok, N, 1, Shifted>, blocks, kLookupThreads, 0, s, a, who);
         else
-            lookupWideKernel<In, Out, Tok, N, 4, Shifted><<<blocks, kLookupThreads, 0, s>>>(a);
+            launchBehind(lookupWideKernel<In, Out, Tok, N, 4, Shifted>, blocks, kLookupThreads, 0, s, a, who);
     } else {
         a.pieces = Shifted ? (a.dim + N - 1) / N + 1 : a.dim / N;
         a.perRow = FastDiv(a.pieces);
@@ -1282,9 +1290,9 @@ void launchLookup(LookupArgs a, cudaStream_t s, const char* who)
         const int unroll = all >= sms * 2 * kLookupThreads * 4 ? 4 : 1;
         const unsigned blocks = gridOf((all + kLookupThreads * unroll - 1) / (kLookupThreads * unroll), who);
         if (Shifted && unroll == 1)
-            lookupShiftedKernel<In, Out, Tok, N, 1><<<blocks, kLookupThreads, 0, s>>>(a);
+            launchBehind(lookupShiftedKernel<In, Out, Tok, N, 1>, blocks, kLookupThreads, 0, s, a, who);
         else if (Shifted)
-            lookupShiftedKernel<In, Out, Tok, N, 4><<<blocks, kLookupThreads, 0, s>>>(a);
+            launchBehind(lookupShiftedKernel<In, Out, Tok, N, 4>, blocks, kLookupThreads, 0, s, a, who);
         else if (unroll == 1)
             lookupKernel<In, Out, Tok, N, 1><<<blocks, kLookupThreads, 0, s>>>(a);
         else
@@ -1470,16 +1478,18 @@ void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaSt
     cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
     if (ctas > 8)
         cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), who);
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim = {ctas, 1, 1};
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {ctas, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks, 1, 1);
     config.blockDim = dim3(kClusterThreads, 1, 1);
     config.dynamicSmemBytes = shared;
     config.stream = s;
-    config.attrs = &attr;
-    config.numAttrs = 1;
+    config.attrs = attr;
+    config.numAttrs = 2;
     cudaCheck(cudaLaunchKernelEx(&config, kernel, a), who);
 }
 

@@ -9,8 +9,8 @@
 // are a few megabytes at most, so the calls are bound by the launch and by one chain of
 // dependent reads. Up to kScanInBlock requests every CTA scans all of them itself into shared
 // memory: one launch, no wait on another CTA. Past it the scan is a kernel of its own, of one
-// CTA, that leaves it in scratch: 300 CTAs that each read 8191 requests took 7 us over
-// that, a CTA alone 3 and the start of a second kernel 1.
+// CTA, that leaves it in scratch: 300 CTAs that each read 8191 requests took 7 us over that,
+// one CTA and the start of a second kernel 4.
 #include "sequences.cuh"
 
 #include <algorithm>
@@ -20,10 +20,11 @@
 namespace eb {
 namespace {
 
-constexpr uint32_t kItems = 8;  // requests a thread scans
-constexpr int kThreads = 256, kScanThreads = 1024;
+constexpr uint32_t kItems = 4;  // requests a thread scans
+constexpr int kThreads = 512, kScanThreads = 1024;
 constexpr uint32_t kScanInBlock = kThreads * kItems;    // 2048
-constexpr uint32_t kScanAtOnce = kScanThreads * kItems; // 8192
+constexpr uint32_t kScanAtOnce = kScanThreads * kItems; // 4096
+constexpr uint32_t kMostCopied = 8192;  // requests whose scan fits shared memory
 constexpr uint32_t kWarps = kThreads / 32;
 
 struct PagedArgs {
@@ -226,6 +227,7 @@ __global__ __launch_bounds__(kScanThreads) void scanKernel(PagedArgs a)
     __shared__ uint32_t upto[kScanAtOnce];
     __shared__ uint32_t segment[kMaxSegments + 1];
     letNextKernelStart();
+    waitForKernelBefore();
     if (threadIdx.x == 0 && a.cells != nullptr)
         a.cells[1] = 0;
     uint32_t carry = 0;
@@ -263,10 +265,11 @@ __device__ __forceinline__ uint32_t requestFrom(const uint32_t* upto, uint32_t r
 
 // ------------------------------------------------------------------ block tables
 
-constexpr uint32_t kEntries = 512;  // of a request's new or returned blocks per warp
-constexpr int kAhead = 4;
+/** Of a request's new or returned blocks, what a warp takes, all of them in flight: few where a
+ *  request's state is at hand in shared memory, so that more warps share a request. */
+constexpr uint32_t entriesOf(bool inBlock) { return inBlock ? 128u : 512u; }
 
-/** A warp takes up to kEntries blocks of one request: those it gets are copied from the pool, and
+/** A warp takes a few blocks of one request: those it gets are copied from the pool, and
  *  those a terminated one gives back are cleared. (One search per entry of the pool's front
  *  instead, 100 instructions per 32 entries against 15, took twice as long.) The requests are
  *  spread over the CTAs for what they hold now, too. */
@@ -280,8 +283,8 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
     const uint32_t* upto = InBlock ? sUpto : a.upto;
     const uint32_t lane = threadIdx.x & 31u, warp = blockIdx.x * kWarps + (threadIdx.x >> 5),
                    warps = gridDim.x * kWarps;
-    if constexpr (!InBlock)
-        waitForKernelBefore();
+    letNextKernelStart();
+    waitForKernelBefore();
     const uint32_t given = __ldg(a.count);
     const uint32_t available = uint64_t(given) > uint64_t(a.poolSize) ? 0u : given;
     if (threadIdx.x == 0)
@@ -302,6 +305,8 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
         return b;
     };
 
+    constexpr uint32_t kEntries = entriesOf(InBlock);
+    constexpr int kAhead = int(kEntries / 32);
     const uint64_t tasks = uint64_t(a.requests) * a.pieces;
     for (uint64_t task = warp; task < tasks; task += warps) {
         const uint32_t r = a.pieces == 1 ? uint32_t(task) : uint32_t(task / a.pieces);
@@ -313,31 +318,27 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
             if (j0 - lane >= adds || sum > available)
                 continue;
             const int32_t* from = a.pool + (sum - adds);
-            for (uint32_t j = j0; j < min(j0 - lane + kEntries, adds); j += 32 * kAhead) {
-                int32_t id[kAhead];
+            int32_t id[kAhead];
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u)
-                    id[u] = j + 32u * u < adds ? __ldg(from + j + 32u * u) : -1;
+            for (int u = 0; u < kAhead; ++u)
+                id[u] = j0 + 32u * u < adds ? __ldg(from + j0 + 32u * u) : -1;
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u) {
-                    if (j + 32u * u < adds) {
-                        row[b.held + j + 32u * u] = id[u];
-                        if (a.used != nullptr && id[u] >= 0 && int64_t(id[u]) < a.usedSize)
-                            a.used[id[u]] = 1;
-                    }
+            for (int u = 0; u < kAhead; ++u) {
+                if (j0 + 32u * u < adds) {
+                    row[b.held + j0 + 32u * u] = id[u];
+                    if (a.used != nullptr && id[u] >= 0 && int64_t(id[u]) < a.usedSize)
+                        a.used[id[u]] = 1;
                 }
             }
-        } else if (a.used != nullptr) {
-            for (uint32_t j = j0; j < min(j0 - lane + kEntries, b.held); j += 32 * kAhead) {
-                int32_t id[kAhead];
+        } else if (a.used != nullptr && j0 - lane < b.held) {
+            int32_t id[kAhead];
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u)
-                    id[u] = j + 32u * u < b.held ? row[j + 32u * u] : -1;
+            for (int u = 0; u < kAhead; ++u)
+                id[u] = j0 + 32u * u < b.held ? row[j0 + 32u * u] : -1;
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u)
-                    if (id[u] >= 0 && int64_t(id[u]) < a.usedSize)
-                        a.used[id[u]] = 0;
-            }
+            for (int u = 0; u < kAhead; ++u)
+                if (id[u] >= 0 && int64_t(id[u]) < a.usedSize)
+                    a.used[id[u]] = 0;
         }
     }
 
@@ -379,21 +380,21 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 
 // ------------------------------------------------------------------ slots
 
-constexpr uint32_t kTokens = 4;  // neighbouring tokens per thread and step
-
-/** ``Copied``: the scan is read from scratch into shared memory first (up to kScanAtOnce requests),
+/** kTokens neighbouring tokens a thread and step: four, stored as words, or one where that leaves
+ *  SMs idle. ``Copied``: the scan is read from scratch into shared memory first (up to kMostCopied requests),
  *  where a search is a tenth of the time. */
-template <class Len, class Slot, bool InBlock, bool Copied>
+template <class Len, class Slot, uint32_t kTokens, bool InBlock, bool Copied>
 __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
 {
     __shared__ uint32_t segment[InBlock ? kMaxSegments + 1 : 1];
     __shared__ int64_t starts[InBlock ? kScanInBlock : 1];
-    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : (Copied ? kScanAtOnce : 1)];
+    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : (Copied ? kMostCopied : 1)];
     const uint32_t* upto = InBlock || Copied ? sUpto : a.upto;
+    letNextKernelStart();
+    waitForKernelBefore();
     if constexpr (InBlock) {
         (void)scanBlock<kThreads, Tokens, Len>(a, 0, 0, sUpto, starts, segment);
     } else {
-        waitForKernelBefore();
         if constexpr (Copied) {
 #pragma unroll 8
             for (uint32_t i = threadIdx.x; i < a.requests; i += kThreads)
@@ -499,14 +500,28 @@ void withLength(uint32_t type, F&& f)
 template <class What, class Len>
 void launchScan(const PagedArgs& a, cudaStream_t s, const char* who)
 {
-    scanKernel<What, Len><<<1, kScanThreads, 0, s>>>(a);
-    launchCheck(who);
+    launchBehind(scanKernel<What, Len>, 1, kScanThreads, 0, s, a, who);
 }
 
 /** CTAs for ``threads`` threads' work, at most ``most`` an SM. */
 unsigned gridFor(int64_t threads, int64_t most)
 {
     return unsigned(std::max<int64_t>(1, std::min(most * smCount(), (threads + kThreads - 1) / kThreads)));
+}
+
+template <class Len, class Slot, uint32_t kTokens>
+void launchSlots(const PagedArgs& a, cudaStream_t s, const char* who)
+{
+    const int64_t threads = (int64_t(a.capacity) + kTokens - 1) / kTokens;
+    if (a.requests <= kScanInBlock) {
+        launchBehind(slotMapKernel<Len, Slot, kTokens, true, false>, gridFor(threads, 4), kThreads, 0, s, a, who);
+        return;
+    }
+    launchScan<Tokens, Len>(a, s, who);
+    if (a.requests <= kMostCopied)
+        launchBehind(slotMapKernel<Len, Slot, kTokens, false, true>, gridFor(threads, 4), kThreads, 0, s, a, who);
+    else
+        launchBehind(slotMapKernel<Len, Slot, kTokens, false, false>, gridFor(threads, 4), kThreads, 0, s, a, who);
 }
 
 }  // namespace
@@ -555,16 +570,16 @@ EB_API eagle_backend_status eagle_backend_x_b200_block_tables(eagle_b200_paged_d
         a.blocks = reinterpret_cast<int32_t*>(d.blocks);
         a.cells = reinterpret_cast<uint32_t*>(d.cells);
         const cudaStream_t s = seamStream(d.stream);
-        a.pieces = uint32_t(std::max<int64_t>(1, (d.width + kEntries - 1) / kEntries));
+        const int64_t entries = entriesOf(d.requests <= int64_t(kScanInBlock));
+        a.pieces = uint32_t(std::max<int64_t>(1, (d.width + entries - 1) / entries));
         withLength(d.length_type, [&](auto len) {
             using Len = decltype(len);
             const int64_t threads = d.requests * a.pieces * 32;  // a warp per request's share
             if (d.requests <= int64_t(kScanInBlock)) {
-                blockTablesKernel<Len, true><<<gridFor(threads, 2), kThreads, 0, s>>>(a);
-                launchCheck(who);
+                launchBehind(blockTablesKernel<Len, true>, gridFor(threads, 4), kThreads, 0, s, a, who);
             } else {
                 launchScan<Blocks, Len>(a, s, who);
-                launchBehind(blockTablesKernel<Len, false>, gridFor(threads, 8), kThreads, 0, s, a, who);
+                launchBehind(blockTablesKernel<Len, false>, gridFor(threads, 4), kThreads, 0, s, a, who);
             }
         });
     });
@@ -613,17 +628,10 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
             withLength(d.slot_type, [&](auto slot) {
                 using Len = decltype(len);
                 using Slot = decltype(slot);
-                const int64_t threads = (d.capacity + kTokens - 1) / kTokens;
-                if (d.requests <= int64_t(kScanInBlock)) {
-                    slotMapKernel<Len, Slot, true, false><<<gridFor(threads, 4), kThreads, 0, s>>>(a);
-                    launchCheck(who);
-                } else {
-                    launchScan<Tokens, Len>(a, s, who);
-                    if (d.requests <= int64_t(kScanAtOnce))
-                        launchBehind(slotMapKernel<Len, Slot, false, true>, gridFor(threads, 6), kThreads, 0, s, a, who);
-                    else
-                        launchBehind(slotMapKernel<Len, Slot, false, false>, gridFor(threads, 8), kThreads, 0, s, a, who);
-                }
+                if (d.capacity <= int64_t(smCount()) * kThreads)
+                    launchSlots<Len, Slot, 1>(a, s, who);
+                else
+                    launchSlots<Len, Slot, 4>(a, s, who);
             });
         });
     });
