@@ -461,20 +461,20 @@ __device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint
 // ---- up to kClusterKeys: one cluster, the keys in its distributed shared memory
 
 constexpr int kClusterThreads = 1024;
-constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterSize = 16;  // past the portable 8: asked for only where more than 8 are needed
 constexpr int kClusterItems = 8;
 constexpr uint32_t kClusterKeys = uint32_t(kClusterThreads) * kClusterSize * kClusterItems;  // 131072
 constexpr uint32_t kPortableKeys = kClusterKeys / 2;
-constexpr uint32_t kPeerBytes = uint32_t(kClusterWarps) * kMaxBins * 4;
+constexpr uint32_t kSmallKeys = 1024;  // up to here in a CTA of 512 threads, which meet at barriers sooner
+constexpr uint32_t peerBytes(int threads) { return uint32_t(threads) / 32u * kMaxBins * 4u; }
 
-/** Cluster 0 sorts: every CTA holds 1024 * Items neighbouring keys in registers; a pass ranks
+/** Cluster 0 sorts: every CTA holds Threads * Items neighbouring keys in registers; a pass ranks
  *  them, puts them in digit order in the CTA's own shared memory, adds up the CTAs' digit
  *  counts over distributed shared memory and stores each key and position into the CTA that
  *  has its place, neighbours mostly to neighbours; two cluster barriers in all. The other
  *  clusters meanwhile zero the first ``zeroed`` rows. */
-template <class Tok, int Items>
-__global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
+template <class Tok, int Threads, int Items>  // Threads >= kMaxBins: a thread per bin
+__global__ __launch_bounds__(Threads) void clusterSortKernel(GradArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ uint32_t tileCount[kMaxBins], base[kMaxBins], scan[33];
@@ -491,28 +491,28 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
             constexpr int64_t kPiece = 65536;
             const int64_t bytes = a.zeroed * a.rowBytes;
             for (int64_t from = at * kPiece; from < bytes; from += others * kPiece)
-                zeroBytes(table + from, table + min(from + kPiece, bytes), threadIdx.x, kClusterThreads);
+                zeroBytes(table + from, table + min(from + kPiece, bytes), threadIdx.x, Threads);
         } else {
-            for (int64_t r = int64_t(at) * kClusterWarps + (threadIdx.x >> 5); r < a.zeroed;
-                 r += int64_t(others) * kClusterWarps)
+            for (int64_t r = int64_t(at) * (Threads / 32) + (threadIdx.x >> 5); r < a.zeroed;
+                 r += int64_t(others) * (Threads / 32))
                 zeroBytes(table + r * a.strideBytes, table + r * a.strideBytes + a.rowBytes, threadIdx.x & 31u, 32u);
         }
         return;
     }
-    constexpr uint32_t kTile = uint32_t(kClusterThreads) * Items;
+    constexpr uint32_t kTile = uint32_t(Threads) * Items, kPeers = peerBytes(Threads);
     uint64_t* at = reinterpret_cast<uint64_t*>(raw);  // key and position by place in the order
     uint64_t* own = at + kTile;                       // by place among the CTA's
     // the lanes' words take the memory of ``own``, empty while they are in use, if that is enough
-    uint32_t* peers = reinterpret_cast<uint32_t*>(kTile * 8 >= kPeerBytes ? own : own + kTile);
+    uint32_t* peers = reinterpret_cast<uint32_t*>(kTile * 8 >= kPeers ? own : own + kTile);
     uint16_t* count = reinterpret_cast<uint16_t*>(
-        reinterpret_cast<char*>(own) + (kTile * 8 >= kPeerBytes ? kTile * 8 : kTile * 8 + kPeerBytes));
+        reinterpret_cast<char*>(own) + (kTile * 8 >= kPeers ? kTile * 8 : kTile * 8 + kPeers));
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t item0 = warp * (32u * Items) + lane;
     if (cta == 0 && threadIdx.x < 2)
         a.listCount[threadIdx.x] = 0;
     if (a.present != nullptr)
-        for (int64_t w = int64_t(cta) * kClusterThreads + threadIdx.x; w < (a.rows + 31) / 32;
-             w += int64_t(ctas) * kClusterThreads)
+        for (int64_t w = int64_t(cta) * Threads + threadIdx.x; w < (a.rows + 31) / 32;
+             w += int64_t(ctas) * Threads)
             a.present[w] = 0;
     uint32_t key[Items], pos[Items], rank[Items];
     loadKeys<Tok, Items>(a, cta * kTile + item0, 32u, key);
@@ -520,7 +520,7 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
     for (int k = 0; k < Items; ++k)
         pos[k] = cta * kTile + item0 + 32u * k;
     for (uint32_t shift = 0; shift < a.bits; shift += a.digitBits) {
-        const uint32_t mine = rankItems<kClusterWarps, Items>(key, shift, a.digitBits, rank, count, peers);
+        const uint32_t mine = rankItems<(Threads / 32), Items>(key, shift, a.digitBits, rank, count, peers);
         uint32_t all = 0;
         const uint32_t first = blockExclusiveSum(mine, all, scan);
         if (threadIdx.x < a.bins) {
@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < Items; ++k) {
-            const uint32_t j = uint32_t(k) * kClusterThreads + threadIdx.x;
+            const uint32_t j = uint32_t(k) * Threads + threadIdx.x;
             const uint64_t v = own[j];
             const uint32_t to = base[(uint32_t(v) >> shift) & (a.bins - 1u)] + j;
             cluster.map_shared_rank(at, to / kTile)[to % kTile] = v;
@@ -1348,10 +1348,10 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
     });
 }
 
-size_t clusterShared(int items)
+size_t clusterShared(int threads, int items)
 {
-    const size_t keys = size_t(kClusterThreads) * items * 8;
-    return 2 * keys + (keys >= kPeerBytes ? 0 : kPeerBytes) + size_t(kClusterWarps) * kMaxBins * 2;
+    const size_t keys = size_t(threads) * items * 8, peers = peerBytes(threads);
+    return 2 * keys + (keys >= peers ? 0 : peers) + peers / 2;
 }
 
 /** Whether the current device holds a cluster of kClusterSize CTAs of the sort (kept per device). */
@@ -1365,14 +1365,14 @@ bool largeClusters()
     if (int(known.size()) <= dev)
         known.resize(size_t(dev) + 1, 0);
     if (known[size_t(dev)] == 0) {
-        auto kernel = clusterSortKernel<int32_t, kClusterItems>;
+        auto kernel = clusterSortKernel<int32_t, kClusterThreads, kClusterItems>;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim = {unsigned(kClusterSize), 1, 1};
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(kClusterSize, 1, 1);
         config.blockDim = dim3(kClusterThreads, 1, 1);
-        config.dynamicSmemBytes = clusterShared(kClusterItems);
+        config.dynamicSmemBytes = clusterShared(kClusterThreads, kClusterItems);
         config.attrs = &attr;
         config.numAttrs = 1;
         int clusters = 0;
@@ -1470,11 +1470,11 @@ void launchBulkSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const cha
     launchBehind(kernel, blocks, kBulkThreads, sizeof(BulkShared), s, a, who);
 }
 
-template <class Tok, int Items>
+template <class Tok, int Threads, int Items>
 void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaStream_t s, const char* who)
 {
-    auto kernel = clusterSortKernel<Tok, Items>;
-    const size_t shared = clusterShared(Items);
+    auto kernel = clusterSortKernel<Tok, Threads, Items>;
+    const size_t shared = clusterShared(Threads, Items);
     cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
     if (ctas > 8)
         cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), who);
@@ -1485,7 +1485,7 @@ void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaSt
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks, 1, 1);
-    config.blockDim = dim3(kClusterThreads, 1, 1);
+    config.blockDim = dim3(Threads, 1, 1);
     config.dynamicSmemBytes = shared;
     config.stream = s;
     config.attrs = attr;
@@ -1571,17 +1571,18 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     if (p.n <= kPortableKeys || (p.n <= kClusterKeys && largeClusters())) {
         a.keyOut = words(p.key[0]);
         a.posOut = words(p.pos[0]);
-        unsigned ctas = 1;
         // what one CTA holds needs no exchange; past that, as many as the cluster may have
+        unsigned ctas = 1;
         if (p.n > uint32_t(kClusterThreads) * kClusterItems)
             ctas = p.n <= kPortableKeys ? 8u : unsigned(kClusterSize);
-        const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
-        // 1024 threads an SM: the SMs beside the cluster, in whole clusters
+        const unsigned threads = p.n <= kSmallKeys ? 512u : unsigned(kClusterThreads);
+        const unsigned perThread = (p.n + ctas * threads - 1) / (ctas * threads);
+        // the SMs beside the cluster, 1024 threads each, in whole clusters
         unsigned blocks = ctas;
         if (!accumulate) {
             a.zeroed = std::min(d.rows, zeroedBesideSort(perThread) / a.rowBytes);
-            const int64_t besides =
-                std::min<int64_t>((a.zeroed * a.rowBytes / 65536 + ctas) / ctas, sms / ctas - 1);
+            const int64_t besides = std::min<int64_t>((a.zeroed * a.rowBytes / 65536 + ctas) / ctas,
+                sms * unsigned(kClusterThreads) / threads / ctas - 1);
             if (besides > 0)
                 blocks += unsigned(besides) * ctas;
             else
@@ -1590,13 +1591,15 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         withIndex(d.token_type, [&](auto tok) {
             using Tok = decltype(tok);
             if (perThread <= 1)
-                launchClusterSort<Tok, 1>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, 512, 1>(a, ctas, blocks, s, who);
+            else if (threads == 512)
+                launchClusterSort<Tok, 512, 2>(a, ctas, blocks, s, who);
             else if (perThread <= 2)
-                launchClusterSort<Tok, 2>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, kClusterThreads, 2>(a, ctas, blocks, s, who);
             else if (perThread <= 4)
-                launchClusterSort<Tok, 4>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, kClusterThreads, 4>(a, ctas, blocks, s, who);
             else
-                launchClusterSort<Tok, kClusterItems>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, kClusterThreads, kClusterItems>(a, ctas, blocks, s, who);
         });
         a.keys = a.keyOut;
         a.order = a.posOut;

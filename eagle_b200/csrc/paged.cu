@@ -20,11 +20,10 @@
 namespace eb {
 namespace {
 
-constexpr uint32_t kItems = 4;  // requests a thread scans
-constexpr int kThreads = 512, kScanThreads = 1024;
-constexpr uint32_t kScanInBlock = kThreads * kItems;    // 2048
-constexpr uint32_t kScanAtOnce = kScanThreads * kItems; // 4096
-constexpr uint32_t kMostCopied = 8192;  // requests whose scan fits shared memory
+constexpr int kThreads = 512, kItems = 4;            // requests a thread scans where every CTA scans
+constexpr int kScanThreads = 1024, kScanItems = 8;   // where one does
+constexpr uint32_t kScanInBlock = kThreads * kItems;         // 2048
+constexpr uint32_t kScanAtOnce = kScanThreads * kScanItems;  // 8192
 constexpr uint32_t kWarps = kThreads / 32;
 
 struct PagedArgs {
@@ -157,29 +156,29 @@ __device__ __forceinline__ uint32_t warpInclusive(uint32_t v)
     return v;
 }
 
-constexpr uint32_t kMaxSegments = kItems * (kScanThreads / 32);
+constexpr uint32_t kMaxSegments = kScanItems * (kScanThreads / 32);
 
-/** Requests [from, from + Threads * kItems), Threads neighbours at a time (a thread reading its own
+/** Requests [from, from + Threads * Items), Threads neighbours at a time (a thread reading its own
  *  neighbours instead took 13 us for 8191 requests), all read at once: their inclusive sums on
  *  top of ``carry`` go to ``upto`` and what they keep to ``kept``. Every warp scans its 32 of each
  *  step, the first one those segments' sums. Returns the new carry. ``segment`` is kMaxSegments
  *  + 1 words of shared memory. */
-template <int Threads, class What, class Len>
+template <int Threads, int Items, class What, class Len>
 __device__ __forceinline__ uint32_t scanBlock(const PagedArgs& a, uint32_t from, uint32_t carry, uint32_t* upto,
     typename What::Kept* kept, uint32_t* segment)
 {
     constexpr uint32_t kOwn = Threads / 32;
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    const uint32_t m = min(a.requests - from, uint32_t(Threads) * kItems);
+    const uint32_t m = min(a.requests - from, uint32_t(Threads * Items));
     const uint32_t items = (m + Threads - 1) / Threads;
-    typename What::template Raw<Len> raw[kItems];
-    uint32_t sum[kItems];
+    typename What::template Raw<Len> raw[Items];
+    uint32_t sum[Items];
 #pragma unroll
-    for (uint32_t k = 0; k < kItems; ++k)
+    for (uint32_t k = 0; k < uint32_t(Items); ++k)
         if (k < items)
             raw[k].read(a, from + min(k * Threads + threadIdx.x, m - 1u));
 #pragma unroll
-    for (uint32_t k = 0; k < kItems; ++k) {
+    for (uint32_t k = 0; k < uint32_t(Items); ++k) {
         if (k < items) {
             const uint32_t i = k * Threads + threadIdx.x;
             What what;
@@ -194,7 +193,7 @@ __device__ __forceinline__ uint32_t scanBlock(const PagedArgs& a, uint32_t from,
     }
     __syncthreads();
     if (warp == 0) {
-        constexpr uint32_t kEach = kItems * kOwn / 32;  // segments a lane adds up
+        constexpr uint32_t kEach = Items * kOwn / 32;  // segments a lane adds up
         uint32_t mine[kEach], total = 0;
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) {
@@ -213,7 +212,7 @@ __device__ __forceinline__ uint32_t scanBlock(const PagedArgs& a, uint32_t from,
     }
     __syncthreads();
 #pragma unroll
-    for (uint32_t k = 0; k < kItems; ++k)
+    for (uint32_t k = 0; k < uint32_t(Items); ++k)
         if (k < items && k * Threads + threadIdx.x < m)
             upto[k * Threads + threadIdx.x] = addUpTo(segment[k * kOwn + warp], sum[k]);
     __syncthreads();
@@ -232,7 +231,7 @@ __global__ __launch_bounds__(kScanThreads) void scanKernel(PagedArgs a)
         a.cells[1] = 0;
     uint32_t carry = 0;
     for (uint32_t from = 0; from < a.requests; from += kScanAtOnce) {
-        carry = scanBlock<kScanThreads, What, Len>(a, from, carry, upto, nullptr, segment);
+        carry = scanBlock<kScanThreads, kScanItems, What, Len>(a, from, carry, upto, nullptr, segment);
         for (uint32_t i = threadIdx.x; i < min(a.requests - from, kScanAtOnce); i += kScanThreads)
             a.upto[from + i] = upto[i];
         __syncthreads();
@@ -267,7 +266,7 @@ __device__ __forceinline__ uint32_t requestFrom(const uint32_t* upto, uint32_t r
 
 /** Of a request's new or returned blocks, what a warp takes, all of them in flight: few where a
  *  request's state is at hand in shared memory, so that more warps share a request. */
-constexpr uint32_t entriesOf(bool inBlock) { return inBlock ? 128u : 512u; }
+constexpr uint32_t entriesOf(bool inBlock) { return inBlock ? 128u : 256u; }
 
 /** A warp takes a few blocks of one request: those it gets are copied from the pool, and
  *  those a terminated one gives back are cleared. (One search per entry of the pool's front
@@ -290,7 +289,7 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
     if (threadIdx.x == 0)
         sShort = 0;
     if constexpr (InBlock)
-        (void)scanBlock<kThreads, Blocks, Len>(a, 0, 0, sUpto, kept, segment);
+        (void)scanBlock<kThreads, kItems, Blocks, Len>(a, 0, 0, sUpto, kept, segment);
     else
         __syncthreads();
     auto request = [&](uint32_t r) {
@@ -381,19 +380,19 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 // ------------------------------------------------------------------ slots
 
 /** kTokens neighbouring tokens a thread and step: four, stored as words, or one where that leaves
- *  SMs idle. ``Copied``: the scan is read from scratch into shared memory first (up to kMostCopied requests),
+ *  SMs idle. ``Copied``: the scan is read from scratch into shared memory first (up to kScanAtOnce requests),
  *  where a search is a tenth of the time. */
 template <class Len, class Slot, uint32_t kTokens, bool InBlock, bool Copied>
 __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
 {
     __shared__ uint32_t segment[InBlock ? kMaxSegments + 1 : 1];
     __shared__ int64_t starts[InBlock ? kScanInBlock : 1];
-    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : (Copied ? kMostCopied : 1)];
+    __shared__ uint32_t sUpto[InBlock ? kScanInBlock : (Copied ? kScanAtOnce : 1)];
     const uint32_t* upto = InBlock || Copied ? sUpto : a.upto;
     letNextKernelStart();
     waitForKernelBefore();
     if constexpr (InBlock) {
-        (void)scanBlock<kThreads, Tokens, Len>(a, 0, 0, sUpto, starts, segment);
+        (void)scanBlock<kThreads, kItems, Tokens, Len>(a, 0, 0, sUpto, starts, segment);
     } else {
         if constexpr (Copied) {
 #pragma unroll 8
@@ -518,7 +517,7 @@ void launchSlots(const PagedArgs& a, cudaStream_t s, const char* who)
         return;
     }
     launchScan<Tokens, Len>(a, s, who);
-    if (a.requests <= kMostCopied)
+    if (a.requests <= kScanAtOnce)
         launchBehind(slotMapKernel<Len, Slot, kTokens, false, true>, gridFor(threads, 4), kThreads, 0, s, a, who);
     else
         launchBehind(slotMapKernel<Len, Slot, kTokens, false, false>, gridFor(threads, 4), kThreads, 0, s, a, who);
