@@ -15,8 +15,8 @@ As with ``Compactor`` and ``Reducer`` a class prepares a call -- it checks the t
 holds them and allocates outputs and workspace once -- and calling it only enqueues
 (and can be captured in a CUDA graph); the function of the same name prepares and calls.
 Calls of one prepared object share its outputs and workspace: those that may overlap on
-the GPU must be ordered by the caller, two graphs captured from it included.
-No operator here records an autograd graph.
+the GPU must be ordered by the caller, two graphs captured from it included; a graph does
+not keep the object, its owner does. No operator here records an autograd graph.
 """
 
 from __future__ import annotations
@@ -92,6 +92,12 @@ def _raw_stream(device):
 _current = None
 
 
+def _capturing(handle):
+    flag = ctypes.c_int32()
+    _abi.check(_abi.lib().eagle_backend_stream_is_capturing(handle, ctypes.byref(flag)))
+    return bool(flag.value)
+
+
 class _Call:
     """A prepared call: ``_desc`` and the C entry, enqueued on the tensors' device."""
 
@@ -110,8 +116,9 @@ class _Call:
             if stream.device != self.device:
                 raise ValueError(f"the stream is on {stream.device}, the tensors on {self.device}")
             handle = stream.cuda_stream
-        if handle != self._home:
-            # the allocator may hand these out again once they are dropped: not before this stream is past the call
+        if handle != self._home and not _capturing(handle):
+            # the allocator may hand these out again once they are dropped: not before this stream is past the
+            # call (a capture runs nothing: what its graph uses, the graph's owner keeps)
             s = stream if stream is not None else _t().cuda.current_stream(self.device)
             for t in self._owned:
                 t.record_stream(s)
@@ -205,7 +212,7 @@ class Embedding(_Call):
             raise ValueError("the table must be (rows, dim) with contiguous rows")
         if table.numel() > 0 and table.shape[0] > 1 and table.stride(0) < table.shape[1]:
             raise ValueError("the table's rows overlap")
-        _no_grad("embedding", table)
+        _no_grad("embedding", table, out)
         shape = (*tokens.shape, table.shape[1])
         _type(tokens.dtype, "tokens", "index")
         _type(dtype or table.dtype, "the table and dtype", "element")

@@ -58,7 +58,7 @@ constexpr int kLookupThreads = 256;
 template <class Tok>
 __device__ __forceinline__ int64_t rowOfToken(const void* tokens, int64_t at, int64_t first, int64_t rows)
 {
-    const int64_t id = int64_t(__ldg(reinterpret_cast<const Tok*>(tokens) + at));
+    const int64_t id = int64_t(reinterpret_cast<const Tok*>(tokens)[at]);
     if (id < first)
         return -1;
     const uint64_t r = uint64_t(id) - uint64_t(first);  // first >= 0, so the difference is exact
@@ -147,8 +147,8 @@ __device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
     const uint64_t at = reinterpret_cast<uint64_t>(p);
     const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
     const uint32_t skip = uint32_t(at) & 15u;
-    const uint4 lo = __ldg(word);
-    const uint4 hi = skip + valid > 16u ? __ldg(word + 1) : make_uint4(0u, 0u, 0u, 0u);
+    const uint4 lo = *word;
+    const uint4 hi = skip + valid > 16u ? word[1] : make_uint4(0u, 0u, 0u, 0u);
     return shiftWords(lo, hi, skip);
 }
 
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookupShiftedKernel(LookupArgs
 /** 32 bytes in one load (two of 16 bytes each touch every sector twice); ``p`` is 32-byte aligned. */
 __device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi)
 {
-    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
                  : "l"(p));
 }
@@ -256,7 +256,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
                     if constexpr (Shifted)
                         got[u][w] = loadShifted(p + w * (N / kWords), 16u);
                     else if constexpr (kWords == 1)
-                        got[u][w] = __ldg(reinterpret_cast<const uint4*>(p));
+                        got[u][w] = *reinterpret_cast<const uint4*>(p);
                     else if (w == 0)
                         load32(p, got[u][0], got[u][kWords - 1]);
                 }
@@ -312,6 +312,7 @@ struct GradArgs {
     uint32_t* present;   // a bit per row that has a token
     uint32_t* hist;      // this pass's digit counts, [tile][bin]
     uint32_t* nextHist;  // the next pass's, gathered by this one
+    uint32_t* totals;    // the digits' counts over all tiles, hist then scanned over the tiles; or null
     const uint32_t* keyIn;
     const uint32_t* posIn;
     uint32_t* keyOut;
@@ -351,7 +352,7 @@ __device__ __forceinline__ void loadKeys(const GradArgs& a, uint32_t from, uint3
     for (int k = 0; k < Items; ++k) {
         const uint32_t i = min(from + uint32_t(k) * step, a.n - 1u);
         const uint32_t b = a.flatTokens ? 0u : a.perBatch(i);
-        id[k] = __ldg(tokens + int64_t(b) * a.tokenBatch + int64_t(i - b * a.perBatch.d) * a.tokenSeq);
+        id[k] = tokens[int64_t(b) * a.tokenBatch + int64_t(i - b * a.perBatch.d) * a.tokenSeq];
     }
 #pragma unroll
     for (int k = 0; k < Items; ++k) {
@@ -392,7 +393,7 @@ __device__ __forceinline__ void zeroUnit(const GradArgs& a, const uint32_t* pres
     const int64_t piece = int64_t(unit - which * a.zeroPieces) * kZeroUnit;
     const int64_t begin = row0 + int64_t(which) * a.zeroRows, end = min(begin + int64_t(a.zeroRows), row1);
     auto absent = [&](int64_t r) {
-        return present == nullptr || ((__ldg(present + (r >> 5)) >> (r & 31)) & 1u) == 0;
+        return present == nullptr || ((present[r >> 5] >> (r & 31)) & 1u) == 0;
     };
     if (a.rowBytes <= kZeroByWarp) {
         for (int64_t r = begin + (threadIdx.x >> 5); r < end; r += blockDim.x >> 5)
@@ -586,6 +587,7 @@ constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortItems = 8;
 constexpr uint32_t kSortTile = uint32_t(kSortThreads) * kSortItems;  // 4096 keys
+constexpr uint32_t kTilesAdded = 128;  // adding up so many in every tile costs what the scan's launch does
 
 /** A tile's digit counts of the first pass, and the rows that have a token. */
 template <class Tok>
@@ -614,8 +616,40 @@ __global__ __launch_bounds__(kSortThreads) void histogramKernel(GradArgs a)
         a.hist[size_t(blockIdx.x) * a.bins + threadIdx.x] = count[threadIdx.x];
 }
 
+/** The tiles' counts of each bin, scanned in place over the tiles, and their sums: a CTA takes 32
+ *  bins and cuts the tiles into 32 stretches, added up, scanned and gone over again. */
+__global__ __launch_bounds__(1024) void columnScanKernel(GradArgs a)
+{
+    __shared__ uint32_t sum[32][33];
+    letNextKernelStart();
+    waitForKernelBefore();
+    const uint32_t column = threadIdx.x & 31u, stretch = threadIdx.x >> 5, bin = blockIdx.x * 32u + column;
+    const uint32_t each = (a.tiles + 31u) / 32u, t0 = min(stretch * each, a.tiles), t1 = min(t0 + each, a.tiles);
+    uint32_t mine = 0;
+    if (bin < a.bins)
+#pragma unroll 8
+        for (uint32_t t = t0; t < t1; ++t)
+            mine += __ldcg(a.hist + size_t(t) * a.bins + bin);
+    sum[stretch][column] = mine;
+    __syncthreads();
+    uint32_t before = 0;
+    for (uint32_t s = 0; s < stretch; ++s)
+        before += sum[s][column];
+    if (bin >= a.bins)
+        return;
+    if (stretch == 31)
+        a.totals[bin] = before + mine;
+    for (uint32_t t = t0; t < t1; ++t) {
+        uint32_t* at = a.hist + size_t(t) * a.bins + bin;
+        const uint32_t c = __ldcg(at);
+        *at = before;
+        before += c;
+    }
+}
+
 /** One pass over one tile: a bin's first place is the keys of lower bins plus those of its
- *  own in earlier tiles, added up from every tile's counts by the bin's thread. */
+ *  own in earlier tiles, added up from every tile's counts by the bin's thread; past
+ *  kTilesAdded tiles, where that would grow with their square, a scan has done it. */
 template <bool First, class Tok>
 __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
 {
@@ -641,7 +675,10 @@ __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
         }
     }
     uint32_t before = 0, total = 0, all = 0;
-    if (threadIdx.x < a.bins) {
+    if (threadIdx.x < a.bins && a.totals != nullptr) {
+        before = __ldcg(a.hist + size_t(blockIdx.x) * a.bins + threadIdx.x);
+        total = __ldcg(a.totals + threadIdx.x);
+    } else if (threadIdx.x < a.bins) {
         const uint32_t* column = a.hist + threadIdx.x;
 #pragma unroll 16
         for (uint32_t t = 0; t < a.tiles; ++t) {
@@ -734,13 +771,13 @@ __device__ __forceinline__ void loadEight(uint32_t (&v)[kRowsInFlight], const ui
     uint32_t other)
 {
     if (i < n && n - i >= 8u) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(from + i));
-        const uint4 y = __ldg(reinterpret_cast<const uint4*>(from + i) + 1);
+        const uint4 x = *reinterpret_cast<const uint4*>(from + i);
+        const uint4 y = reinterpret_cast<const uint4*>(from + i)[1];
         v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
     } else {
 #pragma unroll
         for (uint32_t u = 0; u < kRowsInFlight; ++u)
-            v[u] = i < n && u < n - i ? __ldg(from + i + u) : other;
+            v[u] = i < n && u < n - i ? from[i + u] : other;
     }
 }
 
@@ -757,7 +794,7 @@ __device__ __forceinline__ int64_t vectorOf(const GradArgs& a, uint32_t t)
 __device__ __forceinline__ void listRun(const GradArgs& a, uint32_t chunk, uint32_t key)
 {
     const uint64_t past = (uint64_t(chunk) + kWarpParts) * a.chunk;  // the first of one partial too many
-    if (past < a.n && __ldg(a.keys + past) == key)
+    if (past < a.n && a.keys[past] == key)
         a.longList[atomicAdd(a.listCount + 1, 1u)] = chunk;
     else
         a.list[atomicAdd(a.listCount, 1u)] = chunk;
@@ -828,12 +865,12 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
     const uint32_t len = min(size, a.n - begin);
     for (uint32_t i = threadIdx.x; i <= 2 * size; i += kBulkThreads) {
         const bool in = i < a.n - begin;
-        s.key[i] = in ? __ldg(a.keys + begin + i) : kNoKey;
+        s.key[i] = in ? a.keys[begin + i] : kNoKey;
         if (i < 2 * size)
-            s.token[i] = in ? __ldg(a.order + begin + i) : 0u;
+            s.token[i] = in ? a.order[begin + i] : 0u;
     }
-    const uint32_t left = begin > 0 ? __ldg(a.keys + begin - 1) : kNoKey;
-    const uint32_t before = begin > 0 ? __ldg(a.keys + begin - size) : kNoKey;  // the chunk before's first
+    const uint32_t left = begin > 0 ? a.keys[begin - 1] : kNoKey;
+    const uint32_t before = begin > 0 ? a.keys[begin - size] : kNoKey;  // the chunk before's first
     if (threadIdx.x == 0) {
         for (uint32_t k = 0; k < kBulkStages; ++k) {
             mbarInit(&s.full[k], 1);
@@ -984,7 +1021,7 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
     // the first key of the d-th chunk from this one
     auto firstKey = [&](int d) {
         const int64_t i = (int64_t(chunk) + d) * a.chunk;
-        return i >= 0 && i < int64_t(a.n) ? __ldg(a.keys + i) : kNoKey;
+        return i >= 0 && i < int64_t(a.n) ? a.keys[i] : kNoKey;
     };
     uint32_t key[kRowsInFlight], token[kRowsInFlight];
     loadEight(key, a.keys, begin, a.n, kNoKey);
@@ -994,7 +1031,7 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
         return;
     uint32_t current = first, skipped = kNoKey;
     bool fromBefore = false;
-    if (begin > 0 && __ldg(a.keys + begin - 1) == first) {
+    if (begin > 0 && a.keys[begin - 1] == first) {
         if (firstKey(-1) == first || firstKey(1) == first) {
             fromBefore = true;
         } else {
@@ -1010,7 +1047,7 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
     bool extending = false, done = false;
     for (uint32_t i0 = begin; !done; i0 += kRowsInFlight) {
         if (i0 >= stop) {
-            if (extending || current == kNoKey || end == a.n || __ldg(a.keys + end) != current)
+            if (extending || current == kNoKey || end == a.n || a.keys[end] != current)
                 break;
             if (fromBefore)
                 break;
@@ -1029,7 +1066,7 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
                 continue;
             const int64_t at = vectorOf(a, token[u]);
             if constexpr (P == Piece::Aligned)
-                got[u] = __ldg(reinterpret_cast<const uint4*>(values + at + col0));
+                got[u] = *reinterpret_cast<const uint4*>(values + at + col0);
             else if constexpr (P == Piece::Shifted)
                 got[u] = loadShifted(values + at + col0, min(uint32_t(N), a.dim - col0) * uint32_t(sizeof(In)));
             else {
@@ -1088,7 +1125,7 @@ __global__ __launch_bounds__(kSumThreads) void sumKernel(GradArgs a)
         return;
     if (fromBefore) {
         storePartial<P, N>(a, a.head, chunk, col0, apart, acc);
-    } else if (!extending && end < a.n && __ldg(a.keys + end) == current) {
+    } else if (!extending && end < a.n && a.keys[end] == current) {
         storePartial<P, N>(a, a.tail, chunk, col0, apart, acc);
         if (slice == 0 && lane == 0)
             listRun(a, chunk, current);
@@ -1163,14 +1200,14 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
     for (uint64_t item = blockIdx.x; item < longItems; item += a.joinBlocks) {
         const uint32_t chunk = a.longList[item / blocks];
         const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
-        const uint32_t key = __ldg(a.keys + (chunk + 1u) * a.chunk);
+        const uint32_t key = a.keys[(chunk + 1u) * a.chunk];
         uint32_t m = 1;  // chunks after this one that the run reaches: the keys are sorted, so they are counted
         for (uint32_t more = 4 * kJoinThreads; more == 4 * kJoinThreads;) {
             bool in[4];
 #pragma unroll
             for (uint32_t u = 0; u < 4; ++u) {
                 const uint64_t c = uint64_t(chunk) + 1u + m + u * kJoinThreads + threadIdx.x;
-                in[u] = c < a.chunks && __ldg(a.keys + c * a.chunk) == key;
+                in[u] = c < a.chunks && a.keys[c * a.chunk] == key;
             }
             more = 0;
 #pragma unroll
@@ -1204,7 +1241,7 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
         const uint32_t chunk = a.list[item / blocks];
         const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
         const uint64_t next = uint64_t(chunk) + 1u + lane;
-        const uint32_t first = next < a.chunks ? __ldg(a.keys + next * a.chunk) : kNoKey;
+        const uint32_t first = next < a.chunks ? a.keys[next * a.chunk] : kNoKey;
         const uint32_t key = __shfl_sync(kFull, first, 0);
         const uint32_t parts = 1u + __popc(__ballot_sync(kFull, first == key));
         if (col < a.width)
@@ -1392,7 +1429,7 @@ struct GradPlan {
     Piece piece = Piece::Strided;
     uint32_t pieces = 0, group = 0, slices = 0, chunk = 0, chunks = 0, width = 0;
     uint64_t present = 0, listCount = 0, hist = 0, zeroed = 0;  // offsets; [0, zeroed) is cleared
-    uint64_t firstHist = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, longList = 0, head = 0, tail = 0, bytes = 0;
+    uint64_t firstHist = 0, totals = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, longList = 0, head = 0, tail = 0, bytes = 0;
 };
 
 GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
@@ -1443,6 +1480,7 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     p.hist = take(p.passes > 1 ? histBytes * (p.passes - 1) : 0);
     p.zeroed = at;
     p.firstHist = take(histBytes);
+    p.totals = take(portable ? 0 : p.bins * 4);
     for (int k = 0; k < (portable ? 1 : 2); ++k) {
         p.key[k] = take(uint64_t(p.n) * 4);
         p.pos[k] = take(uint64_t(p.n) * 4);
@@ -1619,6 +1657,10 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
                 b.posIn = words(p.pos[(k + 1) & 1]);
                 b.keyOut = words(p.key[k & 1]);
                 b.posOut = words(p.pos[k & 1]);
+                if (p.tiles > kTilesAdded) {
+                    b.totals = words(p.totals);
+                    launchBehind(columnScanKernel, (p.bins + 31) / 32, 1024, 0, s, b, who);
+                }
                 if (k == 0)
                     launchPass<true, Tok>(b, p.tiles, s, who);
                 else

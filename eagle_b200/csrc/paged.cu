@@ -56,7 +56,7 @@ struct PagedArgs {
 template <class Len>
 __device__ __forceinline__ int64_t lengthAt(const void* p, uint32_t r)
 {
-    const int64_t v = int64_t(__ldg(reinterpret_cast<const Len*>(p) + r));
+    const int64_t v = int64_t(reinterpret_cast<const Len*>(p)[r]);
     return v < 0 ? 0 : v;
 }
 
@@ -77,9 +77,9 @@ struct Blocks {
         uint8_t ended;
         __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
         {
-            ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
-            length = __ldg(reinterpret_cast<const Len*>(a.lengths) + r);
-            held = __ldg(a.held + r);
+            ended = a.terminated != nullptr ? a.terminated[r] : uint8_t(0);
+            length = reinterpret_cast<const Len*>(a.lengths)[r];
+            held = a.held[r];
         }
     };
     template <class Len>
@@ -121,9 +121,9 @@ struct Tokens {
         uint8_t ended;
         __device__ __forceinline__ void read(const PagedArgs& a, uint32_t r)
         {
-            ended = a.terminated != nullptr ? __ldg(a.terminated + r) : uint8_t(0);
-            fresh = __ldg(reinterpret_cast<const Len*>(a.fresh) + r);
-            start = __ldg(reinterpret_cast<const Len*>(a.start) + r);
+            ended = a.terminated != nullptr ? a.terminated[r] : uint8_t(0);
+            fresh = reinterpret_cast<const Len*>(a.fresh)[r];
+            start = reinterpret_cast<const Len*>(a.start)[r];
         }
     };
     template <class Len>
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
                    warps = gridDim.x * kWarps;
     letNextKernelStart();
     waitForKernelBefore();
-    const uint32_t given = __ldg(a.count);
+    const uint32_t given = *a.count;
     const uint32_t available = uint64_t(given) > uint64_t(a.poolSize) ? 0u : given;
     if (threadIdx.x == 0)
         sShort = 0;
@@ -320,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
             int32_t id[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u)
-                id[u] = j0 + 32u * u < adds ? __ldg(from + j0 + 32u * u) : -1;
+                id[u] = j0 + 32u * u < adds ? from[j0 + 32u * u] : -1;
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 if (j0 + 32u * u < adds) {
@@ -431,7 +431,7 @@ __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
                 if (p < uint64_t(a.room)) {
                     const uint32_t b = a.perBlock(uint32_t(p));
                     within[k] = uint32_t(p) - b * a.perBlock.d;
-                    id[k] = __ldg(a.table + int64_t(r) * a.tableStride + b);
+                    id[k] = a.table[int64_t(r) * a.tableStride + b];
                 }
             }
         }

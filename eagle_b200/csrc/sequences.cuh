@@ -80,6 +80,9 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
 // before it has ended and its writes are visible; the one before lets it start with
 // ``letNextKernelStart``, early, which takes effect when all of its CTAs are running.
 
+// Since what such a kernel reads may be written while it waits, none of it is read through the
+// non-coherent path (__ldg): plain loads, or past L1 (__ldcg).
+
 __device__ __forceinline__ void waitForKernelBefore() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void letNextKernelStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -192,6 +192,25 @@ def test_gradient_sizes(eb, n, rows, dim, kind):
     _check_gradient(eb, grad, torch.from_numpy(_ids(rng, kind, n, rows)).cuda(), rows, dtype=torch.float32)
 
 
+@pytest.mark.parametrize("kind", ("uniform", "skewed", "one"))
+@pytest.mark.parametrize("n,rows", [(512, 70000), (513, 300), (1024, 511), (1025, 262143), (8192, 300),
+                                    (8193, 70000), (65536, 300000), (65537, 5000), (131072, 262144),
+                                    (131073, 700), (131073, 300000), (530000, 70000)])
+def test_gradient_sorts(eb, n, rows, kind):
+    """Every size at which the sort changes its form, of one to three passes."""
+    rng = _gen(19, n, rows)
+    grad = _values(rng, (n, 8), torch.float32).cuda()
+    ids = torch.from_numpy(_ids(rng, kind, n, rows)).cuda()
+    got = _check_gradient(eb, grad, ids, rows)
+    # the runs' order is that of the tokens: a sum of whole numbers of one run's positions is exact
+    place = (torch.arange(n, device="cuda") % 64).float()[:, None].expand(n, 8)
+    want = torch.zeros(rows + 1, dtype=torch.float64, device="cuda")
+    want.index_add_(0, torch.where(ids < 0, rows, ids), place[:, 0].double())
+    if float(want[:rows].max()) < 2**24:
+        assert torch.equal(eb.embedding_grad(place, ids, rows)[:, 3].double(), want[:rows])
+    assert torch.equal(eb.embedding_grad(grad, ids, rows), got)
+
+
 @pytest.mark.parametrize("source", FLOATS)
 @pytest.mark.parametrize("target", FLOATS)
 @pytest.mark.parametrize("accumulate", (False, True))
@@ -673,3 +692,57 @@ def test_a_training_step(eb):
     u = half_step(torch.float32)
     tol = (m + 6) * u / (1 - m * u) * size * float(np.float32(scale))
     assert bool(((total.double() - exact).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("n", (100, 9000, 140000))
+def test_in_the_body_of_a_device_loop(eb, n):
+    """Captured into a WHILE node's body, as the until-done loop runs: three passes, each adding the gradient of
+    one batch, looking up the rows of the next and taking one more block for every request."""
+    import ctypes
+
+    from eagle_b200 import _abi
+    from eagle_b200.graphs import CaptureConditional, Graph, StreamCapturer
+
+    rng = _gen(20, n)
+    rows, dim, requests, passes = 500, 64, 3000, 3
+    table = _values(rng, (rows, dim), torch.float32).cuda()
+    ids = torch.from_numpy(_ids(rng, "skewed", n, rows)).cuda()
+    grad = _values(rng, (n, dim), torch.float32).cuda()
+    total = torch.zeros(rows, dim, device="cuda")
+    cells = torch.tensor([0, passes, 0, 0], dtype=torch.int32, device="cuda")
+    lengths = torch.full((requests,), 5, dtype=torch.int32, device="cuda")
+    held = torch.ones(requests, dtype=torch.int32, device="cuda")
+    tables = torch.zeros(requests, 4, dtype=torch.int32, device="cuda")
+    pool = torch.arange(requests, dtype=torch.int32, device="cuda")
+    count = torch.tensor([requests], dtype=torch.int32, device="cuda")
+    grow = eb.BlockTables(lengths, held, tables, pool, count, block=4)
+    spot = eb.SlotMap(tables, held, held, requests + 7, block=4)
+    look = eb.Embedding(table, ids, scale=2.0)
+    add = eb.EmbeddingGrad(grad, ids, rows, out=total, accumulate=True)
+    want = eb.embedding_grad(grad, ids, rows)
+    origin = torch.cuda.Stream()
+    s = origin.cuda_stream
+    torch.cuda.synchronize()
+    at = cells.data_ptr()
+    loop = CaptureConditional(s, count_ptr=at, baseline_ptr=at + 4, loop_cap=10, counter_ptr=at + 8)
+    cap = StreamCapturer(s)
+    cap.begin()
+    body = loop.begin()
+    on = torch.cuda.ExternalStream(body)
+    for call in (grow, spot, look, add):
+        call(on)
+    d = _abi.new(_abi.CellOpDesc, op=_abi.CELL_BUMP, device=-1, stream=int(body))
+    d.p[0] = at
+    _abi.check(_abi.lib().eagle_backend_cell_op(ctypes.byref(d)))
+    loop.end()
+    launcher = Graph.from_captured(cap.end()).launcher()
+    launcher.stream(s)
+    launcher.launch()
+    launcher.synchronize()
+    assert cells.tolist()[:2] == [passes, passes]
+    assert torch.equal(total, want + want + want)
+    assert torch.equal(look.out, eb.embedding(table, ids, scale=2.0))
+    assert grow.cells.tolist() == [requests, 0] and torch.equal(tables[:, 1], pool)
+    assert spot.offsets[-1].item() == requests
+    # position 1 lies in the first block, whose id is 0
+    assert bool((spot.slots[:requests] == 1).all()) and bool((spot.slots[requests:] == -1).all())
