@@ -412,19 +412,17 @@ __device__ __forceinline__ void zeroUnit(const GradArgs& a, const uint32_t* pres
  *  (item k of lane l is the warp's 32 k + l-th). The lanes of one digit find one another in a
  *  word of shared memory, each setting its own bit: match_any takes about 7 cycles per
  *  different value and warp (200 for random digits) and a ballot per bit 110, this 40.
- *  ``count`` and ``peers`` are [warp][bins] of shared memory; count is left scanned over the
- *  warps, and bin threadIdx.x's sum is returned. */
+ *  ``count`` and ``peers`` are [warp][bins] of shared memory, peers zero and left so; count is
+ *  left scanned over the warps, and bin threadIdx.x's sum is returned. */
 template <int Warps, int Items>
 __device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint32_t shift, uint32_t bits,
     uint32_t (&rank)[Items], uint16_t* count, uint32_t* peers)
 {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, bins = 1u << bits;
-    __syncthreads();  // whoever still reads this memory
+    __syncthreads();  // whoever still reads the counts of the pass before
     uint32_t* words = reinterpret_cast<uint32_t*>(count);
     for (uint32_t i = threadIdx.x; i < Warps * bins / 2; i += Warps * 32)
         words[i] = 0;
-    for (uint32_t i = threadIdx.x; i < Warps * bins; i += Warps * 32)
-        peers[i] = 0;
     __syncthreads();
     uint16_t* mine = count + warp * bins;
     uint32_t* same = peers + warp * bins;
@@ -461,21 +459,28 @@ __device__ __forceinline__ uint32_t rankItems(const uint32_t (&key)[Items], uint
 
 // ---- up to kClusterKeys: one cluster, the keys in its distributed shared memory
 
-constexpr int kClusterThreads = 1024;
+constexpr int kClusterThreads = 512;  // a thread per bin; 1024, half the keys each, took 1.4 times as long
+constexpr int kClusterWarps = kClusterThreads / 32;
 constexpr int kClusterSize = 16;  // past the portable 8: asked for only where more than 8 are needed
-constexpr int kClusterItems = 8;
+constexpr int kClusterItems = 16;
 constexpr uint32_t kClusterKeys = uint32_t(kClusterThreads) * kClusterSize * kClusterItems;  // 131072
 constexpr uint32_t kPortableKeys = kClusterKeys / 2;
-constexpr uint32_t kSmallKeys = 1024;  // up to here in a CTA of 512 threads, which meet at barriers sooner
-constexpr uint32_t peerBytes(int threads) { return uint32_t(threads) / 32u * kMaxBins * 4u; }
+constexpr uint32_t kAloneKeys = 4096;  // sorted by one CTA as fast as by eight, which exchange them
+static_assert(kClusterThreads >= int(kMaxBins), "a thread per bin");
 
-/** Cluster 0 sorts: every CTA holds Threads * Items neighbouring keys in registers; a pass ranks
+/** Shared memory of the sort: the keys by place twice, the ranks' words and counts. */
+constexpr size_t clusterShared(int items)
+{
+    return size_t(kClusterThreads) * items * 16 + size_t(kClusterWarps) * kMaxBins * 6;
+}
+
+/** Cluster 0 sorts: every CTA holds kClusterThreads * Items neighbouring keys in registers; a pass ranks
  *  them, puts them in digit order in the CTA's own shared memory, adds up the CTAs' digit
  *  counts over distributed shared memory and stores each key and position into the CTA that
  *  has its place, neighbours mostly to neighbours; two cluster barriers in all. The other
  *  clusters meanwhile zero the first ``zeroed`` rows. */
-template <class Tok, int Threads, int Items>  // Threads >= kMaxBins: a thread per bin
-__global__ __launch_bounds__(Threads) void clusterSortKernel(GradArgs a)
+template <class Tok, int Items>
+__global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
 {
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ uint32_t tileCount[kMaxBins], base[kMaxBins], scan[33];
@@ -492,36 +497,36 @@ __global__ __launch_bounds__(Threads) void clusterSortKernel(GradArgs a)
             constexpr int64_t kPiece = 65536;
             const int64_t bytes = a.zeroed * a.rowBytes;
             for (int64_t from = at * kPiece; from < bytes; from += others * kPiece)
-                zeroBytes(table + from, table + min(from + kPiece, bytes), threadIdx.x, Threads);
+                zeroBytes(table + from, table + min(from + kPiece, bytes), threadIdx.x, kClusterThreads);
         } else {
-            for (int64_t r = int64_t(at) * (Threads / 32) + (threadIdx.x >> 5); r < a.zeroed;
-                 r += int64_t(others) * (Threads / 32))
+            for (int64_t r = int64_t(at) * kClusterWarps + (threadIdx.x >> 5); r < a.zeroed;
+                 r += int64_t(others) * kClusterWarps)
                 zeroBytes(table + r * a.strideBytes, table + r * a.strideBytes + a.rowBytes, threadIdx.x & 31u, 32u);
         }
         return;
     }
-    constexpr uint32_t kTile = uint32_t(Threads) * Items, kPeers = peerBytes(Threads);
+    constexpr uint32_t kTile = uint32_t(kClusterThreads) * Items;
     uint64_t* at = reinterpret_cast<uint64_t*>(raw);  // key and position by place in the order
     uint64_t* own = at + kTile;                       // by place among the CTA's
-    // the lanes' words take the memory of ``own``, empty while they are in use, if that is enough
-    uint32_t* peers = reinterpret_cast<uint32_t*>(kTile * 8 >= kPeers ? own : own + kTile);
-    uint16_t* count = reinterpret_cast<uint16_t*>(
-        reinterpret_cast<char*>(own) + (kTile * 8 >= kPeers ? kTile * 8 : kTile * 8 + kPeers));
+    uint32_t* peers = reinterpret_cast<uint32_t*>(own + kTile);
+    uint16_t* count = reinterpret_cast<uint16_t*>(peers + kClusterWarps * kMaxBins);
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t item0 = warp * (32u * Items) + lane;
     if (cta == 0 && threadIdx.x < 2)
         a.listCount[threadIdx.x] = 0;
     if (a.present != nullptr)
-        for (int64_t w = int64_t(cta) * Threads + threadIdx.x; w < (a.rows + 31) / 32;
-             w += int64_t(ctas) * Threads)
+        for (int64_t w = int64_t(cta) * kClusterThreads + threadIdx.x; w < (a.rows + 31) / 32;
+             w += int64_t(ctas) * kClusterThreads)
             a.present[w] = 0;
+    for (uint32_t i = threadIdx.x; i < kClusterWarps * kMaxBins; i += kClusterThreads)
+        peers[i] = 0;
     uint32_t key[Items], pos[Items], rank[Items];
     loadKeys<Tok, Items>(a, cta * kTile + item0, 32u, key);
 #pragma unroll
     for (int k = 0; k < Items; ++k)
         pos[k] = cta * kTile + item0 + 32u * k;
     for (uint32_t shift = 0; shift < a.bits; shift += a.digitBits) {
-        const uint32_t mine = rankItems<(Threads / 32), Items>(key, shift, a.digitBits, rank, count, peers);
+        const uint32_t mine = rankItems<kClusterWarps, Items>(key, shift, a.digitBits, rank, count, peers);
         uint32_t all = 0;
         const uint32_t first = blockExclusiveSum(mine, all, scan);
         if (threadIdx.x < a.bins) {
@@ -552,7 +557,7 @@ __global__ __launch_bounds__(Threads) void clusterSortKernel(GradArgs a)
         __syncthreads();
 #pragma unroll
         for (int k = 0; k < Items; ++k) {
-            const uint32_t j = uint32_t(k) * Threads + threadIdx.x;
+            const uint32_t j = uint32_t(k) * kClusterThreads + threadIdx.x;
             const uint64_t v = own[j];
             const uint32_t to = base[(uint32_t(v) >> shift) & (a.bins - 1u)] + j;
             cluster.map_shared_rank(at, to / kTile)[to % kTile] = v;
@@ -658,6 +663,8 @@ __global__ __launch_bounds__(kSortThreads) void passKernel(GradArgs a)
     waitForKernelBefore();
     uint32_t* peers = reinterpret_cast<uint32_t*>(raw);
     uint16_t* count = reinterpret_cast<uint16_t*>(peers + kSortWarps * kMaxBins);
+    for (uint32_t i = threadIdx.x; i < kSortWarps * kMaxBins; i += kSortThreads)
+        peers[i] = 0;
     __shared__ uint32_t base[kMaxBins], scan[33];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t item0 = blockIdx.x * kSortTile + warp * (32u * kSortItems) + lane;
@@ -1385,12 +1392,6 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
     });
 }
 
-size_t clusterShared(int threads, int items)
-{
-    const size_t keys = size_t(threads) * items * 8, peers = peerBytes(threads);
-    return 2 * keys + (keys >= peers ? 0 : peers) + peers / 2;
-}
-
 /** Whether the current device holds a cluster of kClusterSize CTAs of the sort (kept per device). */
 bool largeClusters()
 {
@@ -1402,14 +1403,14 @@ bool largeClusters()
     if (int(known.size()) <= dev)
         known.resize(size_t(dev) + 1, 0);
     if (known[size_t(dev)] == 0) {
-        auto kernel = clusterSortKernel<int32_t, kClusterThreads, kClusterItems>;
+        auto kernel = clusterSortKernel<int32_t, kClusterItems>;
         cudaLaunchAttribute attr{};
         attr.id = cudaLaunchAttributeClusterDimension;
         attr.val.clusterDim = {unsigned(kClusterSize), 1, 1};
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(kClusterSize, 1, 1);
         config.blockDim = dim3(kClusterThreads, 1, 1);
-        config.dynamicSmemBytes = clusterShared(kClusterThreads, kClusterItems);
+        config.dynamicSmemBytes = clusterShared(kClusterItems);
         config.attrs = &attr;
         config.numAttrs = 1;
         int clusters = 0;
@@ -1508,11 +1509,11 @@ void launchBulkSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const cha
     launchBehind(kernel, blocks, kBulkThreads, sizeof(BulkShared), s, a, who);
 }
 
-template <class Tok, int Threads, int Items>
+template <class Tok, int Items>
 void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaStream_t s, const char* who)
 {
-    auto kernel = clusterSortKernel<Tok, Threads, Items>;
-    const size_t shared = clusterShared(Threads, Items);
+    auto kernel = clusterSortKernel<Tok, Items>;
+    const size_t shared = clusterShared(Items);
     cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
     if (ctas > 8)
         cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), who);
@@ -1523,7 +1524,7 @@ void launchClusterSort(const GradArgs& a, unsigned ctas, unsigned blocks, cudaSt
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(blocks, 1, 1);
-    config.blockDim = dim3(Threads, 1, 1);
+    config.blockDim = dim3(kClusterThreads, 1, 1);
     config.dynamicSmemBytes = shared;
     config.stream = s;
     config.attrs = attr;
@@ -1542,7 +1543,7 @@ void launchPass(const GradArgs& a, unsigned tiles, cudaStream_t s, const char* w
 
 /** Bytes of rows that the SMs without part in a cluster's sort zero meanwhile: what they write in
  *  about the sort's time, at 3.3 TB/s (7 us with one key a thread, 14 with two, 31 with eight). */
-constexpr int64_t zeroedBesideSort(unsigned perThread) { return (12ll + 12ll * perThread) << 20; }
+constexpr int64_t zeroedBesideSort(unsigned perThread) { return (18ll + 6ll * perThread) << 20; }
 
 /** And those that the SMs without a join zero: what they write in about 8 us. */
 constexpr int64_t kZeroedBesideJoin = 32ll << 20;
@@ -1609,18 +1610,14 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     if (p.n <= kPortableKeys || (p.n <= kClusterKeys && largeClusters())) {
         a.keyOut = words(p.key[0]);
         a.posOut = words(p.pos[0]);
-        // what one CTA holds needs no exchange; past that, as many as the cluster may have
-        unsigned ctas = 1;
-        if (p.n > uint32_t(kClusterThreads) * kClusterItems)
-            ctas = p.n <= kPortableKeys ? 8u : unsigned(kClusterSize);
-        const unsigned threads = p.n <= kSmallKeys ? 512u : unsigned(kClusterThreads);
-        const unsigned perThread = (p.n + ctas * threads - 1) / (ctas * threads);
-        // the SMs beside the cluster, 1024 threads each, in whole clusters
+        const unsigned ctas = p.n <= kAloneKeys ? 1u : (p.n <= kPortableKeys ? 8u : unsigned(kClusterSize));
+        const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
+        // the SMs beside the cluster, two CTAs each, in whole clusters
         unsigned blocks = ctas;
         if (!accumulate) {
             a.zeroed = std::min(d.rows, zeroedBesideSort(perThread) / a.rowBytes);
-            const int64_t besides = std::min<int64_t>((a.zeroed * a.rowBytes / 65536 + ctas) / ctas,
-                sms * unsigned(kClusterThreads) / threads / ctas - 1);
+            const int64_t besides =
+                std::min<int64_t>((a.zeroed * a.rowBytes / 65536 + ctas) / ctas, 2 * sms / ctas - 1);
             if (besides > 0)
                 blocks += unsigned(besides) * ctas;
             else
@@ -1629,15 +1626,15 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         withIndex(d.token_type, [&](auto tok) {
             using Tok = decltype(tok);
             if (perThread <= 1)
-                launchClusterSort<Tok, 512, 1>(a, ctas, blocks, s, who);
-            else if (threads == 512)
-                launchClusterSort<Tok, 512, 2>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, 1>(a, ctas, blocks, s, who);
             else if (perThread <= 2)
-                launchClusterSort<Tok, kClusterThreads, 2>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, 2>(a, ctas, blocks, s, who);
             else if (perThread <= 4)
-                launchClusterSort<Tok, kClusterThreads, 4>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, 4>(a, ctas, blocks, s, who);
+            else if (perThread <= 8)
+                launchClusterSort<Tok, 8>(a, ctas, blocks, s, who);
             else
-                launchClusterSort<Tok, kClusterThreads, kClusterItems>(a, ctas, blocks, s, who);
+                launchClusterSort<Tok, kClusterItems>(a, ctas, blocks, s, who);
         });
         a.keys = a.keyOut;
         a.order = a.posOut;
