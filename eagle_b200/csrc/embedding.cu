@@ -302,6 +302,7 @@ struct GradArgs {
     int64_t valueBatch, valueSeq, valueDim;
     FastDiv perBatch;  // by seq
     bool flatTokens, flatValues;
+    bool tableAligned;  // every pack of the table's rows lies on its words
     bool accumulate;
     float scale;
     uint32_t n;
@@ -734,7 +735,7 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
     const float (&acc)[N])
 {
     Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
-    if constexpr (P == Piece::Aligned) {
+    if (P == Piece::Aligned || (P == Piece::Shifted && a.tableAligned && col0 + N <= a.dim)) {
         Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + col0);
         Pack<Out, N> p;
         if (a.accumulate)
@@ -751,6 +752,35 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
                 out[col] = fromFloat<Out>(a.accumulate ? toFloat(out[col]) + a.scale * acc[e] : a.scale * acc[e]);
         }
     }
+}
+
+/** A warp's 32 * N neighbouring columns from ``col0`` on, held N to a lane, through shared memory
+ *  (``stage``, as many floats), so that rows that do not lie on words are written by neighbouring
+ *  lanes all the same. The whole warp calls. */
+template <class Out, int N>
+__device__ __forceinline__ void storeStaged(const GradArgs& a, uint32_t row, uint32_t col0, const float (&acc)[N],
+    float* stage)
+{
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        stage[lane * N + e] = acc[e];
+    __syncwarp();
+    Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
+    float was[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const uint32_t col = col0 + 32u * e + lane;
+        was[e] = a.accumulate && col < a.dim ? toFloat(out[col]) : 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const uint32_t col = col0 + 32u * e + lane;
+        const float v = a.scale * stage[32 * e + lane];
+        if (col < a.dim)
+            out[col] = fromFloat<Out>(a.accumulate ? was[e] + v : v);
+    }
+    __syncwarp();
 }
 
 template <Piece P, int N>
@@ -822,7 +852,9 @@ constexpr uint32_t kBulkSlot = kBulkSlab + 16;    // a piece of any alignment, i
 constexpr uint32_t kBulkRows = 4;                 // rows per barrier
 constexpr uint32_t kBulkStages = 4;
 constexpr uint32_t kMaxChunk = 64;
-constexpr int64_t kBulkLeast = 1024;  // bytes of a row
+// bytes of an aligned row from which this is faster than loads into registers (65536 tokens of 512
+// bytes: 67 us against 56; of 800: 74, 72); of one that is not, half of that (520: 91, 104)
+constexpr int64_t kBulkLeast = 1024;
 constexpr uint32_t kBulkWaits = 1u << 22;  // polls before a wait gives up
 
 struct BulkShared {
@@ -936,6 +968,13 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
     }
     const uint32_t col0 = slab0 + threadIdx.x * N;
     const bool active = col0 < a.dim;
+    float* stage = reinterpret_cast<float*>(raw + sizeof(BulkShared)) + (threadIdx.x & ~31u) * N;
+    auto store = [&](uint32_t row, const float (&sum)[N]) {
+        if constexpr (!Aligned)
+            storeStaged<Out, N>(a, row, slab0 + (threadIdx.x & ~31u) * N, sum, stage);
+        else if (active)
+            storeRow<In, Out, P, N>(a, row, col0, 1u, sum);
+    };
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e)
@@ -956,12 +995,10 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
                 break;
             const uint32_t key = s.key[r0 + j * kBulkRows + u];
             if (key != current) {
-                if (active) {
-                    if (partial)
-                        storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
-                    else
-                        storeRow<In, Out, P, N>(a, current, col0, 1u, acc);
-                }
+                if (!partial)
+                    store(current, acc);
+                else if (active)
+                    storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
                 partial = false;
                 current = key;
 #pragma unroll
@@ -988,16 +1025,12 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
         if ((threadIdx.x & 31u) == 0)
             mbarArrive(&s.empty[stage]);
     }
-    if (!active)
-        return;
-    if (partial) {
-        storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
-    } else if (joined) {
-        storePartial<P, N>(a, a.tail, chunk, col0, 1u, acc);
-        if (slab == 0 && threadIdx.x == 0)
+    if (!partial && !joined) {
+        store(current, acc);
+    } else if (active) {
+        storePartial<P, N>(a, partial ? a.head : a.tail, chunk, col0, 1u, acc);
+        if (!partial && slab == 0 && threadIdx.x == 0)
             listRun(a, chunk, current);
-    } else {
-        storeRow<In, Out, P, N>(a, current, col0, 1u, acc);
     }
 }
 
@@ -1505,8 +1538,9 @@ template <class In, class Out, bool Aligned>
 void launchBulkSum(const GradArgs& a, unsigned blocks, cudaStream_t s, const char* who)
 {
     auto kernel = bulkSumKernel<In, Out, Aligned>;
-    cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(sizeof(BulkShared))), who);
-    launchBehind(kernel, blocks, kBulkThreads, sizeof(BulkShared), s, a, who);
+    const size_t shared = sizeof(BulkShared) + (Aligned ? 0 : kBulkLanes * 16 / sizeof(In) * sizeof(float));
+    cudaCheck(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(shared)), who);
+    launchBehind(kernel, blocks, kBulkThreads, shared, s, a, who);
 }
 
 template <class Tok, int Items>
@@ -1588,6 +1622,8 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.perBatch = FastDiv(uint32_t(d.seq));
     a.flatTokens = isFlat(d.batch, d.seq, a.tokenBatch, a.tokenSeq);
     a.flatValues = isFlat(d.batch, d.seq, a.valueBatch, a.valueSeq);
+    const int64_t outWord = std::min(16, 16 / inBytes * outBytes);
+    a.tableAligned = d.table % uint64_t(outWord) == 0 && a.strideBytes % outWord == 0;
     a.accumulate = accumulate;
     a.scale = float(d.scale);
     a.n = p.n;
@@ -1668,7 +1704,8 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         a.order = words(p.pos[(p.passes + 1) & 1]);
     }
     const uint64_t lanes = uint64_t(p.chunks) * p.slices * p.group;
-    const bool bulk = p.piece != Piece::Strided && d.dim * inBytes >= kBulkLeast;
+    const bool bulk = p.piece != Piece::Strided
+        && d.dim * inBytes >= (p.piece == Piece::Aligned ? kBulkLeast : kBulkLeast / 2);
     if (bulk) {
         a.slices = uint32_t((d.dim * inBytes + kBulkSlab - 1) / kBulkSlab);
         a.sumBlocks = gridOf(int64_t(p.chunks) * a.slices, who);
