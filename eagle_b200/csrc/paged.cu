@@ -49,7 +49,6 @@ struct PagedArgs {
     void* positions;
     int32_t* tokenRequests;
     int32_t* offsets;
-    uint32_t pieces; // warps' shares of a row of the table
     uint32_t* upto;  // scratch: the inclusive scan (more than kScanInBlock requests)
 };
 
@@ -264,14 +263,10 @@ __device__ __forceinline__ uint32_t requestFrom(const uint32_t* upto, uint32_t r
 
 // ------------------------------------------------------------------ block tables
 
-/** Of a request's new or returned blocks, what a warp takes, all of them in flight: few where a
- *  request's state is at hand in shared memory, so that more warps share a request. */
-constexpr uint32_t entriesOf(bool inBlock) { return inBlock ? 128u : 256u; }
-
-/** A warp takes a few blocks of one request: those it gets are copied from the pool, and
- *  those a terminated one gives back are cleared. (One search per entry of the pool's front
- *  instead, 100 instructions per 32 entries against 15, took twice as long.) The requests are
- *  spread over the CTAs for what they hold now, too. */
+/** A warp, or several where there are more warps than requests, takes one request's blocks: those
+ *  it gets are copied from the pool, and those a terminated one gives back are cleared. (One
+ *  search per entry of the pool's front instead, 100 instructions per 32 entries against 15,
+ *  took twice as long.) The requests are spread over the CTAs for what they hold now, too. */
 template <class Len, bool InBlock>
 __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 {
@@ -304,40 +299,44 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
         return b;
     };
 
-    constexpr uint32_t kEntries = entriesOf(InBlock);
-    constexpr int kAhead = int(kEntries / 32);
-    const uint64_t tasks = uint64_t(a.requests) * a.pieces;
-    for (uint64_t task = warp; task < tasks; task += warps) {
-        const uint32_t r = a.pieces == 1 ? uint32_t(task) : uint32_t(task / a.pieces);
-        const uint32_t j0 = uint32_t(task - uint64_t(r) * a.pieces) * kEntries + lane;
+    constexpr int kAhead = InBlock ? 4 : 8;
+    constexpr uint32_t kEntries = 32u * kAhead;
+    // ``share`` warps to a request where there are as many
+    const uint32_t share = a.requests == 0 ? 0u : max(1u, warps / a.requests);
+    const uint32_t part = share > 1 ? warp / a.requests : 0u;
+    for (uint32_t r = warp - part * a.requests; r < a.requests && part < share; r += warps) {
         const Blocks b = request(r);
         int32_t* row = a.table + int64_t(r) * a.tableStride;
         if (b.live) {
             const uint32_t adds = b.adds(a), sum = upto[r];
-            if (j0 - lane >= adds || sum > available)
+            if (sum > available)
                 continue;
             const int32_t* from = a.pool + (sum - adds);
-            int32_t id[kAhead];
+            for (uint32_t j = part * kEntries + lane; j < adds; j += share * kEntries) {
+                int32_t id[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-                id[u] = j0 + 32u * u < adds ? from[j0 + 32u * u] : -1;
+                for (int u = 0; u < kAhead; ++u)
+                    id[u] = j + 32u * u < adds ? from[j + 32u * u] : -1;
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (j0 + 32u * u < adds) {
-                    row[b.held + j0 + 32u * u] = id[u];
-                    if (a.used != nullptr && id[u] >= 0 && int64_t(id[u]) < a.usedSize)
-                        a.used[id[u]] = 1;
+                for (int u = 0; u < kAhead; ++u) {
+                    if (j + 32u * u < adds) {
+                        row[b.held + j + 32u * u] = id[u];
+                        if (a.used != nullptr && id[u] >= 0 && int64_t(id[u]) < a.usedSize)
+                            a.used[id[u]] = 1;
+                    }
                 }
             }
-        } else if (a.used != nullptr && j0 - lane < b.held) {
-            int32_t id[kAhead];
+        } else if (a.used != nullptr) {
+            for (uint32_t j = part * kEntries + lane; j < b.held; j += share * kEntries) {
+                int32_t id[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-                id[u] = j0 + 32u * u < b.held ? row[j0 + 32u * u] : -1;
+                for (int u = 0; u < kAhead; ++u)
+                    id[u] = j + 32u * u < b.held ? row[j + 32u * u] : -1;
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u)
-                if (id[u] >= 0 && int64_t(id[u]) < a.usedSize)
-                    a.used[id[u]] = 0;
+                for (int u = 0; u < kAhead; ++u)
+                    if (id[u] >= 0 && int64_t(id[u]) < a.usedSize)
+                        a.used[id[u]] = 0;
+            }
         }
     }
 
@@ -569,11 +568,11 @@ EB_API eagle_backend_status eagle_backend_x_b200_block_tables(eagle_b200_paged_d
         a.blocks = reinterpret_cast<int32_t*>(d.blocks);
         a.cells = reinterpret_cast<uint32_t*>(d.cells);
         const cudaStream_t s = seamStream(d.stream);
-        const int64_t entries = entriesOf(d.requests <= int64_t(kScanInBlock));
-        a.pieces = uint32_t(std::max<int64_t>(1, (d.width + entries - 1) / entries));
+        // a thread per four entries that the call can write, a warp per request at least
+        const int64_t entries = std::min(d.pool_size + (d.used != 0 ? d.used_size : 0), d.requests * d.width);
+        const int64_t threads = std::max(d.requests * 32, entries / 4);
         withLength(d.length_type, [&](auto len) {
             using Len = decltype(len);
-            const int64_t threads = d.requests * a.pieces * 32;  // a warp per request's share
             if (d.requests <= int64_t(kScanInBlock)) {
                 launchBehind(blockTablesKernel<Len, true>, gridFor(threads, 4), kThreads, 0, s, a, who);
             } else {
