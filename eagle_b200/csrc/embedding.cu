@@ -3,21 +3,23 @@
 //   embedding       values[t, :] = round(scale * table[token[t] - first, :])
 //   embedding_grad  table[v, :] = round(scale * sum over {t : token[t] = first + v} of values[t, :])
 //
-// The lookup is a gather of rows: every thread moves 16-byte pieces of the flattened
-// output, several in flight, so it is bound by HBM (by the launch for a few tokens).
+// The lookup is a gather of rows in 16-byte pieces, several in flight per lane: HBM bounds it
+// (65536 rows of 16 KB to bf16: 155 us, 5.6 TB/s of what it has to move, 6.0 of DRAM traffic),
+// or the launch where there are few tokens (64: 3.4 us).
 //
-// The gradient is a scatter-add, done without atomics on the values: the tokens are
-// sorted by id (stable, so equal ids keep token order), the sorted order is cut into
-// chunks of a fixed length, and every run of equal ids inside a chunk is summed in
-// registers by the lanes that own its columns. A run inside one chunk goes straight to
-// its row; one that crosses chunks leaves a 32-bit partial per chunk, joined in
-// chunk order by a second kernel. A row is thus one sum in an order fixed by the sizes
-// alone. Rows without a token are zeroed by CTAs that only store, beside those that sum.
+// The gradient is a scatter-add, done without atomics on the values: the tokens are sorted by
+// id (stable, so equal ids keep token order), the sorted order is cut into chunks of a length
+// that the sizes fix, and every run of equal ids is summed in registers by the lanes that own
+// its columns. A run inside one chunk, or across one boundary, goes straight to its row; a
+// longer one leaves a 32-bit partial per chunk, joined in chunk order by a second kernel. A
+// row is thus one sum in one order. Rows without a token are zeroed by CTAs that only store,
+// beside the sort, the sums and the joins. 131072 tokens of 4096 bf16 into as many rows take
+// 365 us, 5.9 TB/s of what has to move: 32 in the sort, 300 in the sums at 6.0 TB/s of DRAM
+// traffic, 30 in the joins and the zeroing beside them.
 //
-// The sort is least-significant-digit radix over bits(rows) bits, at most 9 a pass. A
-// tile is 4096 keys: each warp ranks its 256 by match_any, a scan over the warps orders
-// the tile. Up to one tile the whole sort is one CTA's, in shared memory. Past it every
-// pass adds up the tiles' digit counts itself (no look-back, no wait on another CTA): the
+// The sort is least-significant-digit radix over bits(rows) bits, at most 9 a pass: up to 131072
+// tokens in one launch, by a CTA or a cluster that keeps the keys in shared memory; past that
+// a kernel a pass, each adding up the tiles' digit counts itself (no wait on another CTA): the
 // first counts come from a kernel of their own, each later pass's are gathered by the pass
 // before, which knows where its keys land.
 #include "sequences.cuh"
@@ -209,9 +211,10 @@ __global__ __launch_bounds__(kLookupThreads) void lookupShiftedKernel(LookupArgs
     }
 }
 
-// Wide rows: a warp takes 32 * Unroll packs of one row, so that the row, its addresses and its
-// alignment are worked out once for all of them (per pack, that took more time than the
-// bytes: 128 us against 210 at 65536 rows of 16 KB, and 8 against 20 at 10007 of 2002 bytes).
+// Wide rows (32 packs and more): a warp takes 32 * Unroll packs of one row, so that the row, its
+// addresses and its alignment are worked out once for all of them. Worked out per pack, as
+// for the narrow ones, that took more time than the bytes: 210 us against 155 at 65536 rows of
+// 16 KB, and 20 against 8 at 10007 of 2002 bytes.
 
 /** 32 bytes in one load (two of 16 bytes each touch every sector twice); ``p`` is 32-byte aligned. */
 __device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi)
@@ -1576,11 +1579,12 @@ void launchPass(const GradArgs& a, unsigned tiles, cudaStream_t s, const char* w
 }
 
 /** Bytes of rows that the SMs without part in a cluster's sort zero meanwhile: what they write in
- *  about the sort's time, at 3.3 TB/s (7 us with one key a thread, 14 with two, 31 with eight). */
+ *  about the sort's time (7 us with one key a thread, 14 with four, 30 with sixteen). */
 constexpr int64_t zeroedBesideSort(unsigned perThread) { return (18ll + 6ll * perThread) << 20; }
 
-/** And those that the SMs without a join zero: what they write in about 8 us. */
-constexpr int64_t kZeroedBesideJoin = 32ll << 20;
+/** And those that are left to the SMs without a join, whose 10 us of dependent reads they cover (131072
+ *  tokens of 8 KB: 370 us with 32 MB, 365 with 144, 377 with all that is left). */
+constexpr int64_t kZeroedBesideJoin = 128ll << 20;
 
 void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
 {
