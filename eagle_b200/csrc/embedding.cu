@@ -545,29 +545,29 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
         if (ctas == 1) {
             __syncthreads();
         } else {
-        cluster.sync();
-        uint32_t before = 0, total = 0;
-        if (threadIdx.x < a.bins) {
+            cluster.sync();
+            uint32_t before = 0, total = 0;
+            if (threadIdx.x < a.bins) {
 #pragma unroll 8
-            for (uint32_t c = 0; c < ctas; ++c) {
-                const uint32_t v = cluster.map_shared_rank(tileCount, c)[threadIdx.x];
-                total += v;
-                before += c < cta ? v : 0u;
+                for (uint32_t c = 0; c < ctas; ++c) {
+                    const uint32_t v = cluster.map_shared_rank(tileCount, c)[threadIdx.x];
+                    total += v;
+                    before += c < cta ? v : 0u;
+                }
             }
-        }
-        const uint32_t lower = blockExclusiveSum(total, all, scan);
-        if (threadIdx.x < a.bins)
-            base[threadIdx.x] = lower + before - first;  // from a place among the CTA's to one in the order
-        __syncthreads();
+            const uint32_t lower = blockExclusiveSum(total, all, scan);
+            if (threadIdx.x < a.bins)
+                base[threadIdx.x] = lower + before - first;  // from a place among the CTA's to one in the order
+            __syncthreads();
 #pragma unroll
-        for (int k = 0; k < Items; ++k) {
-            const uint32_t j = uint32_t(k) * kClusterThreads + threadIdx.x;
-            const uint64_t v = own[j];
-            const uint32_t to = base[(uint32_t(v) >> shift) & (a.bins - 1u)] + j;
-            cluster.map_shared_rank(at, to / kTile)[to % kTile] = v;
-        }
-        cluster.sync();
-        from = at;
+            for (int k = 0; k < Items; ++k) {
+                const uint32_t j = uint32_t(k) * kClusterThreads + threadIdx.x;
+                const uint64_t v = own[j];
+                const uint32_t to = base[(uint32_t(v) >> shift) & (a.bins - 1u)] + j;
+                cluster.map_shared_rank(at, to / kTile)[to % kTile] = v;
+            }
+            cluster.sync();
+            from = at;
         }
 #pragma unroll
         for (int k = 0; k < Items; ++k) {
@@ -732,6 +732,14 @@ constexpr uint32_t kRowsInFlight = 8;
  *  last stride is not 1. */
 enum class Piece { Aligned, Shifted, Strided };
 
+/** A row's value from its sum, and from what is there if that is added to: one rounding in 32 bits
+ *  (written out, so that every path has the same bits) and the one to the row's type. */
+template <class Out>
+__device__ __forceinline__ Out scaled(const GradArgs& a, float sum, Out was)
+{
+    return fromFloat<Out>(a.accumulate ? __fmaf_rn(a.scale, sum, toFloat(was)) : __fmul_rn(a.scale, sum));
+}
+
 /** The columns ``col0``, ``col0 + apart``, ... of a row; ``apart`` is 1 but for Strided pieces. */
 template <class In, class Out, Piece P, int N>
 __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32_t col0, uint32_t apart,
@@ -740,19 +748,19 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
     Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
     if (P == Piece::Aligned || (P == Piece::Shifted && a.tableAligned && col0 + N <= a.dim)) {
         Pack<Out, N>* at = reinterpret_cast<Pack<Out, N>*>(out + col0);
-        Pack<Out, N> p;
+        Pack<Out, N> p{};
         if (a.accumulate)
             p = *at;
 #pragma unroll
         for (int e = 0; e < N; ++e)
-            p.e[e] = fromFloat<Out>(a.accumulate ? toFloat(p.e[e]) + a.scale * acc[e] : a.scale * acc[e]);
+            p.e[e] = scaled<Out>(a, acc[e], p.e[e]);
         *at = p;
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             const uint32_t col = col0 + uint32_t(e) * apart;
             if (col < a.dim)
-                out[col] = fromFloat<Out>(a.accumulate ? toFloat(out[col]) + a.scale * acc[e] : a.scale * acc[e]);
+                out[col] = scaled<Out>(a, acc[e], a.accumulate ? out[col] : Out());
         }
     }
 }
@@ -770,18 +778,17 @@ __device__ __forceinline__ void storeStaged(const GradArgs& a, uint32_t row, uin
         stage[lane * N + e] = acc[e];
     __syncwarp();
     Out* out = reinterpret_cast<Out*>(a.table) + int64_t(row) * a.tableStride;
-    float was[N];
+    Out was[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         const uint32_t col = col0 + 32u * e + lane;
-        was[e] = a.accumulate && col < a.dim ? toFloat(out[col]) : 0.0f;
+        was[e] = a.accumulate && col < a.dim ? out[col] : Out();
     }
 #pragma unroll
     for (int e = 0; e < N; ++e) {
         const uint32_t col = col0 + 32u * e + lane;
-        const float v = a.scale * stage[32 * e + lane];
         if (col < a.dim)
-            out[col] = fromFloat<Out>(a.accumulate ? was[e] + v : v);
+            out[col] = scaled<Out>(a, stage[32 * e + lane], was[e]);
     }
     __syncwarp();
 }
@@ -1218,8 +1225,7 @@ __device__ __forceinline__ void storeJoined(const GradArgs& a, uint32_t row, uin
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (col + e < a.dim)
-            out[col + e] =
-                fromFloat<Out>(a.accumulate ? toFloat(out[col + e]) + a.scale * got[e] : a.scale * got[e]);
+            out[col + e] = scaled<Out>(a, got[e], a.accumulate ? out[col + e] : Out());
 }
 
 /** Rows of up to kWarpParts partials: a warp adds 128 columns of one, in chunk order. Rows of

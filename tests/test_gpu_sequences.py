@@ -285,6 +285,14 @@ def test_gradient_bits_do_not_depend_on_the_run(eb, n, dim):
     shifted = torch.empty(n, dim + 1, device="cuda")[:, 1:]
     shifted.copy_(grad)
     assert torch.equal(eb.embedding_grad(shifted, ids, rows), want)
+    # rows on words, off them, and values apart from one another: the same sums, added the same way
+    base = _values(rng, (rows, dim), torch.float32).cuda()
+    strided = torch.empty(dim, n, device="cuda").t()
+    strided.copy_(grad)
+    added = [eb.embedding_grad(g, ids, rows, out=o, scale=0.3, accumulate=True)
+             for g in (grad, shifted, strided) for o in (base.clone(), torch.cat((base[:, :1], base), 1)[:, 1:])]
+    assert all(torch.equal(added[0], other) for other in added[1:])
+    assert torch.equal(eb.embedding_grad(strided, ids, rows), want)
     call = eb.EmbeddingGrad(grad, ids, rows)
     side = torch.cuda.Stream()
     busy = torch.randn(4096, 4096, device="cuda")
