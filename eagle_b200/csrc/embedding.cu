@@ -469,6 +469,7 @@ constexpr int kClusterSize = 16;  // past the portable 8: asked for only where m
 constexpr int kClusterItems = 16;
 constexpr uint32_t kClusterKeys = uint32_t(kClusterThreads) * kClusterSize * kClusterItems;  // 131072
 constexpr uint32_t kPortableKeys = kClusterKeys / 2;
+constexpr uint32_t kFewKeys = 8192;    // from here on 16 CTAs, where the device has such clusters, beat 8
 constexpr uint32_t kAloneKeys = 4096;  // sorted by one CTA as fast as by eight, which exchange them
 static_assert(kClusterThreads >= int(kMaxBins), "a thread per bin");
 
@@ -1656,7 +1657,9 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     if (p.n <= kPortableKeys || (p.n <= kClusterKeys && largeClusters())) {
         a.keyOut = words(p.key[0]);
         a.posOut = words(p.pos[0]);
-        const unsigned ctas = p.n <= kAloneKeys ? 1u : (p.n <= kPortableKeys ? 8u : unsigned(kClusterSize));
+        unsigned ctas = 1;
+        if (p.n > kAloneKeys)
+            ctas = p.n <= kFewKeys || !largeClusters() ? 8u : unsigned(kClusterSize);
         const unsigned perThread = (p.n + ctas * unsigned(kClusterThreads) - 1) / (ctas * unsigned(kClusterThreads));
         // the SMs beside the cluster, two CTAs each, in whole clusters
         unsigned blocks = ctas;
