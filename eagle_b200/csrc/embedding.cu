@@ -343,6 +343,7 @@ struct GradArgs {
     int64_t zeroed;       // rows [0, zeroed) are zeroed, with tokens or without, beside the sort
     int64_t zeroedBefore; // rows up to this are zeroed before the joins, the others beside them
     uint32_t joinBlocks;  // CTAs that join; the others zero
+    uint32_t joinLanes;   // lanes that hold a row's columns, or 128 of them, four each
 };
 
 /** The keys of Items tokens, ``step`` apart from ``from`` on (kNoKey past the last). No branch
@@ -1230,14 +1231,14 @@ __device__ __forceinline__ void storeJoined(const GradArgs& a, uint32_t row, uin
 }
 
 /** Rows of up to kWarpParts partials: a warp adds 128 columns of one, in chunk order. Rows of
- *  more: the eight warps of a CTA add an eighth of its partials each, in chunk order, then the
- *  eight sums in order. (A frequent id of ordinary text has tens of partials and there are a
+ *  more: a CTA's eight warps (of narrow rows up to 64 groups of lanes) add an eighth (a 64th) of
+ *  its partials each, in chunk order, then those sums in order. (A frequent id of ordinary text has tens of partials and there are a
  *  few hundred of them: a CTA each, all columns in turn, took twice as long. A batch of one id
  *  has thousands.) */
 template <class Out>
-__global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
+__global__ __launch_bounds__(kJoinThreads, 6) void joinKernel(GradArgs a)  // six an SM, for the zeroing ones
 {
-    __shared__ float4 part[kJoinWarps][32];
+    __shared__ float4 part[kJoinThreads];
     letNextKernelStart();
     waitForKernelBefore();
     if (blockIdx.x >= a.joinBlocks) {
@@ -1246,10 +1247,12 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
     }
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     const uint32_t blocks = (a.dim + kJoinColumns - 1) / kJoinColumns;
+    // a long run's columns by groups of joinLanes lanes, its partials by the groups
+    const uint32_t group = threadIdx.x / a.joinLanes, groups = kJoinThreads / a.joinLanes, at = threadIdx.x % a.joinLanes;
     const uint64_t longItems = uint64_t(a.listCount[1]) * blocks, items = uint64_t(a.listCount[0]) * blocks;
     for (uint64_t item = blockIdx.x; item < longItems; item += a.joinBlocks) {
         const uint32_t chunk = a.longList[item / blocks];
-        const uint32_t col = uint32_t(item % blocks) * kJoinColumns + lane * 4u;
+        const uint32_t col = uint32_t(item % blocks) * kJoinColumns + at * 4u;
         const uint32_t key = a.keys[(chunk + 1u) * a.chunk];
         uint32_t m = 1;  // chunks after this one that the run reaches: the keys are sorted, so they are counted
         for (uint32_t more = 4 * kJoinThreads; more == 4 * kJoinThreads;) {
@@ -1265,18 +1268,18 @@ __global__ __launch_bounds__(kJoinThreads) void joinKernel(GradArgs a)
                 more += uint32_t(__syncthreads_count(in[u]));
             m += more;
         }
-        const uint32_t parts = m + 1u, each = (parts + kJoinWarps - 1) / kJoinWarps;
-        const uint32_t p0 = warp * each, p1 = min(p0 + each, parts);
+        const uint32_t parts = m + 1u, each = (parts + groups - 1) / groups;
+        const uint32_t p0 = group * each, p1 = min(p0 + each, parts);
         if (col < a.width && p0 < p1)
-            part[warp][lane] = addPartials<16>(a, chunk, p0, p1, col);
+            part[threadIdx.x] = addPartials<16>(a, chunk, p0, p1, col);
         else
-            part[warp][lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            part[threadIdx.x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         __syncthreads();
-        if (warp == 0 && col < a.dim) {
-            float4 sum = part[0][lane];
-#pragma unroll
-            for (int w = 1; w < kJoinWarps; ++w) {
-                const float4 v = part[w][lane];
+        if (group == 0 && col < a.dim) {
+            float4 sum = part[at];
+#pragma unroll 8
+            for (uint32_t g = 1; g < groups; ++g) {
+                const float4 v = part[g * a.joinLanes + at];
                 sum.x += v.x;
                 sum.y += v.y;
                 sum.z += v.z;
@@ -1505,9 +1508,12 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     p.slices = (p.pieces + p.group - 1) / p.group;
     // the longest chunk that still leaves enough warps of 256 columns to hide the row loads: a
     // longer one leaves fewer partials of long runs. Of the sizes alone, not of types or
-    // alignment: it fixes the order of the sums, and the scratch the query asks for
+    // alignment: it fixes the order of the sums, and the scratch the query asks for. (Wanting
+    // 2048 warps for wide rows too, 65536 tokens of 512 take 64 us instead of 59; wanting 4096
+    // for narrow ones, 65536 of 128 take 42 instead of 38.)
+    const uint64_t wanted = d.dim >= 512 ? 4096 : 2048;
     p.chunk = 8;
-    while (p.chunk < 64 && uint64_t(p.n) * ((uint64_t(d.dim) + 255) / 256) / (p.chunk * 2) >= 4096)
+    while (p.chunk < 64 && uint64_t(p.n) * ((uint64_t(d.dim) + 7) / 8) / 32 / (p.chunk * 2) >= wanted)
         p.chunk *= 2;
     p.chunks = (p.n + p.chunk - 1) / p.chunk;
     p.width = uint32_t(roundUp(uint64_t(d.dim), 8));
@@ -1748,6 +1754,9 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     });
     if (p.chunks > 1) {
         const int64_t items = int64_t(p.chunks / 2) * ((d.dim + kJoinColumns - 1) / kJoinColumns);
+        a.joinLanes = 4;
+        while (a.joinLanes < 32 && a.joinLanes * 4 < a.dim)
+            a.joinLanes *= 2;
         a.joinBlocks = unsigned(std::min<int64_t>(items, sms * 8));
         const unsigned all = gridOf(a.joinBlocks + (a.present == nullptr ? 0 : unitsOf(d.rows - a.zeroedBefore)), who);
         withElement(d.table_type,

@@ -60,7 +60,7 @@ def _check_lookup(eb, table, tokens, *, scale=1.0, first=0, out=None, dtype=None
     return got
 
 
-@pytest.mark.parametrize("dim", (1, 2, 8, 33, 64, 777, 1024, 4100))
+@pytest.mark.parametrize("dim", (1, 2, 8, 33, 64, 255, 256, 257, 777, 1024, 4100, 20003))
 @pytest.mark.parametrize("n", (1, 31, 1000))
 def test_lookup_sizes(eb, n, dim):
     rng = _gen(1, n, dim)
@@ -185,7 +185,8 @@ def _ids(rng, kind, n, rows):
 @pytest.mark.parametrize("kind", ("uniform", "skewed", "one", "none", "falling"))
 @pytest.mark.parametrize("n,rows,dim", [(0, 5, 8), (1, 1, 1), (1, 300, 64), (7, 3, 24), (65, 2, 520), (301, 8209, 40),
                                         (4096, 511, 72), (4096, 512, 33), (4097, 513, 64), (9000, 40009, 777),
-                                        (20000, 1000, 128), (5000, 300000, 16)])
+                                        (20000, 1000, 128), (5000, 300000, 16), (60, 9, 20000), (60, 9, 20003),
+                                        (3000, 40, 2052)])
 def test_gradient_sizes(eb, n, rows, dim, kind):
     rng = _gen(6, n, rows, dim)
     grad = _values(rng, (n, dim), torch.bfloat16).cuda()
