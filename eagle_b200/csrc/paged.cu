@@ -486,15 +486,6 @@ PagedArgs pagedArgs(const eagle_b200_paged_desc& d, const char* who)
 
 int64_t pagedScratch(const eagle_b200_paged_desc& d) { return d.requests > int64_t(kScanInBlock) ? d.requests * 4 : 16; }
 
-template <class F>
-void withLength(uint32_t type, F&& f)
-{
-    if (type == EAGLE_B200_TYPE_I32)
-        f(int32_t{});
-    else
-        f(int64_t{});
-}
-
 template <class What, class Len>
 void launchScan(const PagedArgs& a, cudaStream_t s, const char* who)
 {
@@ -571,7 +562,7 @@ EB_API eagle_backend_status eagle_backend_x_b200_block_tables(eagle_b200_paged_d
         // a thread per four entries that the call can write, a warp per request at least
         const int64_t entries = std::min(d.pool_size + (d.used != 0 ? d.used_size : 0), d.requests * d.width);
         const int64_t threads = std::max(d.requests * 32, entries / 4);
-        withLength(d.length_type, [&](auto len) {
+        withIndex(d.length_type, [&](auto len) {
             using Len = decltype(len);
             if (d.requests <= int64_t(kScanInBlock)) {
                 launchBehind(blockTablesKernel<Len, true>, gridFor(threads, 4), kThreads, 0, s, a, who);
@@ -622,8 +613,8 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
         a.tokenRequests = reinterpret_cast<int32_t*>(d.token_requests);
         a.offsets = reinterpret_cast<int32_t*>(d.offsets);
         const cudaStream_t s = seamStream(d.stream);
-        withLength(d.length_type, [&](auto len) {
-            withLength(d.slot_type, [&](auto slot) {
+        withIndex(d.length_type, [&](auto len) {
+            withIndex(d.slot_type, [&](auto slot) {
                 using Len = decltype(len);
                 using Slot = decltype(slot);
                 if (d.capacity <= int64_t(smCount()) * kThreads)

@@ -72,6 +72,38 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
     T e[N];
 };
 
+/** The 16 bytes ``skip`` into 32 neighbouring ones. */
+__device__ __forceinline__ uint4 shiftWords(uint4 lo, uint4 hi, uint32_t skip)
+{
+    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    if (skip & 8u) {
+#pragma unroll
+        for (int j = 0; j < 6; ++j)
+            w[j] = w[j + 2];
+    }
+    if (skip & 4u) {
+#pragma unroll
+        for (int j = 0; j < 5; ++j)
+            w[j] = w[j + 1];
+    }
+    const uint32_t shift = (skip & 3u) * 8u;
+    return make_uint4(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift),
+        __funnelshift_r(w[2], w[3], shift), __funnelshift_r(w[3], w[4], shift));
+}
+
+/** 16 bytes from any address of whole elements, of which ``valid`` bytes are wanted: the one or
+ *  two aligned words that hold them (each holds a wanted byte, so it lies in mapped memory),
+ *  shifted together. What lies past ``valid`` is unspecified. */
+__device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
+{
+    const uint64_t at = reinterpret_cast<uint64_t>(p);
+    const uint4* word = reinterpret_cast<const uint4*>(at & ~uint64_t(15));
+    const uint32_t skip = uint32_t(at) & 15u;
+    const uint4 lo = *word;
+    const uint4 hi = skip + valid > 16u ? word[1] : make_uint4(0u, 0u, 0u, 0u);
+    return shiftWords(lo, hi, skip);
+}
+
 // ------------------------------------------------------------- kernels in a row
 //
 // A call of several kernels launches each but the first while the one before it still runs
@@ -139,6 +171,48 @@ inline unsigned gridOf(int64_t want, const char* who)
     if (want > 0x7fffffffll)
         unsupported(std::string(who) + ": the call is larger than one launch holds");
     return unsigned(want);
+}
+
+/** What the embedding's entries refuse. */
+inline void checkEmbedding(const eagle_b200_embedding_desc& d, const char* who)
+{
+    const std::string w(who);
+    (void)elementBytes(d.table_type, who);
+    (void)elementBytes(d.values_type, who);
+    (void)indexBytes(d.token_type, who);
+    if (d.rows < 0 || d.rows > 0x7ffffffell)
+        invalid(w + ": rows must lie in [0, 2^31 - 2]");
+    if (d.dim < 0 || d.dim > (1ll << 24))
+        invalid(w + ": dim must lie in [0, 2^24]");
+    if (d.first < 0)
+        invalid(w + ": first must not be negative");
+    if (d.batch < 0 || d.seq < 0 || d.batch > 0x7fffffffll || d.seq > 0x7fffffffll || d.batch * d.seq > 0x7fffffffll)
+        invalid(w + ": batch * seq must lie in [0, 2^31 - 1]");
+    if (d.rows > 1 && d.table_stride < d.dim)
+        invalid(w + ": the table's rows overlap (table_stride below dim)");
+}
+
+/** One stride serves both token axes. */
+inline bool isFlat(int64_t batch, int64_t seq, int64_t outer, int64_t inner) { return batch <= 1 || outer == seq * inner; }
+
+template <class F>
+void withElement(uint32_t type, F&& f)
+{
+    if (type == EAGLE_B200_TYPE_F32)
+        f(float{});
+    else if (type == EAGLE_B200_TYPE_BF16)
+        f(__nv_bfloat16{});
+    else
+        f(__half{});
+}
+
+template <class F>
+void withIndex(uint32_t type, F&& f)
+{
+    if (type == EAGLE_B200_TYPE_I32)
+        f(int32_t{});
+    else
+        f(int64_t{});
 }
 
 }  // namespace eb
