@@ -95,7 +95,7 @@ __global__ __launch_bounds__(kLookupThreads) void lookupKernel(LookupArgs a)
 #pragma unroll
         for (int e = 0; e < N; ++e)
             out.e[e] = fromFloat<Out>(from[u] >= 0 ? toFloat(got[u].e[e]) * a.scale : 0.0f);
-        *reinterpret_cast<Pack<Out, N>*>(values + to[u]) = out;
+        storePack(values + to[u], out);
     }
 }
 
@@ -161,16 +161,8 @@ __global__ __launch_bounds__(kLookupThreads) void lookupShiftedKernel(LookupArgs
 // for the narrow ones, that took more time than the bytes: 210 us against 155 at 65536 rows of
 // 16 KB, and 20 against 8 at 10007 of 2002 bytes.
 
-/** 32 bytes in one load (two of 16 bytes each touch every sector twice); ``p`` is 32-byte aligned. */
-__device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi)
-{
-    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
-                 : "l"(p));
-}
-
-/** ``Shifted``: packs are cut where the output's 16-byte words begin and read from wherever that
- *  falls in the table; the up to N - 1 values before the first and after the last are taken
+/** ``Shifted``: packs are cut where the output's words (of 16 bytes, or 32 if the table's type is the
+ *  narrower) begin and read from wherever that falls in the table; the up to N - 1 values before the first and after the last are taken
  *  one to a lane. */
 template <class In, class Out, class Tok, int N, int Unroll, bool Shifted>
 __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
@@ -189,7 +181,9 @@ __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
     Out* to = reinterpret_cast<Out*>(a.values) + at;
     uint32_t lead = 0;
     if constexpr (Shifted)
-        lead = min(((0u - uint32_t(reinterpret_cast<uint64_t>(to))) & 15u) / uint32_t(sizeof(Out)), a.dim);
+        lead = min(((0u - uint32_t(reinterpret_cast<uint64_t>(to))) & (N * uint32_t(sizeof(Out)) - 1u))
+                / uint32_t(sizeof(Out)),
+            a.dim);
     const uint32_t whole = (a.dim - lead) / N;
     const uint32_t pack0 = segment * (32u * Unroll) + lane;
     constexpr int kWords = N * int(sizeof(In)) / 16;
@@ -219,10 +213,11 @@ __global__ __launch_bounds__(kLookupThreads) void lookupWideKernel(LookupArgs a)
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 out.e[e] = fromFloat<Out>(row >= 0 ? toFloat(in.e[e]) * a.scale : 0.0f);
-            uint4* words = reinterpret_cast<uint4*>(to + lead + (pack0 + 32u * u) * N);
-#pragma unroll
-            for (int w = 0; w < int(sizeof(out)) / 16; ++w)
-                __stcs(words + w, reinterpret_cast<const uint4*>(&out)[w]);  // L2 is for the table's rows
+            Out* p = to + lead + (pack0 + 32u * u) * N;
+            if constexpr (sizeof(out) == 16)
+                __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&out));  // L2 is for the rows
+            else
+                storePack(p, out);
         }
     }
     if constexpr (Shifted) {
@@ -305,10 +300,10 @@ void enqueueLookup(const eagle_b200_embedding_desc& d, const char* who)
                 using Tok = decltype(tok);
                 // a pack is 16 bytes of the narrower type; every row has to start on its words
                 constexpr int N = 16 / int(sizeof(In) < sizeof(Out) ? sizeof(In) : sizeof(Out));
-                constexpr int64_t kInPack = N * int(sizeof(In));
-                const bool wide = d.dim % N == 0 && d.table % kInPack == 0 && d.values % 16 == 0
-                    && d.table_stride * inBytes % kInPack == 0 && d.value_strides[0] * outBytes % 16 == 0
-                    && d.value_strides[1] * outBytes % 16 == 0;
+                constexpr int64_t kInPack = N * int(sizeof(In)), kOutPack = N * int(sizeof(Out));
+                const bool wide = d.dim % N == 0 && d.table % kInPack == 0 && d.values % kOutPack == 0
+                    && d.table_stride * inBytes % kInPack == 0 && d.value_strides[0] * outBytes % kOutPack == 0
+                    && d.value_strides[1] * outBytes % kOutPack == 0;
                 if (wide)
                     launchLookup<In, Out, Tok, N, false>(a, s, who);
                 else

@@ -499,7 +499,7 @@ __device__ __forceinline__ void storeRow(const GradArgs& a, uint32_t row, uint32
 #pragma unroll
         for (int e = 0; e < N; ++e)
             p.e[e] = scaled<Out>(a, acc[e], p.e[e]);
-        *at = p;
+        storePack(out + col0, p);
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -544,10 +544,11 @@ __device__ __forceinline__ void storePartial(const GradArgs& a, float* to, uint3
 {
     float* row = to + size_t(chunk) * a.width;
     if constexpr (P != Piece::Strided) {
+        Pack<float, N> p;
 #pragma unroll
-        for (int e = 0; e < N; e += 4)
-            *reinterpret_cast<float4*>(row + col0 + e) =
-                make_float4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+        for (int e = 0; e < N; ++e)
+            p.e[e] = acc[e];
+        storePack(row + col0, p);
     } else {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
@@ -1110,7 +1111,7 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
     p.tiles = (p.n + kSortTile - 1) / kSortTile;
     // whole 16-byte words if every vector and every row of the table starts on them
     const int pack = 16 / inBytes;
-    const int64_t outWord = std::min(16, pack * outBytes);
+    const int64_t outWord = pack * outBytes;
     if (d.value_strides[2] == 1 || d.dim <= 1)
         p.piece = d.dim % pack == 0 && d.values % 16 == 0 && d.table % uint64_t(outWord) == 0
                 && d.value_strides[0] * inBytes % 16 == 0 && d.value_strides[1] * inBytes % 16 == 0
@@ -1256,7 +1257,7 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.perBatch = FastDiv(uint32_t(d.seq));
     a.flatTokens = isFlat(d.batch, d.seq, a.tokenBatch, a.tokenSeq);
     a.flatValues = isFlat(d.batch, d.seq, a.valueBatch, a.valueSeq);
-    const int64_t outWord = std::min(16, 16 / inBytes * outBytes);
+    const int64_t outWord = 16 / inBytes * outBytes;
     a.tableAligned = d.table % uint64_t(outWord) == 0 && a.strideBytes % outWord == 0;
     a.accumulate = accumulate;
     a.scale = float(d.scale);

@@ -72,6 +72,28 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
     T e[N];
 };
 
+/** 32 bytes in one load; ``p`` is 32-byte aligned. (Two of 16 touch every sector of a warp's twice.) */
+__device__ __forceinline__ void load32(const void* p, uint4& lo, uint4& hi)
+{
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
+                 : "l"(p));
+}
+
+/** A pack of 8, 16 or 32 bytes in one store to an address aligned to as much. */
+template <class T, int N>
+__device__ __forceinline__ void storePack(T* to, const Pack<T, N>& p)
+{
+    if constexpr (sizeof(p) == 32) {
+        const uint4* w = reinterpret_cast<const uint4*>(&p);
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0].x), "r"(w[0].y),
+                     "r"(w[0].z), "r"(w[0].w), "r"(w[1].x), "r"(w[1].y), "r"(w[1].z), "r"(w[1].w)
+                     : "memory");
+    } else {
+        *reinterpret_cast<Pack<T, N>*>(to) = p;
+    }
+}
+
 /** The 16 bytes ``skip`` into 32 neighbouring ones. */
 __device__ __forceinline__ uint4 shiftWords(uint4 lo, uint4 hi, uint32_t skip)
 {

@@ -105,6 +105,12 @@ def test_lookup_strides(eb):
     _check_lookup(eb, wide[:, 8:72], ids, out=out)
     room[:, 2:36, 8:72] = 7.0
     assert bool((room == 7.0).all())
+    # wider outputs at every 4 bytes of a 32-byte word
+    for shift in range(8):
+        room = torch.full((12, 34, 272), 7.0, device="cuda")
+        _check_lookup(eb, _values(_gen(4, shift), (200, 264), torch.float16).cuda(), ids,
+                      out=room[..., shift:shift + 264])
+        assert bool((room[..., :shift] == 7.0).all()) and bool((room[..., shift + 264:] == 7.0).all())
     # the token axes the other way round
     swapped = torch.empty(34, 12, 64, dtype=torch.float16, device="cuda").transpose(0, 1)
     _check_lookup(eb, wide[:, 8:72], ids, out=swapped)
@@ -242,7 +248,7 @@ def test_gradient_strides(eb, n):
     _check_gradient(eb, grad, ids.t().contiguous().t(), rows)
     _check_gradient(eb, grad.reshape(2, 3, n // 6, dim), ids.view(2, 3, n // 6), rows)
     # a table's gradient inside a larger plane; what lies around it stays
-    for columns in (slice(8, 72), slice(3, 67)):
+    for columns in (slice(8, 72), slice(3, 67), slice(4, 68)):
         room = torch.full((rows + 2, 80), 5.0, device="cuda")
         _check_gradient(eb, grad, ids, rows, out=room[1:-1, columns])
         room[1:-1, columns] = 5.0
