@@ -1216,6 +1216,7 @@ constexpr int64_t zeroedBesideSort(unsigned perThread) { return (18ll + 6ll * pe
 /** And those that are left to the SMs without a join, whose 10 us of dependent reads they cover (131072
  *  tokens of 8 KB: 370 us with 32 MB, 365 with 144, 377 with all that is left). */
 constexpr int64_t kZeroedBesideJoin = 128ll << 20;
+constexpr int64_t kZeroedBesideSums = 24ll << 20;  // but the sums, of 5 us at least, have some first
 
 void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
 {
@@ -1350,8 +1351,10 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         a.sumBlocks = gridOf(int64_t((lanes + kSumThreads - 1) / kSumThreads), who);
     }
     a.zeroedBefore = d.rows;
-    if (a.present != nullptr && p.chunks > 1)
-        a.zeroedBefore = std::max(a.zeroed, d.rows - kZeroedBesideJoin / a.rowBytes);
+    if (a.present != nullptr && p.chunks > 1) {
+        const int64_t left = (d.rows - a.zeroed) * a.rowBytes;
+        a.zeroedBefore -= std::min(kZeroedBesideJoin, std::max(left / 2, left - kZeroedBesideSums)) / a.rowBytes;
+    }
     const int64_t zeroing = a.present == nullptr ? 0 : unitsOf(a.zeroedBefore - a.zeroed);
     const unsigned blocks = gridOf(int64_t(a.sumBlocks) + zeroing, who);
     withElement(d.values_type, [&](auto in) {
