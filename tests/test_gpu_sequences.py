@@ -218,6 +218,29 @@ def test_gradient_sorts(eb, n, rows, kind):
     assert torch.equal(eb.embedding_grad(grad, ids, rows), got)
 
 
+@pytest.mark.parametrize("dim", (4, 60, 520, 521))
+@pytest.mark.parametrize("longest", (3, 40, 130, 2600))
+def test_gradient_runs(eb, dim, longest):
+    """Runs of every length around the chunks', beginning and ending everywhere in them; whole numbers, so that
+    any order of the sums is exact and a row lost, doubled or split shows."""
+    for seed in range(6):
+        rng = _gen(21, dim, longest, seed)
+        lengths = rng.integers(0, longest + 1, 40) if seed % 2 else \
+            rng.choice([n for n in (0, 1, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 256, 257, 2048,
+                                    2111) if n <= longest], 60)
+        rows = len(lengths)
+        ids = np.repeat(np.arange(rows), lengths)
+        ids = np.concatenate((ids, np.full(rng.integers(0, 30), rows)))  # and some without a row
+        ids = torch.from_numpy(rng.permutation(ids)).cuda()
+        grad = torch.from_numpy(rng.integers(-8, 9, (ids.numel(), dim)).astype(np.float32)).cuda()
+        want = torch.zeros(rows + 1, dim, dtype=torch.float64, device="cuda").index_add_(0, ids, grad.double())[:rows]
+        assert torch.equal(eb.embedding_grad(grad, ids, rows).double(), want)
+        assert torch.equal(eb.embedding_grad(grad.bfloat16(), ids, rows, dtype=torch.float32).double(), want)
+        out = torch.ones(rows, dim, device="cuda")
+        eb.embedding_grad(grad.half(), ids, rows, scale=2.0, out=out, accumulate=True)
+        assert torch.equal(out.double(), 1 + 2 * want)
+
+
 @pytest.mark.parametrize("source", FLOATS)
 @pytest.mark.parametrize("target", FLOATS)
 @pytest.mark.parametrize("accumulate", (False, True))
@@ -709,10 +732,11 @@ def test_a_training_step(eb):
     assert bool(((total.double() - exact).abs() <= tol).all())
 
 
-@pytest.mark.parametrize("n", (100, 9000, 140000))
+@pytest.mark.parametrize("n", (500, 9000, 140000))
 def test_in_the_body_of_a_device_loop(eb, n):
     """Captured into a WHILE node's body, as the until-done loop runs: three passes, each adding the gradient of
-    one batch, looking up the rows of the next and taking one more block for every request."""
+    one batch, looking up the rows of the next and taking one more block for every request; calls right before
+    the loop, as the first and last of its body, and right after a loop and a memset."""
     import ctypes
 
     from eagle_b200 import _abi
@@ -735,6 +759,7 @@ def test_in_the_body_of_a_device_loop(eb, n):
     look = eb.Embedding(table, ids, scale=2.0)
     add = eb.EmbeddingGrad(grad, ids, rows, out=total, accumulate=True)
     want = eb.embedding_grad(grad, ids, rows)
+    first, after, last = eb.Embedding(table, ids), eb.EmbeddingGrad(total, ids[:rows], rows), eb.Embedding(table, ids)
     origin = torch.cuda.Stream()
     s = origin.cuda_stream
     torch.cuda.synchronize()
@@ -742,14 +767,19 @@ def test_in_the_body_of_a_device_loop(eb, n):
     loop = CaptureConditional(s, count_ptr=at, baseline_ptr=at + 4, loop_cap=10, counter_ptr=at + 8)
     cap = StreamCapturer(s)
     cap.begin()
+    first(origin)
     body = loop.begin()
     on = torch.cuda.ExternalStream(body)
-    for call in (grow, spot, look, add):
+    for call in (grow, spot, look):
         call(on)
     d = _abi.new(_abi.CellOpDesc, op=_abi.CELL_BUMP, device=-1, stream=int(body))
     d.p[0] = at
     _abi.check(_abi.lib().eagle_backend_cell_op(ctypes.byref(d)))
+    add(on)
     loop.end()
+    after(origin)
+    _abi.check(_abi.lib().eagle_backend_memset_device(at + 12, 4, s))
+    last(origin)
     launcher = Graph.from_captured(cap.end()).launcher()
     launcher.stream(s)
     launcher.launch()
@@ -757,6 +787,8 @@ def test_in_the_body_of_a_device_loop(eb, n):
     assert cells.tolist()[:2] == [passes, passes]
     assert torch.equal(total, want + want + want)
     assert torch.equal(look.out, eb.embedding(table, ids, scale=2.0))
+    assert torch.equal(first.out, eb.embedding(table, ids)) and torch.equal(last.out, first.out)
+    assert torch.equal(after.out, eb.embedding_grad(total, ids[:rows], rows))
     assert grow.cells.tolist() == [requests, 0] and torch.equal(tables[:, 1], pool)
     assert spot.offsets[-1].item() == requests
     # position 1 lies in the first block, whose id is 0
