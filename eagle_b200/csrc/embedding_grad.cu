@@ -130,9 +130,10 @@ __device__ __forceinline__ void zeroBytes(char* from, char* to, uint32_t at, uin
 }
 
 /** Zero unit ``unit`` of the rows [row0, row1), of those whose bit in ``present`` is clear
- *  (all if it is null): a unit is ``zeroRows`` rows or, of longer ones, a piece of kZeroUnit bytes. CTAs that
- *  take neighbouring units one after the other write at 7 TB/s; a grid that strides over a
- *  large plane, each warp a row, at 4. */
+ *  (all if it is null): a unit is ``zeroRows`` rows or, of longer ones, a piece of kZeroUnit
+ *  bytes. CTAs that take neighbouring units one after the other write at 7.4 TB/s; a grid of as
+ *  many CTAs as fit, striding over the plane, at 6.2, and beside the sums, a row a warp, at less:
+ *  there the same work took 410 us instead of 312. */
 __device__ __forceinline__ void zeroUnit(const GradArgs& a, const uint32_t* present, int64_t row0, int64_t row1,
     uint64_t unit)
 {
