@@ -331,6 +331,7 @@ SIGNATURES = {
     "eagle_backend_x_b200_compact_sum": (_i32, [ctypes.POINTER(CompactDesc), _u64, _u64, _u32]),
     "eagle_backend_x_b200_embedding": (_i32, [ctypes.POINTER(EmbeddingDesc)]),
     "eagle_backend_x_b200_embedding_grad": (_i32, [ctypes.POINTER(EmbeddingDesc)]),
+    "eagle_backend_x_b200_embedding_grad_wait_check": (_i32, [ctypes.POINTER(EmbeddingDesc), _u32, _u32]),
     "eagle_backend_x_b200_block_tables": (_i32, [ctypes.POINTER(PagedDesc)]),
     "eagle_backend_x_b200_slot_map": (_i32, [ctypes.POINTER(PagedDesc)]),
     "eagle_backend_x_b200_engine_create": (_i32, [ctypes.POINTER(EngineDesc), ctypes.POINTER(_P)]),

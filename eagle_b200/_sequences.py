@@ -248,7 +248,10 @@ class EmbeddingGrad(_Call):
     default ``grad``'s). With ``accumulate`` the sums are added to ``out`` (required then):
     rows without a token stay as they are. Each row is summed in 32 bits in one order that
     the sizes alone fix and rounded once, so the bits do not depend on the launch. The
-    workspace is about 16 bytes a token and a 32-bit row per 4 to 32 tokens."""
+    workspace is about 16 bytes a token and a 32-bit row per 4 to 32 tokens.
+
+    The waits for rows on their way are bounded. Should one run out, the rows of ``out`` that
+    needed them hold NaN, and :meth:`check` says so."""
 
     def __init__(self, grad, tokens, rows: int, *, scale: float = 1.0, first: int = 0, out=None, dtype=None,
                  accumulate: bool = False):
@@ -285,6 +288,18 @@ class EmbeddingGrad(_Call):
     def __call__(self, stream=None):
         self._enqueue(stream)
         return self.out
+
+    def check(self, stream=None):
+        """Wait for ``stream`` (by default the current one) and raise :class:`BackendError` if a wait of the last
+        call, which it is past then, ran out."""
+        if self.tokens.numel() == 0 or self.out.numel() == 0:
+            return
+        torch = _t()
+        with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream(self.device)):
+            lost = int(self._work[:4].view(torch.int32).item())
+        if lost:
+            raise _abi.BackendError(_abi.ERROR, "embedding_grad: a wait for rows ran out; the rows that needed them "
+                                                "are NaN")
 
 
 def embedding_grad(grad, tokens, rows: int, *, scale: float = 1.0, first: int = 0, out=None, dtype=None,

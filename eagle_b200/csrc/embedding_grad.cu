@@ -73,6 +73,9 @@ struct GradArgs {
     uint32_t slices;     // groups a row takes
     uint32_t pieces;     // packs (or columns) per row
     uint32_t sumBlocks;  // CTAs that sum; the others zero
+    uint32_t polls;      // of a wait for rows, after which it gives up
+    uint32_t asked;      // groups of rows asked for in the first chunk, at most
+    uint32_t* lost;      // set to 1 where a wait gave up
     uint32_t* listCount; // {runs of up to kWarpParts partials, of more}
     uint32_t* list;      // the chunks they start in
     uint32_t* longList;
@@ -264,6 +267,8 @@ __global__ __launch_bounds__(kClusterThreads) void clusterSortKernel(GradArgs a)
     const uint32_t item0 = warp * (32u * Items) + lane;
     if (cta == 0 && threadIdx.x < 2)
         a.listCount[threadIdx.x] = 0;
+    if (cta == 0 && threadIdx.x == 2)
+        *a.lost = 0;
     if (a.present != nullptr)
         for (int64_t w = int64_t(cta) * kClusterThreads + threadIdx.x; w < (a.rows + 31) / 32;
              w += int64_t(ctas) * kClusterThreads)
@@ -613,6 +618,7 @@ constexpr uint32_t kMaxChunk = 64;
 // bytes: 67 us against 56; of 800: 74, 72); of one that is not, half of that (520: 91, 104)
 constexpr int64_t kBulkLeast = 1024;
 constexpr uint32_t kBulkWaits = 1u << 22;  // polls before a wait gives up
+constexpr uint32_t kEvery = 0xffffffffu;
 
 struct BulkShared {
     alignas(16) unsigned char row[kBulkStages][kBulkRows][kBulkSlot];
@@ -642,9 +648,11 @@ __device__ __forceinline__ void bulkCopy(void* dst, const void* src, uint32_t by
 /** One CTA sums the runs that start in one chunk over 2 KB of the columns. A warp asks the copy
  *  engine for the rows, up to 16 ahead and each as the whole 16-byte words that hold it; four
  *  warps add them from shared memory. So the memory is kept busy whatever the adding
- *  threads wait for: 24 warps and 130 KB in flight an SM. */
+ *  threads wait for: six CTAs an SM, which is what the shared memory holds, with 24 adding warps
+ *  and up to 32 KB asked for each. (Compiled for those six, 131072 tokens of 8 KB take 360 us;
+ *  for no number, 377.) */
 template <class In, class Out, bool Aligned>
-__global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
+__global__ __launch_bounds__(kBulkThreads, 6) void bulkSumKernel(GradArgs a)
 {
     constexpr int N = 16 / int(sizeof(In));
     constexpr Piece P = Aligned ? Piece::Aligned : Piece::Shifted;
@@ -697,10 +705,12 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
     const uint32_t steps = (r1 - r0 + kBulkRows - 1) / kBulkRows;
     if (threadIdx.x >= kBulkLanes) {
         if (threadIdx.x == kBulkLanes) {
-            for (uint32_t j = 0; j < steps; ++j) {
+            const uint32_t most = chunk == 0 ? min(steps, a.asked) : steps;
+            uint32_t j = 0;
+            for (; j < most; ++j) {
                 const uint32_t stage = j % kBulkStages;
-                if (j >= kBulkStages && !mbarWait(&s.empty[stage], (j / kBulkStages - 1) & 1u, kBulkWaits))
-                    return;  // the adding warps gave up; they wait for what was asked for
+                if (j >= kBulkStages && !mbarWait(&s.empty[stage], (j / kBulkStages - 1) & 1u, a.polls))
+                    break;  // an adding warp gave up
                 const uint32_t rows = min(kBulkRows, r1 - r0 - j * kBulkRows);
                 const char* from[kBulkRows];
                 uint32_t size_[kBulkRows], sum = 0;
@@ -720,6 +730,9 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
                     if (u < rows)
                         bulkCopy(s.row[stage][u], from[u], size_[u], &s.full[stage]);
             }
+            // the shared memory stays until the last copies are there, whoever gave up
+            for (uint32_t k = j > kBulkStages ? j - kBulkStages : 0u; k < j; ++k)
+                (void)mbarWait(&s.full[k % kBulkStages], (k / kBulkStages) & 1u, a.polls);
         }
         return;
     }
@@ -738,30 +751,31 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
         acc[e] = 0.0f;
     uint32_t current = s.key[r0];
     bool partial = fromBefore;  // the run being summed began before: its sum is the chunk's head
-    for (uint32_t j = 0; j < steps; ++j) {
-        const uint32_t stage = j % kBulkStages, parity = (j / kBulkStages) & 1u;
-        if (!mbarWait(&s.full[stage], parity, kBulkWaits) && !mbarWait(&s.full[stage], parity, kBulkWaits)) {
+    // the run of ``key`` from here on: what was summed goes where it belongs
+    auto turnTo = [&](uint32_t key) {
+        if (!partial)
+            store(current, acc);
+        else if (active)
+            storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
+        partial = false;
+        current = key;
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                acc[e] = __int_as_float(0x7fc00000);  // rows that never came show
-        }
+        for (int e = 0; e < N; ++e)
+            acc[e] = 0.0f;
+    };
+    uint32_t j = 0;
+    for (; j < steps; ++j) {
+        const uint32_t stage = j % kBulkStages, parity = (j / kBulkStages) & 1u;
+        if (!__all_sync(kFull, mbarWait(&s.full[stage], parity, a.polls)))
+            break;
         const uint32_t rows = min(kBulkRows, r1 - r0 - j * kBulkRows);
 #pragma unroll
         for (uint32_t u = 0; u < kBulkRows; ++u) {
             if (u >= rows)
                 break;
             const uint32_t key = s.key[r0 + j * kBulkRows + u];
-            if (key != current) {
-                if (!partial)
-                    store(current, acc);
-                else if (active)
-                    storePartial<P, N>(a, a.head, chunk, col0, 1u, acc);
-                partial = false;
-                current = key;
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    acc[e] = 0.0f;
-            }
+            if (key != current)
+                turnTo(key);
             if (active) {
                 uint4 w;
                 if constexpr (Aligned) {
@@ -781,6 +795,19 @@ __global__ __launch_bounds__(kBulkThreads) void bulkSumKernel(GradArgs a)
         __syncwarp();
         if ((threadIdx.x & 31u) == 0)
             mbarArrive(&s.empty[stage]);
+    }
+    if (j < steps) {
+        // a wait gave up: the rows from there on count as NaN, unread, and the stage is not given
+        // back, so that nothing more is asked for into it
+        *a.lost = 1u;
+#pragma unroll 1
+        for (uint32_t r = r0 + j * kBulkRows; r < r1; ++r) {
+            if (s.key[r] != current)
+                turnTo(s.key[r]);
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                acc[e] = __int_as_float(0x7fc00000);
+        }
     }
     if (!partial && !joined) {
         store(current, acc);
@@ -1094,7 +1121,8 @@ struct GradPlan {
     uint32_t n = 0, bits = 0, passes = 0, digitBits = 0, bins = 0, tiles = 0;
     Piece piece = Piece::Strided;
     uint32_t pieces = 0, group = 0, slices = 0, chunk = 0, chunks = 0, width = 0;
-    uint64_t present = 0, listCount = 0, hist = 0, zeroed = 0;  // offsets; [0, zeroed) is cleared
+    bool bulk = false;
+    uint64_t lost = 0, present = 0, listCount = 0, hist = 0, zeroed = 0;  // offsets; [0, zeroed) is cleared
     uint64_t firstHist = 0, totals = 0, key[2] = {0, 0}, pos[2] = {0, 0}, list = 0, longList = 0, head = 0, tail = 0, bytes = 0;
 };
 
@@ -1119,6 +1147,7 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
                 && d.table_stride * outBytes % outWord == 0
             ? Piece::Aligned
             : Piece::Shifted;
+    p.bulk = p.piece != Piece::Strided && d.dim * inBytes >= (p.piece == Piece::Aligned ? kBulkLeast : kBulkLeast / 2);
     const int64_t columns = p.piece == Piece::Strided ? 4 : pack;
     p.pieces = uint32_t((d.dim + columns - 1) / columns);
     p.group = 1;
@@ -1142,6 +1171,7 @@ GradPlan planGrad(const eagle_b200_embedding_desc& d, const char* who)
         at += roundUp(bytes, 256);
         return was;
     };
+    p.lost = take(4);  // the scratch's first word: the caller may read it
     p.present = take((uint64_t(d.rows) + 31) / 32 * 4);
     p.listCount = take(8);
     const bool portable = p.n <= kPortableKeys;  // the query's answer does not depend on the device
@@ -1219,7 +1249,9 @@ constexpr int64_t zeroedBesideSort(unsigned perThread) { return (18ll + 6ll * pe
 constexpr int64_t kZeroedBesideJoin = 128ll << 20;
 constexpr int64_t kZeroedBesideSums = 24ll << 20;  // but the sums, of 5 us at least, have some first
 
-void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who)
+/** ``asked``: see GradArgs; anything below kEvery withholds rows, which the waits for them then miss. */
+void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who, uint32_t polls = kBulkWaits,
+    uint32_t asked = kEvery)
 {
     const int inBytes = elementBytes(d.values_type, who), outBytes = elementBytes(d.table_type, who);
     requireAddress(d.table, uint64_t(outBytes), who, "table");
@@ -1273,6 +1305,9 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.group = p.group;
     a.slices = p.slices;
     a.pieces = p.pieces;
+    a.polls = polls;
+    a.asked = asked;
+    a.lost = words(p.lost);
     a.listCount = words(p.listCount);
     a.list = words(p.list);
     a.longList = words(p.longList);
@@ -1343,9 +1378,7 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         a.order = words(p.pos[(p.passes + 1) & 1]);
     }
     const uint64_t lanes = uint64_t(p.chunks) * p.slices * p.group;
-    const bool bulk = p.piece != Piece::Strided
-        && d.dim * inBytes >= (p.piece == Piece::Aligned ? kBulkLeast : kBulkLeast / 2);
-    if (bulk) {
+    if (p.bulk) {
         a.slices = uint32_t((d.dim * inBytes + kBulkSlab - 1) / kBulkSlab);
         a.sumBlocks = gridOf(int64_t(p.chunks) * a.slices, who);
     } else {
@@ -1362,9 +1395,9 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
         withElement(d.table_type, [&](auto out) {
             using In = decltype(in);
             using Out = decltype(out);
-            if (bulk && p.piece == Piece::Aligned)
+            if (p.bulk && p.piece == Piece::Aligned)
                 launchBulkSum<In, Out, true>(a, blocks, s, who);
-            else if (bulk)
+            else if (p.bulk)
                 launchBulkSum<In, Out, false>(a, blocks, s, who);
             else if (p.piece == Piece::Aligned)
                 launchSum<In, Out, Piece::Aligned>(a, blocks, s, who);
@@ -1409,5 +1442,25 @@ EB_API eagle_backend_status eagle_backend_x_b200_embedding_grad(eagle_b200_embed
         requireDevice();
         DeviceScope scope(resolveDevice(d.device, d.table));
         enqueueGrad(d, p, who);
+    });
+}
+
+EB_API eagle_backend_status eagle_backend_x_b200_embedding_grad_wait_check(eagle_b200_embedding_desc* desc,
+    uint32_t polls, uint32_t asked)
+{
+    return guarded([&] {
+        const char* who = "eagle_backend_x_b200_embedding_grad_wait_check";
+        const eagle_b200_embedding_desc d = readDesc(desc, EAGLE_B200_EMBEDDING_ACCUMULATE, who);
+        checkEmbedding(d, who);
+        const GradPlan p = planGrad(d, who);
+        if (p.n == 0 || d.rows == 0 || d.dim == 0 || !p.bulk)
+            invalid(std::string(who) + ": needs tokens, and rows long enough for the copy engine");
+        if (polls == 0 || polls > kBulkWaits)
+            invalid(std::string(who) + ": polls must lie in [1, 2^22]");
+        if (d.scratch == 0)
+            invalid(std::string(who) + ": needs embedding_grad's scratch (query it there)");
+        requireDevice();
+        DeviceScope scope(resolveDevice(d.device, d.table));
+        enqueueGrad(d, p, who, polls, asked);
     });
 }

@@ -943,8 +943,20 @@ eagle_backend_status eagle_backend_x_b200_embedding(const struct eagle_b200_embe
  * (stable) and each row summed in 32 bits in token order, in runs of a length fixed by the
  * sizes alone, so the bits depend on neither the launch nor the device's load; one
  * rounding to table_type at the end. The values' strides may be anything, 0 (a broadcast
- * gradient) included. Query with scratch == 0. */
+ * gradient) included. Query with scratch == 0.
+ * Long rows are brought in by the copy engine, and the waits for them are bounded (2^22
+ * polls). The first 32-bit word of scratch is 0 after a call with tokens, rows and a dim;
+ * it is 1 if a wait gave up: the rows of the table that needed values which had not come
+ * then hold NaN in those columns, the others are as ever. */
 eagle_backend_status eagle_backend_x_b200_embedding_grad(struct eagle_b200_embedding_desc* desc);
+
+/* eagle_backend_x_b200_embedding_grad_wait_check: embedding_grad with the values behind the
+ * first 4 * ``asked`` positions of the sorted order never asked for in the first run of
+ * positions that is summed together, to exercise the bounded wait: those that add them
+ * poll ``polls`` times (in [1, 2^22]; embedding_grad uses 2^22) and give up. Same desc and
+ * scratch; INVALID_ARGUMENT where the values' rows are too short for the copy engine. */
+eagle_backend_status eagle_backend_x_b200_embedding_grad_wait_check(struct eagle_b200_embedding_desc* desc,
+    uint32_t polls, uint32_t asked);
 
 /* A paged cache: ``requests`` sequences whose tokens lie in blocks of ``block`` places;
  * row r of ``table`` (int32[requests][width], row stride ``table_stride``) names request

@@ -793,3 +793,49 @@ def test_in_the_body_of_a_device_loop(eb, n):
     assert spot.offsets[-1].item() == requests
     # position 1 lies in the first block, whose id is 0
     assert bool((spot.slots[:requests] == 1).all()) and bool((spot.slots[requests:] == -1).all())
+
+
+# ------------------------------------------------------------------------- waits that run out
+
+@pytest.mark.parametrize("dim", (1024, 1023))
+@pytest.mark.parametrize("asked", (0, 1, 2, 5))
+@pytest.mark.parametrize("lengths", ([3, 2, 3, 2], [2, 5, 4, 1], [40, 3, 1], [1, 39, 2, 2], [8, 8, 8]))
+def test_gradient_wait_gives_up(eb, dim, asked, lengths):
+    """Some rows of the first chunk (8 sorted positions here) are never asked for: the runs whose rows had all come
+    are right, those that needed the others NaN and no others, and the call can tell; the same workspace then
+    serves a whole gradient. Every wait ends: 1024 polls."""
+    import ctypes
+
+    from eagle_b200 import _abi
+
+    chunk, group = 8, 4
+    ids = np.repeat(np.arange(len(lengths) + 20), lengths + [2] * 20)
+    rows, n = int(ids[-1]) + 2, len(ids)
+    grad = _values(_gen(22, dim), (n, dim), torch.bfloat16).cuda()
+    out = torch.full((rows, dim), 5.0, device="cuda")
+    call = eb.EmbeddingGrad(grad, torch.from_numpy(ids).cuda(), rows, out=out)
+    want = call().clone()
+    call.check()
+    d = _abi.new(_abi.EmbeddingDesc)
+    ctypes.memmove(ctypes.byref(d), ctypes.byref(call._desc), ctypes.sizeof(d))
+    d.stream = torch.cuda.current_stream().cuda_stream
+    _abi.check(_abi.lib().eagle_backend_x_b200_embedding_grad_wait_check(ctypes.byref(d), 1024, asked))
+    torch.cuda.synchronize()
+    # the first chunk sums its own 8 positions, and those of a run that goes on over one boundary only
+    starts = np.cumsum([0] + lengths)
+    last = int(np.searchsorted(starts, chunk - 1, side="right")) - 1
+    whole = starts[last] > 0 and starts[last + 1] <= 2 * chunk and starts[last + 1] > chunk
+    summed = starts[last + 1] if whole else chunk
+    lost = set(ids[min(group * asked, summed):summed].tolist())
+    for r in range(rows):
+        if r in lost:
+            assert bool(out[r].isnan().all()), r
+        else:
+            assert torch.equal(out[r], want[r]), r
+    if lost:
+        with pytest.raises(eb.BackendError, match="wait"):
+            call.check()
+    else:
+        call.check()
+    assert torch.equal(call(), want)
+    call.check()

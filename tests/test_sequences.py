@@ -155,3 +155,17 @@ def test_host_tensors_are_refused(eb):
         eb.block_tables(lengths, lengths, tables, lengths, lengths[:1], block=16)
     with pytest.raises(ValueError, match="CUDA tensor"):
         eb.slot_map(tables, lengths, lengths, 8, block=16)
+
+
+@pytest.mark.parametrize("fields,polls", [
+    (dict(batch=0), 100), (dict(rows=0), 100), (dict(dim=0, table_stride=0), 100),
+    (dict(), 100),  # 128 bytes a row: read without the copy engine
+    (dict(dim=1024, table_stride=1024), 0), (dict(dim=1024, table_stride=1024), 2**22 + 1),
+    (dict(dim=1024, table_stride=1024, scratch=0), 100), (dict(dim=1024, table_stride=1024, first=-1), 100),
+])
+def test_gradient_wait_check_refuses(fields, polls):
+    d = _embedding(**{"scratch": 1 << 20, **fields})
+    d.value_strides[:] = [8 * d.dim, d.dim, 1]
+    entry = _abi.lib().eagle_backend_x_b200_embedding_grad_wait_check
+    assert entry(ctypes.byref(d), polls, 1) == _abi.INVALID_ARGUMENT
+    assert "wait_check" in _abi.last_error()
