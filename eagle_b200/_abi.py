@@ -38,6 +38,7 @@ MODEL_OSCILLATOR, MODEL_OSCILLATOR_SPREAD, MODEL_GAMBLER, MODEL_LORENZ = 0, 1, 2
 MODE_BAND, MODE_PERSIST, MODE_FUSED, MODE_BAND_EAGER = 0, 1, 2, 3
 TYPE_F32, TYPE_BF16, TYPE_F16, TYPE_I32, TYPE_I64 = range(5)
 EMBEDDING_ACCUMULATE = 1
+SLOT_MAP_HELD = 2
 FLAG_FMA = 1
 FLAG_INDEX_ORDER = 2
 

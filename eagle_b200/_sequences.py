@@ -355,7 +355,9 @@ class BlockTables(_Call):
     (``held`` for the next call) and int32 ``[taken, short]``.
 
     A request is *short*, and keeps what it holds, when its row is too narrow or the pool,
-    less what the requests before it asked for, too small. ``held`` and ``pool`` are not
+    less what the requests before it asked for, too small. Entries of a row past what its
+    request holds are left as they were, given back ones included: :class:`SlotMap` takes
+    ``blocks`` to pass over them. ``held`` and ``pool`` are not
     written, so a call repeated on the same inputs gives the same result."""
 
     def __init__(self, lengths, held, table, pool, count, *, block: int, used=None, terminated=None):
@@ -406,23 +408,29 @@ class SlotMap(_Call):
     (``dtype`` int64 or int32), its position (``start``'s type) and its request (int32), and
     int32 ``offsets`` of requests + 1 entries, request r's tokens being
     ``offsets[r]:offsets[r + 1]``. A token whose position lies past the table's width, whose
-    block is not there (a negative entry) or whose slot does not fit ``dtype`` has slot -1.
+    block is not there (a negative entry) or whose slot does not fit ``dtype`` has slot -1;
+    with ``held`` (int32: the blocks each request holds, ``BlockTables.blocks``) also one
+    whose position lies past those. Give it wherever a row of the table serves one request
+    after the other: without, a request left short takes what the one before left there.
 
     The first three have ``capacity`` entries whatever the number of tokens, so that a
     captured graph can serve any batch: entries past the last token have slot -1, position
     0 and request -1 (:class:`Embedding` gives zeros for a token marked -1); tokens past
     ``capacity`` are left out, which ``offsets`` shows."""
 
-    def __init__(self, table, start, fresh, capacity: int, *, block: int, terminated=None, dtype=None):
+    def __init__(self, table, start, fresh, capacity: int, *, block: int, held=None, terminated=None, dtype=None):
         torch = _t()
         d = _paged_desc(table, start, block, terminated, "start")
         device, requests = table.device, table.shape[0]
         _vector(fresh, requests, (start.dtype,), device, "fresh")
+        if held is not None:
+            _vector(held, requests, (torch.int32,), device, "held")
+            d.held, d.flags = _ptr(held), _abi.SLOT_MAP_HELD
         dtype = dtype or torch.int64
         d.slot_type = _type(dtype, "dtype", "index")
         if int(capacity) < 0:
             raise ValueError("capacity must not be negative")
-        self.table, self.start, self.fresh, self.terminated = table, start, fresh, terminated
+        self.table, self.start, self.fresh, self.held, self.terminated = table, start, fresh, held, terminated
         d.capacity = int(capacity)
         d.start, d.fresh = _ptr(start), _ptr(fresh)
         self._work = _query("eagle_backend_x_b200_slot_map", d, device)  # refuses before anything is allocated
@@ -440,7 +448,8 @@ class SlotMap(_Call):
         return self.slots, self.positions, self.requests, self.offsets
 
 
-def slot_map(table, start, fresh, capacity: int, *, block: int, terminated=None, dtype=None, stream=None):
+def slot_map(table, start, fresh, capacity: int, *, block: int, held=None, terminated=None, dtype=None, stream=None):
     """The packed new tokens' ``(slots, positions, requests, offsets)`` (:class:`SlotMap`)."""
     with _on(stream):
-        return SlotMap(table, start, fresh, capacity, block=block, terminated=terminated, dtype=dtype)(stream)
+        return SlotMap(table, start, fresh, capacity, block=block, held=held, terminated=terminated,
+                       dtype=dtype)(stream)

@@ -380,8 +380,8 @@ __global__ __launch_bounds__(kThreads) void blockTablesKernel(PagedArgs a)
 
 /** kTokens neighbouring tokens a thread and step: four, stored as words, or one where that leaves
  *  SMs idle. ``Copied``: the scan is read from scratch into shared memory first (up to kScanAtOnce requests),
- *  where a search is a tenth of the time. */
-template <class Len, class Slot, uint32_t kTokens, bool InBlock, bool Copied>
+ *  where a search is a tenth of the time. ``Held``: entries past what a request holds are not read. */
+template <class Len, class Slot, uint32_t kTokens, bool InBlock, bool Copied, bool Held>
 __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
 {
     __shared__ uint32_t segment[InBlock ? kMaxSegments + 1 : 1];
@@ -430,7 +430,8 @@ __global__ __launch_bounds__(kThreads) void slotMapKernel(PagedArgs a)
                 if (p < uint64_t(a.room)) {
                     const uint32_t b = a.perBlock(uint32_t(p));
                     within[k] = uint32_t(p) - b * a.perBlock.d;
-                    id[k] = a.table[int64_t(r) * a.tableStride + b];
+                    if (!Held || int64_t(b) < int64_t(a.held[r]))
+                        id[k] = a.table[int64_t(r) * a.tableStride + b];
                 }
             }
         }
@@ -498,19 +499,20 @@ unsigned gridFor(int64_t threads, int64_t most)
     return unsigned(std::max<int64_t>(1, std::min(most * smCount(), (threads + kThreads - 1) / kThreads)));
 }
 
-template <class Len, class Slot, uint32_t kTokens>
+template <class Len, class Slot, uint32_t kTokens, bool Held>
 void launchSlots(const PagedArgs& a, cudaStream_t s, const char* who)
 {
     const int64_t threads = (int64_t(a.capacity) + kTokens - 1) / kTokens;
     if (a.requests <= kScanInBlock) {
-        launchBehind(slotMapKernel<Len, Slot, kTokens, true, false>, gridFor(threads, 4), kThreads, 0, s, a, who);
+        launchBehind(slotMapKernel<Len, Slot, kTokens, true, false, Held>, gridFor(threads, 4), kThreads, 0, s, a, who);
         return;
     }
     launchScan<Tokens, Len>(a, s, who);
     if (a.requests <= kScanAtOnce)
-        launchBehind(slotMapKernel<Len, Slot, kTokens, false, true>, gridFor(threads, 4), kThreads, 0, s, a, who);
+        launchBehind(slotMapKernel<Len, Slot, kTokens, false, true, Held>, gridFor(threads, 4), kThreads, 0, s, a, who);
     else
-        launchBehind(slotMapKernel<Len, Slot, kTokens, false, false>, gridFor(threads, 4), kThreads, 0, s, a, who);
+        launchBehind(slotMapKernel<Len, Slot, kTokens, false, false, Held>, gridFor(threads, 4), kThreads, 0, s, a,
+            who);
 }
 
 }  // namespace
@@ -578,7 +580,8 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
 {
     return guarded([&] {
         const char* who = "eagle_backend_x_b200_slot_map";
-        const eagle_b200_paged_desc d = readDesc(desc, 0u, who);
+        const eagle_b200_paged_desc d = readDesc(desc, EAGLE_B200_SLOT_MAP_HELD, who);
+        const bool held = (d.flags & EAGLE_B200_SLOT_MAP_HELD) != 0;
         if (desc->struct_size < sizeof d)
             invalid(std::string(who) + ": struct_size too small for the query's answer");
         PagedArgs a = pagedArgs(d, who);
@@ -600,6 +603,8 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
         if (d.requests > 0) {
             requireAddress(d.start, uint64_t(bytes), who, "start");
             requireAddress(d.fresh, uint64_t(bytes), who, "fresh");
+            if (held)
+                requireAddress(d.held, 4, who, "held");
             if (d.width > 0)
                 requireAddress(d.table, 4, who, "table");
         }
@@ -607,6 +612,7 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
         DeviceScope scope(resolveDevice(d.device, d.offsets));
         a.start = reinterpret_cast<const void*>(d.start);
         a.fresh = reinterpret_cast<const void*>(d.fresh);
+        a.held = reinterpret_cast<const int32_t*>(d.held);
         a.capacity = uint32_t(d.capacity);
         a.slots = reinterpret_cast<void*>(d.slots);
         a.positions = reinterpret_cast<void*>(d.positions);
@@ -617,10 +623,15 @@ EB_API eagle_backend_status eagle_backend_x_b200_slot_map(eagle_b200_paged_desc*
             withIndex(d.slot_type, [&](auto slot) {
                 using Len = decltype(len);
                 using Slot = decltype(slot);
-                if (d.capacity <= int64_t(smCount()) * kThreads)
-                    launchSlots<Len, Slot, 1>(a, s, who);
+                const bool few = d.capacity <= int64_t(smCount()) * kThreads;
+                if (few && held)
+                    launchSlots<Len, Slot, 1, true>(a, s, who);
+                else if (few)
+                    launchSlots<Len, Slot, 1, false>(a, s, who);
+                else if (held)
+                    launchSlots<Len, Slot, 4, true>(a, s, who);
                 else
-                    launchSlots<Len, Slot, 4>(a, s, who);
+                    launchSlots<Len, Slot, 4, false>(a, s, who);
             });
         });
     });

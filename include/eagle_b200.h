@@ -903,6 +903,9 @@ eagle_backend_status eagle_backend_x_b200_probe_fp64(int32_t device, uint32_t ki
 /* embedding_grad: add to the table's rows instead of writing all of them. */
 #define EAGLE_B200_EMBEDDING_ACCUMULATE 1u
 
+/* slot_map: ``held`` says how many entries of each request's row are its blocks. */
+#define EAGLE_B200_SLOT_MAP_HELD 2u
+
 /* A table of ``rows`` x ``dim`` values, the row of token id ``first + r`` being row r
  * (``first`` > 0: a contiguous shard of a larger table), ``batch`` x ``seq`` token ids,
  * and one vector of ``dim`` values per token. Strides are in elements. */
@@ -963,7 +966,7 @@ eagle_backend_status eagle_backend_x_b200_embedding_grad_wait_check(struct eagle
  * r's blocks in order of position. */
 struct eagle_b200_paged_desc {
     uint32_t struct_size;
-    uint32_t flags;        /* 0 */
+    uint32_t flags;        /* slot_map: EAGLE_B200_SLOT_MAP_HELD */
     int32_t device;        /* -1: the device owning the table */
     uint32_t length_type;  /* of lengths, start, fresh and positions: I32 or I64 */
     uint32_t slot_type;    /* of slots: I32 or I64 */
@@ -975,7 +978,7 @@ struct eagle_b200_paged_desc {
     uint64_t table;
     uint64_t terminated;   /* u8[requests] or 0: a set byte is a finished request */
     uint64_t lengths;      /* block_tables: the length each request is to have room for */
-    uint64_t held;         /* block_tables: int32[requests], the blocks each has */
+    uint64_t held;         /* block_tables, slot_map with SLOT_MAP_HELD: int32[requests], the blocks each has */
     uint64_t pool;         /* block_tables: int32[pool_size], ids of free blocks */
     uint64_t count;        /* block_tables: uint32, how many of the pool are valid */
     int64_t pool_size;
@@ -1013,7 +1016,10 @@ eagle_backend_status eagle_backend_x_b200_block_tables(struct eagle_b200_paged_d
  * both at most 2^31 - 1), and the i-th of them has position start[r] + i, request r and
  * slot table[r][position / block] * block + position % block; slot -1 where the position
  * lies past the table's width (one past length_type's range wraps), the entry is
- * negative or the slot does not fit slot_type.
+ * negative or the slot does not fit slot_type. With SLOT_MAP_HELD (block_tables' blocks
+ * as ``held``) also where it lies past the blocks the request holds: block_tables leaves
+ * what a request gave back in its row, and a request that comes into that row and is
+ * left short has it behind its own. Without, every entry that is not negative counts.
  * Entries past the last token get slot -1, position 0 and request -1; tokens past
  * ``capacity`` are left out. Negative starts and counts count as 0. Query with
  * scratch == 0. */

@@ -839,3 +839,72 @@ def test_gradient_wait_gives_up(eb, dim, asked, lengths):
         call.check()
     assert torch.equal(call(), want)
     call.check()
+
+
+# ------------------------------------------------------------------------- rows that serve one request after the other
+
+@pytest.mark.parametrize("requests", (0, 1, 5, 513, 2048, 2049, 8192, 8193))
+@pytest.mark.parametrize("dtype,slot", [(np.int32, torch.int64), (np.int64, torch.int32)])
+def test_slots_of_held_blocks(eb, requests, dtype, slot):
+    """Entries past what a request holds are as good as absent."""
+    rng = _gen(23, requests)
+    width, block = 12, 16
+    table = rng.integers(-1, 1000, (requests, width)).astype(np.int32)
+    held = rng.integers(-2, width + 4, requests).astype(np.int32)
+    start = rng.integers(-2, width * block, requests).astype(dtype)
+    fresh = rng.integers(0, 40, requests).astype(dtype)
+    own = np.where(np.arange(width) < held[:, None], table, -1)
+    total = int(fresh.sum())
+    dev = [torch.from_numpy(np.ascontiguousarray(x)).cuda() for x in (table, start, fresh, held)]
+    for capacity in {0, max(0, total - 3), total + 5}:
+        want = _want_slots(own, start, fresh, capacity, block, None, 64 if slot == torch.int64 else 32)
+        got = eb.slot_map(*dev[:3], capacity, block=block, held=dev[3], dtype=slot)
+        for g, w, name in zip(got, want, ("slots", "positions", "requests", "offsets")):
+            assert np.array_equal(g.cpu().numpy().astype(np.int64), w), name
+
+
+def test_a_reused_row_left_short(eb):
+    """The loop of a paged cache, its rows reused: a request that comes into a finished one's row while others took
+    the blocks it gave back has no slot among theirs, in a replayed graph."""
+    dev = dict(dtype=torch.int32, device="cuda")
+    block, width, blocks = 4, 3, 6
+    lengths = torch.tensor([12, 4, 0], **dev)
+    held, start, fresh = (torch.zeros(3, **dev) for _ in range(3))
+    tables = torch.full((3, width), -1, **dev)
+    used = torch.zeros(blocks, dtype=torch.bool, device="cuda")
+    terminated = torch.zeros(3, dtype=torch.bool, device="cuda")
+    free = eb.Compactor(used)
+    grow = eb.BlockTables(lengths, held, tables, free.index_map, free.count, block=block, used=used,
+                          terminated=terminated)
+    spot = eb.SlotMap(tables, start, fresh, 16, block=block, held=held, terminated=terminated)
+
+    def step():
+        free()
+        grow()
+        held.copy_(grow.blocks)
+        spot()
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    graph.replay()
+    assert held.tolist() == [3, 1, 0] and tables[0].tolist() == [0, 1, 2]
+    terminated[0] = True  # request 0 ends
+    graph.replay()
+    assert held.tolist() == [0, 1, 0] and int(used.sum()) == 1
+    lengths.copy_(torch.tensor([0, 12, 12], **dev))  # the others take all but one of the blocks
+    graph.replay()
+    assert held.tolist() == [0, 3, 3] and int(used.sum()) == 6
+    terminated[0] = False  # and the next request comes into its row
+    lengths[0] = 9
+    start.copy_(torch.tensor([0, 4, 0], **dev))
+    fresh.copy_(torch.tensor([9, 2, 3], **dev))
+    graph.replay()
+    assert grow.cells.tolist() == [0, 1] and held.tolist() == [0, 3, 3]
+    assert tables[0].tolist() == [0, 1, 2]  # what the one before left
+    assert spot.offsets.tolist() == [0, 9, 11, 14]
+    assert spot.slots[:9].eq(-1).all() and spot.requests[:9].eq(0).all() and spot.positions[:9].tolist() == list(range(9))
+    rows = tables.cpu().numpy()
+    assert spot.slots[9:14].tolist() == [rows[1, 1] * 4, rows[1, 1] * 4 + 1] + [rows[2, 0] * 4 + i for i in range(3)]

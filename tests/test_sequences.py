@@ -169,3 +169,14 @@ def test_gradient_wait_check_refuses(fields, polls):
     entry = _abi.lib().eagle_backend_x_b200_embedding_grad_wait_check
     assert entry(ctypes.byref(d), polls, 1) == _abi.INVALID_ARGUMENT
     assert "wait_check" in _abi.last_error()
+
+
+@pytest.mark.parametrize("entry,fields,status", [
+    ("slot_map", dict(flags=_abi.SLOT_MAP_HELD, scratch=1 << 20, held=0), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(flags=_abi.SLOT_MAP_HELD, scratch=1 << 20, held=(1 << 20) + 2), _abi.INVALID_ARGUMENT),
+    ("slot_map", dict(flags=4), _abi.UNSUPPORTED),
+    ("block_tables", dict(flags=_abi.SLOT_MAP_HELD), _abi.UNSUPPORTED),
+])
+def test_slot_map_held_refuses(entry, fields, status):
+    d = _paged(**fields)
+    assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == status
