@@ -358,7 +358,10 @@ class BlockTables(_Call):
     less what the requests before it asked for, too small. Entries of a row past what its
     request holds are left as they were, given back ones included: :class:`SlotMap` takes
     ``blocks`` to pass over them. ``held`` and ``pool`` are not
-    written, so a call repeated on the same inputs gives the same result."""
+    written, so a call repeated on the same inputs gives the same result. Copy ``blocks`` to
+    ``held`` before the free list is made again: a terminated request whose old count stays
+    gives the same blocks back in every call, whoever has them by then, and an id that is in
+    the pool and given back too is set and cleared in no order. No two requests share a block."""
 
     def __init__(self, lengths, held, table, pool, count, *, block: int, used=None, terminated=None):
         torch = _t()

@@ -1005,7 +1005,11 @@ struct eagle_b200_paged_desc {
  * fit in what the requests before it left of the pool (those left short included), or
  * that needs more than ``width``, keeps what it holds and is counted short; one that
  * needs no more than it holds keeps its blocks. A terminated request gives its blocks
- * back: their bytes in ``used`` are cleared and it then holds 0. Entries of ``table``
+ * back: their bytes in ``used`` are cleared and it then holds 0. A block has one place:
+ * an id among the pool's valid ones, or in the rows of two requests, that a terminated
+ * request still holds is set and cleared in no order. So ``held`` is to be this call's
+ * ``blocks`` before the free list is made again: a terminated request whose old count
+ * stays gives the same blocks back in every call, whoever has them by then. Entries of ``table``
  * past what a request holds are left as they were; ``held`` is not written. A count
  * above pool_size (compact_device's report of a failure) is an empty pool. Negative
  * lengths and holdings count as 0. Query with scratch == 0. */
