@@ -144,34 +144,36 @@ def _query(entry, desc, device):
 
 # ------------------------------------------------------------------------- embedding
 
-def _axes(x, dims, what):
-    """Sizes and strides of the first ``dims`` axes of ``x`` as (batch, seq)."""
-    shape, stride = list(x.shape[:dims]), list(x.stride()[:dims])
-    while len(shape) > 2:  # join the two leading axes if one stride serves both
-        if shape[0] != 1 and shape[1] != 1 and stride[0] != shape[1] * stride[1]:
-            raise ValueError(f"{what} of {dims} axes must join into two (reshape it)")
-        keep = 1 if shape[1] != 1 else 0
-        shape[:2], stride[:2] = [shape[0] * shape[1]], [stride[keep]]
-    while len(shape) < 2:
-        shape.insert(0, 1)
-        stride.insert(0, 0)
-    return shape, stride
+def _axes(tokens, values):
+    """The tokens' axes as (batch, seq): sizes, and strides of the tokens and of their vectors. Neighbouring axes
+    are joined where one stride serves both, in both tensors."""
+    if tokens.numel() == 0:
+        return [0, 1], [0, 0], [0, 0]
+    joined = []
+    for n, s, v in zip(tokens.shape, tokens.stride(), values.stride()):
+        if n == 1:
+            continue
+        if joined and joined[-1][1:] == (n * s, n * v):
+            joined[-1] = (joined[-1][0] * n, s, v)
+        else:
+            joined.append((n, s, v))
+    if len(joined) > 2:
+        raise ValueError(f"the {tokens.dim()} axes of the tokens must join into two, for them and their vectors alike "
+                         "(reshape them)")
+    return tuple(zip(*([(1, 0, 0)] * (2 - len(joined)) + joined)))
 
 
 def _embedding_desc(table, values, tokens, rows, scale, first, device):
     torch = _t()
     dim = values.shape[-1]
-    shape, token_strides = _axes(tokens, tokens.dim(), "tokens")
-    vshape, value_strides = _axes(values, tokens.dim(), "the tokens' vectors")
-    if shape != vshape:  # they join differently: both as one long axis
-        raise ValueError("tokens and their vectors must have the same leading axes")
+    shape, token_strides, value_strides = _axes(tokens, values)
     d = _abi.new(_abi.EmbeddingDesc, device=device.index, table_type=_type(table.dtype, "the table", "element"),
                  values_type=_type(values.dtype, "the tokens' vectors", "element"),
                  token_type=_type(tokens.dtype, "tokens", "index"), table=_ptr(table), tokens=_ptr(tokens),
                  values=_ptr(values), rows=int(rows), dim=dim, first=int(first), batch=shape[0], seq=shape[1],
                  table_stride=max(table.stride(0), dim), scale=float(scale))
     d.token_strides[:] = token_strides
-    d.value_strides[:] = value_strides + [values.stride(-1) if values.dim() else 1]
+    d.value_strides[:] = [*value_strides, values.stride(-1)]
     return d
 
 
@@ -198,7 +200,8 @@ class Embedding(_Call):
 
     ``table`` is (rows, dim), float32, bfloat16 or float16, each row contiguous; the rows
     may lie apart (a slice of a wider or longer one). ``tokens`` are int32 or int64 of any
-    shape and strides. A token outside ``[first, first + rows)`` -- padding marked -1, a row
+    shape; their axes must join into two, each of one stride (two axes or fewer always do).
+    A token outside ``[first, first + rows)`` -- padding marked -1, a row
     that another rank's shard holds -- gives zeros. ``out`` (or its ``dtype``, by default the
     table's) may be any of the three types. Calls return ``out``, of shape
     ``(*tokens.shape, dim)``."""
@@ -244,7 +247,8 @@ class EmbeddingGrad(_Call):
     ``first + v``, and zeros for a row without a token.
 
     ``grad`` is ``(*tokens.shape, dim)``, float32, bfloat16 or float16, with any strides, a
-    broadcast's zeros included. ``out`` is (rows, dim), contiguous rows, of ``dtype`` (by
+    broadcast's zeros included (of more than two leading axes: that join into two where the
+    tokens' do). ``out`` is (rows, dim), contiguous rows, of ``dtype`` (by
     default ``grad``'s). With ``accumulate`` the sums are added to ``out`` (required then):
     rows without a token stay as they are. Each row is summed in 32 bits in one order that
     the sizes alone fix and rounded once, so the bits do not depend on the launch. The

@@ -908,3 +908,15 @@ def test_a_reused_row_left_short(eb):
     assert spot.slots[:9].eq(-1).all() and spot.requests[:9].eq(0).all() and spot.positions[:9].tolist() == list(range(9))
     rows = tables.cpu().numpy()
     assert spot.slots[9:14].tolist() == [rows[1, 1] * 4, rows[1, 1] * 4 + 1] + [rows[2, 0] * 4 + i for i in range(3)]
+
+
+# ------------------------------------------------------------------------- calls that were refused
+
+def test_axes_that_join_behind_the_first(eb):
+    """Tokens of three axes whose last two join, and whose first two do not, are looked up and summed."""
+    rng = _gen(24)
+    table = _values(rng, (50, 24), torch.bfloat16).cuda()
+    ids = torch.from_numpy(rng.integers(-1, 50, (40, 3))).cuda().t().view(3, 8, 5)
+    _check_lookup(eb, table, ids)
+    _check_gradient(eb, _values(rng, (3, 8, 5, 24), torch.float32).cuda(), ids, 50)
+    _check_gradient(eb, _values(rng, (3, 40, 30), torch.float32).cuda()[..., 3:27].unflatten(1, (8, 5)), ids, 50)

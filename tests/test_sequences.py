@@ -180,3 +180,37 @@ def test_gradient_wait_check_refuses(fields, polls):
 def test_slot_map_held_refuses(entry, fields, status):
     d = _paged(**fields)
     assert getattr(_abi.lib(), "eagle_backend_x_b200_" + entry)(ctypes.byref(d)) == status
+
+
+def _offsets(shape, strides):
+    grid = torch.zeros(tuple(shape), dtype=torch.int64)
+    for axis, (n, s) in enumerate(zip(shape, strides)):
+        grid += (torch.arange(n) * s).view([-1 if a == axis else 1 for a in range(len(shape))])
+    return grid.flatten()
+
+
+def test_axes_join_wherever_one_stride_serves_them():
+    """Any number of axes, as long as they make two of one stride each; which ones join does not matter."""
+    from eagle_b200._sequences import _axes
+
+    ids = torch.arange(2 * 3 * 4 * 5)
+    vectors = torch.zeros(120, 7)
+    wide = torch.zeros(3, 40, 9)[:, :20, 1:8]
+    for tokens, values in (
+            (ids[0], vectors[0]), (ids, vectors), (ids.view(24, 5), vectors.view(24, 5, 7)),
+            (ids.view(24, 5).t(), vectors.view(5, 24, 7)), (ids[:1].view(1, 1, 1), vectors[:1].view(1, 1, 1, 7)),
+            (ids.view(2, 3, 4, 5), vectors.view(2, 3, 4, 5, 7)), (ids.view(12, 1, 10), vectors.view(12, 1, 10, 7)),
+            # the last two axes join and the first two do not, and the other way round
+            (ids.view(40, 3).t().view(3, 8, 5), vectors.view(3, 8, 5, 7)),
+            (ids.view(24, 5)[:, :4].unflatten(0, (4, 6)), vectors[:96].view(4, 6, 4, 7)),
+            (ids[:60].view(3, 4, 5), wide.unflatten(1, (4, 5))), (ids[:8].expand(5, 3, 8), vectors.view(5, 3, 8, 7)),
+            (ids.view(2, 60)[:0], vectors.view(2, 60, 7)[:0]), (ids.view(2, 3, 20)[:, :0], vectors.view(2, 3, 20, 7)[:, :0]),
+            (ids.view(2, 3, 20).transpose(0, 2)[:0], vectors.view(20, 3, 2, 7)[:0])):
+        shape, at, to = _axes(tokens, values)
+        assert len(shape) == len(at) == len(to) == 2 and shape[0] * shape[1] == tokens.numel()
+        assert torch.equal(_offsets(shape, at), _offsets(tokens.shape, tokens.stride()))
+        assert torch.equal(_offsets(shape, to), _offsets(tokens.shape, values.stride()[:-1]))
+    for tokens, values in ((ids.view(5, 4, 6).transpose(0, 2), vectors.view(6, 4, 5, 7)),
+                           (ids.view(24, 5)[:, :4].unflatten(0, (4, 6)), vectors.view(4, 30, 7)[:, :24].unflatten(1, (6, 4)))):
+        with pytest.raises(ValueError, match="join"):
+            _axes(tokens, values)
