@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import math
 
 from . import _abi
 from ._api import _ptr, _t
@@ -69,13 +70,28 @@ def _extent(x):
     return x.data_ptr(), x.data_ptr() + (last + 1) * x.element_size()
 
 
+def _beside(x, y):
+    """Whether ``x`` and ``y`` lie in columns of one plane that do not meet: apart within every row of it."""
+    pitch, runs = 0, []
+    for t in (x, y):
+        inner = t.dim() - 1 if t.dim() and t.stride(-1) == 1 else t.dim()  # the axes before a contiguous last one
+        runs.append((t.shape[-1] if inner < t.dim() else 1) * t.element_size())
+        for n, s in zip(t.shape[:inner], t.stride()):
+            if n > 1:
+                pitch = math.gcd(pitch, s * t.element_size())
+    if pitch == 0:
+        return False
+    ahead = (y.data_ptr() - x.data_ptr()) % pitch
+    return runs[0] <= ahead and ahead + runs[1] <= pitch
+
+
 def _apart(out, what, *inputs):
     """``out`` shares no memory with the inputs."""
     lo, hi = _extent(out)
     for x in inputs:
         if x is not None:
             a, b = _extent(x)
-            if lo < b and a < hi:
+            if lo < b and a < hi and not _beside(out, x):
                 raise ValueError(f"{what} overlaps an input")
 
 

@@ -920,3 +920,17 @@ def test_axes_that_join_behind_the_first(eb):
     _check_lookup(eb, table, ids)
     _check_gradient(eb, _values(rng, (3, 8, 5, 24), torch.float32).cuda(), ids, 50)
     _check_gradient(eb, _values(rng, (3, 40, 30), torch.float32).cuda()[..., 3:27].unflatten(1, (8, 5)), ids, 50)
+
+
+def test_columns_of_one_plane(eb):
+    """The table and its output, or a gradient and the table's, in columns of one plane: what lies around stays."""
+    rng = _gen(25)
+    for cut, dtype in ((64, torch.bfloat16), (61, torch.bfloat16), (700, torch.float32), (1023, torch.float16)):
+        plane = _values(rng, (300, 2 * cut + 3), dtype).cuda()
+        was = plane.clone()
+        ids = torch.from_numpy(rng.integers(-1, 300, 300)).cuda()
+        left, right = plane[:, :cut], plane[:, cut + 2:2 * cut + 2]
+        _check_lookup(eb, left, ids, out=right)
+        assert torch.equal(left, was[:, :cut]) and torch.equal(plane[:, cut:cut + 2], was[:, cut:cut + 2])
+        _check_gradient(eb, right, ids, 300, out=left)
+        assert torch.equal(plane[:, cut:cut + 2], was[:, cut:cut + 2]) and torch.equal(plane[:, -1], was[:, -1])

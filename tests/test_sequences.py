@@ -214,3 +214,36 @@ def test_axes_join_wherever_one_stride_serves_them():
                            (ids.view(24, 5)[:, :4].unflatten(0, (4, 6)), vectors.view(4, 30, 7)[:, :24].unflatten(1, (6, 4)))):
         with pytest.raises(ValueError, match="join"):
             _axes(tokens, values)
+
+
+def test_planes_apart():
+    """What shares no element is apart, columns of one plane too; whatever does share one is refused."""
+    from eagle_b200._sequences import _apart
+
+    plane = torch.zeros(12, 40)
+    flat = plane.view(-1)
+
+    def places(x):
+        first = (x.data_ptr() - plane.data_ptr()) // 4
+        each = x.element_size() // 4
+        return {int(first + o * each + i) for o in _offsets(x.shape, x.stride()) for i in range(each)}
+
+    views = [plane[:, :16], plane[:, 16:40], plane[:, 15:17], plane[3:5], plane[:, 3], plane[::2, 20:30], plane[1::2, 20:30],
+             flat[40:56], flat[100:101], flat[7], plane[:, :20].unflatten(1, (4, 5))[..., :3],
+             plane[:, :20].unflatten(1, (4, 5))[..., 3:], plane[:1, :8].expand(5, 8), plane[:, 30:].t(), plane[:0],
+             plane.view(torch.int64)[:, 8:12], flat.as_strided((3, 2, 4), (80, 20, 1)), flat.as_strided((3, 4), (80, 2), 41)]
+    beside = 0
+    for out in views:
+        for x in views:
+            try:
+                _apart(out, "out", x)
+            except ValueError:
+                continue
+            assert not places(out) & places(x)
+            beside += 1
+    assert beside > len(views)
+    for out, x in ((plane[:, :16], plane[:, 16:40]), (plane[:, 16:40], plane[:, :16]), (plane[:, 3], plane[:, 4:9]),
+                   (plane[:, :20].unflatten(1, (4, 5))[..., :3], plane[:, :20].unflatten(1, (4, 5))[..., 3:])):
+        _apart(out, "out", x)
+    with pytest.raises(ValueError, match="overlaps"):
+        _apart(plane[:, :16], "out", None, plane[:, 15:])
