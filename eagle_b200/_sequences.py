@@ -16,7 +16,8 @@ holds them and allocates outputs and workspace once -- and calling it only enque
 (and can be captured in a CUDA graph); the function of the same name prepares and calls.
 Calls of one prepared object share its outputs and workspace: those that may overlap on
 the GPU must be ordered by the caller, two graphs captured from it included; a graph does
-not keep the object, its owner does. No operator here records an autograd graph.
+not keep the object, its owner does. No operator here records an autograd graph or carries
+a tangent: tensors that ask for either are refused.
 """
 
 from __future__ import annotations
@@ -60,6 +61,9 @@ def _no_grad(what, *tensors):
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise ValueError(f"{what} records no autograd graph: call it under torch.no_grad() or on detached tensors "
                          "(embedding_grad is the gradient of embedding)")
+    if any(t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} carries no tangent: call it on the primal (forward_ad.unpack_dual), and embedding on "
+                         "the tangent, which it is linear in")
 
 
 def _extent(x):

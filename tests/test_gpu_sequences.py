@@ -934,3 +934,18 @@ def test_columns_of_one_plane(eb):
         assert torch.equal(left, was[:, :cut]) and torch.equal(plane[:, cut:cut + 2], was[:, cut:cut + 2])
         _check_gradient(eb, right, ids, 300, out=left)
         assert torch.equal(plane[:, cut:cut + 2], was[:, cut:cut + 2]) and torch.equal(plane[:, -1], was[:, -1])
+
+
+# ------------------------------------------------------------------------- tensors that are not what their memory holds
+
+def test_dual_tensors_are_refused(eb):
+    from torch.autograd import forward_ad
+
+    table, ids = torch.zeros(10, 16, device="cuda"), torch.zeros(4, dtype=torch.int64, device="cuda")
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(table, torch.ones_like(table))
+        with pytest.raises(ValueError, match="tangent"):
+            eb.embedding(dual, ids)
+        with pytest.raises(ValueError, match="tangent"):
+            eb.embedding_grad(dual[:4], ids, 10)
+        assert torch.equal(eb.embedding(forward_ad.unpack_dual(dual).tangent, ids), torch.ones(4, 16, device="cuda"))

@@ -247,3 +247,20 @@ def test_planes_apart():
         _apart(out, "out", x)
     with pytest.raises(ValueError, match="overlaps"):
         _apart(plane[:, :16], "out", None, plane[:, 15:])
+
+
+def test_tangents_are_refused():
+    """A dual tensor's tangent would be lost without a word."""
+    from torch.autograd import forward_ad
+
+    from eagle_b200._sequences import _no_grad
+
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.zeros(3, 4), torch.ones(3, 4))
+        for grad in (False, True):
+            with torch.set_grad_enabled(grad):
+                with pytest.raises(ValueError, match="tangent"):
+                    _no_grad("embedding", None, dual)
+                _no_grad("embedding", torch.zeros(3, 4), None)
+                _no_grad("embedding", forward_ad.unpack_dual(dual).primal)
+    _no_grad("embedding", torch.zeros(3, 4))
