@@ -53,7 +53,14 @@ def _cuda(x, what, device=None):
         raise ValueError(f"{what} must be a CUDA tensor")
     if device is not None and x.device != device:
         raise ValueError(f"{what} is on {x.device}, not on {device}")
+    _plain(x, what)
     return x
+
+
+def _plain(x, what):
+    """``x``'s memory holds its values (the imaginary part of a conjugate's holds their negatives)."""
+    if x.is_neg():
+        raise ValueError(f"{what} is a view that negates its memory: resolve it first (resolve_neg)")
 
 
 def _no_grad(what, *tensors):

@@ -949,3 +949,13 @@ def test_dual_tensors_are_refused(eb):
         with pytest.raises(ValueError, match="tangent"):
             eb.embedding_grad(dual[:4], ids, 10)
         assert torch.equal(eb.embedding(forward_ad.unpack_dual(dual).tangent, ids), torch.ones(4, 16, device="cuda"))
+
+
+def test_negated_views_are_refused(eb):
+    ids = torch.zeros(4, dtype=torch.int64, device="cuda")
+    view = torch.randn(4, 16, dtype=torch.complex64, device="cuda").conj().imag
+    with pytest.raises(ValueError, match="negates"):
+        eb.embedding_grad(view, ids, 10)
+    with pytest.raises(ValueError, match="negates"):
+        eb.embedding(view[:, :1], ids)
+    _check_gradient(eb, view.resolve_neg(), ids, 10)

@@ -264,3 +264,14 @@ def test_tangents_are_refused():
                 _no_grad("embedding", torch.zeros(3, 4), None)
                 _no_grad("embedding", forward_ad.unpack_dual(dual).primal)
     _no_grad("embedding", torch.zeros(3, 4))
+
+
+def test_negated_views_are_refused():
+    """The imaginary part of a conjugate is a float32 view of memory that holds its negatives."""
+    from eagle_b200._sequences import _plain
+
+    view = torch.randn(4, 1, dtype=torch.complex64).conj().imag
+    assert view.dtype == torch.float32 and view.is_neg()
+    with pytest.raises(ValueError, match="negates"):
+        _plain(view, "grad")
+    _plain(view.resolve_neg(), "grad")
