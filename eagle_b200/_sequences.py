@@ -63,6 +63,14 @@ def _plain(x, what):
         raise ValueError(f"{what} is a view that negates its memory: resolve it first (resolve_neg)")
 
 
+def _whole(value, what):
+    """``value`` as a whole number, one that the descs' 64 bits hold."""
+    n = int(value)
+    if n != value or not -2**63 <= n < 2**63:
+        raise ValueError(f"{what} must be a whole number of at most 64 bits, not {value}")
+    return n
+
+
 def _no_grad(what, *tensors):
     torch = _t()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
@@ -197,7 +205,7 @@ def _embedding_desc(table, values, tokens, rows, scale, first, device):
     d = _abi.new(_abi.EmbeddingDesc, device=device.index, table_type=_type(table.dtype, "the table", "element"),
                  values_type=_type(values.dtype, "the tokens' vectors", "element"),
                  token_type=_type(tokens.dtype, "tokens", "index"), table=_ptr(table), tokens=_ptr(tokens),
-                 values=_ptr(values), rows=int(rows), dim=dim, first=int(first), batch=shape[0], seq=shape[1],
+                 values=_ptr(values), rows=rows, dim=dim, first=_whole(first, "first"), batch=shape[0], seq=shape[1],
                  table_stride=max(table.stride(0), dim), scale=float(scale))
     d.token_strides[:] = token_strides
     d.value_strides[:] = [*value_strides, values.stride(-1)]
@@ -296,9 +304,10 @@ class EmbeddingGrad(_Call):
         _no_grad("embedding_grad", grad, out)
         _type(tokens.dtype, "tokens", "index")
         _type(grad.dtype, "grad", "element")
-        if int(rows) < 0:
+        rows = _whole(rows, "rows")
+        if rows < 0:
             raise ValueError("rows must not be negative")
-        shape = (int(rows), grad.shape[-1])
+        shape = (rows, grad.shape[-1])
         owned = []
         if out is None:
             if accumulate:
@@ -367,7 +376,7 @@ def _paged_desc(table, lengths, block, terminated, what):
     if terminated is not None:
         _vector(terminated, requests, (torch.bool, torch.uint8), device, "terminated")
     return _abi.new(_abi.PagedDesc, device=device.index, length_type=_type(lengths.dtype, what, "index"),
-                    requests=requests, width=width, table_stride=max(table.stride(0), width), block=int(block),
+                    requests=requests, width=width, table_stride=max(table.stride(0), width), block=_whole(block, "block"),
                     table=_ptr(table), terminated=_ptr(terminated) if terminated is not None else 0)
 
 
@@ -462,15 +471,16 @@ class SlotMap(_Call):
             d.held, d.flags = _ptr(held), _abi.SLOT_MAP_HELD
         dtype = dtype or torch.int64
         d.slot_type = _type(dtype, "dtype", "index")
-        if int(capacity) < 0:
+        capacity = _whole(capacity, "capacity")
+        if capacity < 0:
             raise ValueError("capacity must not be negative")
         self.table, self.start, self.fresh, self.held, self.terminated = table, start, fresh, held, terminated
-        d.capacity = int(capacity)
+        d.capacity = capacity
         d.start, d.fresh = _ptr(start), _ptr(fresh)
         self._work = _query("eagle_backend_x_b200_slot_map", d, device)  # refuses before anything is allocated
-        self.slots = torch.empty(int(capacity), dtype=dtype, device=device)
-        self.positions = torch.empty(int(capacity), dtype=start.dtype, device=device)
-        self.requests = torch.empty(int(capacity), dtype=torch.int32, device=device)
+        self.slots = torch.empty(capacity, dtype=dtype, device=device)
+        self.positions = torch.empty(capacity, dtype=start.dtype, device=device)
+        self.requests = torch.empty(capacity, dtype=torch.int32, device=device)
         self.offsets = torch.empty(requests + 1, dtype=torch.int32, device=device)
         d.slots, d.positions, d.token_requests, d.offsets = (_ptr(self.slots), _ptr(self.positions),
                                                              _ptr(self.requests), _ptr(self.offsets))

@@ -959,3 +959,18 @@ def test_negated_views_are_refused(eb):
     with pytest.raises(ValueError, match="negates"):
         eb.embedding(view[:, :1], ids)
     _check_gradient(eb, view.resolve_neg(), ids, 10)
+
+
+@pytest.mark.parametrize("value", (2**64 + 16, 16.5))
+def test_numbers_that_a_desc_would_cut_are_refused(eb, value):
+    dev = dict(device="cuda")
+    ids, cells = torch.zeros(4, dtype=torch.int64, **dev), torch.zeros(3, dtype=torch.int32, **dev)
+    tables = torch.zeros(3, 4, dtype=torch.int32, **dev)
+    for call in (lambda: eb.embedding(torch.zeros(10, 16, **dev), ids, first=value),
+                 lambda: eb.embedding_grad(torch.zeros(4, 16, **dev), ids, 10, first=value),
+                 lambda: eb.embedding_grad(torch.zeros(4, 16, **dev), ids, value),
+                 lambda: eb.block_tables(cells, cells, tables, cells, cells[:1], block=value),
+                 lambda: eb.slot_map(tables, cells, cells, 8, block=value),
+                 lambda: eb.slot_map(tables, cells, cells, value, block=16)):
+        with pytest.raises(ValueError, match="whole"):
+            call()

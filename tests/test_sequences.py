@@ -275,3 +275,12 @@ def test_negated_views_are_refused():
     with pytest.raises(ValueError, match="negates"):
         _plain(view, "grad")
     _plain(view.resolve_neg(), "grad")
+
+
+@pytest.mark.parametrize("value", (2**64 + 5, -2**64 + 5, 2**63, 16.5, float("inf"), float("nan")))
+def test_numbers_that_a_desc_would_cut_are_refused(value):
+    from eagle_b200._sequences import _whole
+
+    with pytest.raises((ValueError, OverflowError)):
+        _whole(value, "first")
+    assert (_whole(5, "first"), _whole(16.0, "block"), _whole(-2**63, "first")) == (5, 16, -2**63)
