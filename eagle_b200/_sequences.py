@@ -15,7 +15,8 @@ As with ``Compactor`` and ``Reducer`` a class prepares a call -- it checks the t
 holds them and allocates outputs and workspace once -- and calling it only enqueues
 (and can be captured in a CUDA graph); the function of the same name prepares and calls.
 Calls of one prepared object share its outputs and workspace: those that may overlap on
-the GPU must be ordered by the caller, two graphs captured from it included; a graph does
+the GPU must be ordered by the caller, two graphs captured from it included, and so must a
+call on another stream behind the preparation; one thread calls it at a time; a graph does
 not keep the object, its owner does. No operator here records an autograd graph or carries
 a tangent: tensors that ask for either are refused.
 """
@@ -136,13 +137,14 @@ def _capturing(handle):
 class _Call:
     """A prepared call: ``_desc`` and the C entry, enqueued on the tensors' device."""
 
-    def _prepare(self, entry, desc, device, owned):
+    def _prepare(self, entry, desc, device, *tensors):
         self.device = device
         self._entry = getattr(_abi.lib(), entry)
         self._desc = desc
         self._ref = ctypes.byref(desc)
-        self._owned = owned  # allocated here, on this stream
+        self._tensors = [t for t in tensors if t is not None]  # what a call reads and writes
         self._home = _raw_stream(device)
+        self._known = set()  # streams that the allocator knows to use them
 
     def _enqueue(self, stream):
         if stream is None:
@@ -151,12 +153,14 @@ class _Call:
             if stream.device != self.device:
                 raise ValueError(f"the stream is on {stream.device}, the tensors on {self.device}")
             handle = stream.cuda_stream
-        if handle != self._home and not _capturing(handle):
-            # the allocator may hand these out again once they are dropped: not before this stream is past the
-            # call (a capture runs nothing: what its graph uses, the graph's owner keeps)
+        if (stream is not None or handle != self._home) and handle not in self._known and not _capturing(handle):
+            # the allocator may hand the tensors' memory out again once they are dropped, the caller's too: not
+            # before this stream is past the call (a capture runs nothing: what its graph uses, the graph's owner
+            # keeps). Once a stream is enough: it is asked for how far it is when they are dropped
             s = stream if stream is not None else _t().cuda.current_stream(self.device)
-            for t in self._owned:
+            for t in self._tensors:
                 t.record_stream(s)
+            self._known.add(handle)
         self._desc.stream = handle
         status = self._entry(self._ref)
         if status:
@@ -256,14 +260,12 @@ class Embedding(_Call):
         _type(dtype or table.dtype, "the table and dtype", "element")
         if out is None:
             out = torch.empty(shape, dtype=dtype or table.dtype, device=device)
-            owned = [out]
         else:
             _check_out(out, shape, dtype, device, "out")
             _apart(out, "out", table, tokens)
-            owned = []
         self.table, self.tokens, self.out = table, tokens, out
         d = _embedding_desc(table, out, tokens, table.shape[0], scale, first, device)
-        self._prepare("eagle_backend_x_b200_embedding", d, device, owned)
+        self._prepare("eagle_backend_x_b200_embedding", d, device, table, tokens, out)
 
     def __call__(self, stream=None):
         self._enqueue(stream)
@@ -308,13 +310,11 @@ class EmbeddingGrad(_Call):
         if rows < 0:
             raise ValueError("rows must not be negative")
         shape = (rows, grad.shape[-1])
-        owned = []
         if out is None:
             if accumulate:
                 raise ValueError("accumulate adds to out: give it")
             _type(dtype or grad.dtype, "dtype", "element")
             out = torch.empty(shape, dtype=dtype or grad.dtype, device=device)
-            owned.append(out)
         else:
             _check_out(out, shape, dtype, device, "out")
             _apart(out, "out", grad, tokens)
@@ -322,8 +322,7 @@ class EmbeddingGrad(_Call):
         d = _embedding_desc(out, grad, tokens, rows, scale, first, device)
         d.flags = _abi.EMBEDDING_ACCUMULATE if accumulate else 0
         self._work = _query("eagle_backend_x_b200_embedding_grad", d, device)
-        owned.append(self._work)
-        self._prepare("eagle_backend_x_b200_embedding_grad", d, device, owned)
+        self._prepare("eagle_backend_x_b200_embedding_grad", d, device, grad, tokens, out, self._work)
 
     def __call__(self, stream=None):
         self._enqueue(stream)
@@ -429,7 +428,8 @@ class BlockTables(_Call):
             d.used, d.used_size = _ptr(used), used.numel()
         d.blocks, d.cells = _ptr(self.blocks), _ptr(self.cells)
         self._work = _query("eagle_backend_x_b200_block_tables", d, device)
-        self._prepare("eagle_backend_x_b200_block_tables", d, device, [self.blocks, self.cells, self._work])
+        self._prepare("eagle_backend_x_b200_block_tables", d, device, lengths, held, table, pool, count, used,
+                      terminated, self.blocks, self.cells, self._work)
 
     def __call__(self, stream=None):
         self._enqueue(stream)
@@ -484,8 +484,8 @@ class SlotMap(_Call):
         self.offsets = torch.empty(requests + 1, dtype=torch.int32, device=device)
         d.slots, d.positions, d.token_requests, d.offsets = (_ptr(self.slots), _ptr(self.positions),
                                                              _ptr(self.requests), _ptr(self.offsets))
-        self._prepare("eagle_backend_x_b200_slot_map", d, device,
-                      [self.slots, self.positions, self.requests, self.offsets, self._work])
+        self._prepare("eagle_backend_x_b200_slot_map", d, device, table, start, fresh, held, terminated, self.slots,
+                      self.positions, self.requests, self.offsets, self._work)
 
     def __call__(self, stream=None):
         self._enqueue(stream)

@@ -974,3 +974,46 @@ def test_numbers_that_a_desc_would_cut_are_refused(eb, value):
                  lambda: eb.slot_map(tables, cells, cells, value, block=16)):
         with pytest.raises(ValueError, match="whole"):
             call()
+
+
+# ------------------------------------------------------------------------- memory that another stream still reads
+
+@pytest.mark.parametrize("form", ("function", "object"))
+def test_inputs_stay_until_the_stream_is_past_them(eb, form):
+    """Tensors dropped right after a call on another stream: their memory is not given to others while that stream,
+    kept busy here, has yet to read it."""
+    n, rows, dim = 5000, 300, 64
+    rng = _gen(26)
+    table, grad = _values(rng, (rows, dim), torch.float32), _values(rng, (n, dim), torch.float32)
+    ids = torch.from_numpy(rng.integers(0, rows, n))
+    lengths = torch.from_numpy(rng.integers(0, 60, n)).int()
+    plane, pool = torch.zeros(n, 4, dtype=torch.int32), torch.arange(n * 4, dtype=torch.int32)
+    none, count = torch.zeros(n, dtype=torch.int32), torch.tensor([n * 4], dtype=torch.int32)
+    cases = [("embedding", eb.Embedding, (table, ids), (), {}),
+             ("embedding_grad", eb.EmbeddingGrad, (grad, ids), (rows,), {}),
+             ("block_tables", eb.BlockTables, (lengths, none, plane, pool, count), (), dict(block=16)),
+             ("slot_map", eb.SlotMap, (plane, none, lengths), (n * 60,), dict(block=16))]
+    side = torch.cuda.Stream()
+    busy = torch.randn(4096, 4096, device="cuda")
+    for name, kind, inputs, rest, keys in cases:
+        def first(out):
+            return out[0] if isinstance(out, tuple) else out
+
+        want = first(getattr(eb, name)(*(x.cuda() for x in inputs), *rest, **keys)).clone()
+        mine = [x.cuda() for x in inputs]
+        places = {x.data_ptr() for x in mine}
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                busy @ busy
+        if form == "function":
+            got = first(getattr(eb, name)(*mine, *rest, **keys, stream=side))
+        else:
+            got = first(kind(*mine, *rest, **keys)(side))
+        sizes = [(x.numel(), x.dtype) for x in mine]
+        mine.clear()
+        again = [torch.empty(size, dtype=dtype, device="cuda") for size, dtype in sizes * 3]
+        assert not side.query()
+        assert not places & {x.data_ptr() for x in again}, name
+        side.synchronize()
+        assert torch.equal(got, want), name
