@@ -1017,3 +1017,79 @@ def test_inputs_stay_until_the_stream_is_past_them(eb, form):
         assert not places & {x.data_ptr() for x in again}, name
         side.synchronize()
         assert torch.equal(got, want), name
+
+
+# ------------------------------------------------------------------------- the order of the sums
+
+def _in_order(grad, ids, rows):
+    """The sums of float32 rows as documented, in float32: the tokens sorted by id, equal ones in token order, the
+    sorted order cut into chunks of 8 to 64 by the sizes; a run in which two chunks or more begin is added up chunk by
+    chunk, any other at once; of up to 32 parts one after the other, of more in equal shares whose sums are added."""
+    n, dim = grad.shape
+    chunk = 8
+    while chunk < 64 and n * ((dim + 7) // 8) // 32 // (2 * chunk) >= (4096 if dim >= 512 else 2048):
+        chunk *= 2
+    lanes = 4
+    while lanes < 32 and lanes * 4 < dim:
+        lanes *= 2
+
+    def added(rows_):
+        return np.cumsum(rows_, axis=0, dtype=np.float32)[-1]
+
+    want = np.zeros((rows, dim), np.float32)
+    order = np.argsort(ids, kind="stable")
+    order = order[(ids[order] >= 0) & (ids[order] < rows)]
+    keys = ids[order]
+    starts = np.flatnonzero(np.r_[True, keys[1:] != keys[:-1]]) if keys.size else []
+    for b, e in zip(starts, np.r_[starts[1:], keys.size]):
+        x = grad[order[b:e]]
+        cuts = np.arange(-(-b // chunk) * chunk, e, chunk)
+        if len(cuts) < 2:
+            want[keys[b]] = added(x)
+            continue
+        parts = np.array([added(p) for p in np.split(x, cuts[cuts > b] - b)])
+        if len(parts) > 32:
+            each = -(-len(parts) // (256 // lanes))
+            parts = np.array([added(parts[i:i + each]) for i in range(0, len(parts), each)])
+        want[keys[b]] = added(parts)
+    return want
+
+
+@pytest.mark.parametrize("kind", ("uniform", "skewed", "one"))
+@pytest.mark.parametrize("n,rows,dim", [(900, 300, 8), (3000, 50, 520), (3000, 700, 513), (8000, 1500, 33), (8000, 300, 264),
+                                        (60000, 4000, 24), (100000, 9000, 8), (100000, 300, 72), (140000, 2000, 8),
+                                        (140000, 70000, 40), (600000, 5000, 4)])
+def test_gradient_order(eb, n, rows, dim, kind):
+    """The bits of each row, in every form of the sort and of the sums: equal ids in token order, chunk by chunk."""
+    rng = _gen(27, n, dim)
+    ids = _ids(rng, kind, n, rows)
+    grad = rng.standard_normal((n, dim)).astype(np.float32)
+    want = _in_order(grad, ids, rows)
+    if kind == "one" or n > 4 * rows:  # another order of equal ids, or other cuts, would show
+        back = _in_order(grad[::-1].copy(), ids[::-1].copy(), rows)
+        assert not np.array_equal(back, want)
+    dev, dev_ids = torch.from_numpy(grad).cuda(), torch.from_numpy(ids).cuda()
+    got = eb.embedding_grad(dev, dev_ids, rows)
+    assert np.array_equal(got.cpu().numpy(), want)
+    # in another memory order, and added to what is there
+    strided = torch.empty(dim, n, device="cuda").t()
+    strided.copy_(dev)
+    out = torch.from_numpy(rng.standard_normal((rows, dim)).astype(np.float32)).cuda()
+    before = out.cpu().numpy().copy()
+    eb.embedding_grad(strided, dev_ids.int(), rows, out=out, accumulate=True)
+    named = np.bincount(ids[ids >= 0], minlength=rows)[:, None] > 0
+    assert np.array_equal(out.cpu().numpy(), np.where(named, before + want, before))
+
+
+@pytest.mark.parametrize("n", (100, 50000, 140000))
+def test_gradient_of_many_rows(eb, n):
+    """A table of more than 2^27 rows, whose ids take four passes; whole numbers, so that the sums are exact."""
+    rows, dim = 2**27 + 5, 2
+    rng = _gen(28, n)
+    ids = torch.from_numpy(np.r_[rng.integers(0, rows, n - 50), np.full(25, rows - 1), np.arange(25)]).cuda()
+    grad = torch.from_numpy(rng.integers(1, 9, (n, dim)).astype(np.float32)).half().cuda()
+    got = eb.embedding_grad(grad, ids, rows)
+    named, place = torch.unique(ids, return_inverse=True)
+    want = torch.zeros(named.numel(), dim, device="cuda").index_add_(0, place, grad.float())
+    assert torch.equal(got[named].float(), want)
+    assert int(got.count_nonzero()) == named.numel() * dim
