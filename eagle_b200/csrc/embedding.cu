@@ -259,9 +259,9 @@ void launchLookup(LookupArgs a, cudaStream_t s, const char* who)
         else if (Shifted)
             launchBehind(lookupShiftedKernel<In, Out, Tok, N, 4>, blocks, kLookupThreads, 0, s, a, who);
         else if (unroll == 1)
-            lookupKernel<In, Out, Tok, N, 1><<<blocks, kLookupThreads, 0, s>>>(a);
+            launchBehind(lookupKernel<In, Out, Tok, N, 1>, blocks, kLookupThreads, 0, s, a, who);
         else
-            lookupKernel<In, Out, Tok, N, 4><<<blocks, kLookupThreads, 0, s>>>(a);
+            launchBehind(lookupKernel<In, Out, Tok, N, 4>, blocks, kLookupThreads, 0, s, a, who);
     }
     launchCheck(who);
 }

@@ -128,11 +128,13 @@ __device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
 
 // ------------------------------------------------------------- kernels in a row
 //
-// A call of several kernels launches each but the first while the one before it still runs
-// (programmatic dependent launch), so that its CTAs are in place when their turn comes. Such
-// a kernel touches no memory before ``waitForKernelBefore``, which returns once every kernel
-// before it has ended and its writes are visible; the one before lets it start with
-// ``letNextKernelStart``, early, which takes effect when all of its CTAs are running.
+// Kernels are launched while whatever runs before them, another of the call's or anything else on
+// the stream, may still be running (programmatic dependent launch), so that their CTAs are in
+// place when their turn comes. Such a kernel touches no memory before ``waitForKernelBefore``,
+// which returns once every kernel before it has ended and its writes are visible; one of these
+// lets the next start with ``letNextKernelStart``, early, which takes effect when all of its
+// CTAs are running. Launched in plain order, and so without the wait: histogramKernel, behind a
+// memset, and zeroRowsKernel.
 
 // Since what such a kernel reads may be written while it waits, none of it is read through the
 // non-coherent path (__ldg): plain loads, or past L1 (__ldcg).
@@ -140,7 +142,7 @@ __device__ __forceinline__ uint4 loadShifted(const void* p, uint32_t valid)
 __device__ __forceinline__ void waitForKernelBefore() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void letNextKernelStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-/** Launch ``kernel(args)``, which starts with waitForKernelBefore, behind another of the call's. */
+/** Launch ``kernel(args)``, which starts with waitForKernelBefore, behind whatever the stream has before it. */
 template <class Args>
 void launchBehind(void (*kernel)(Args), unsigned blocks, unsigned threads, size_t shared, cudaStream_t s,
     const Args& args, const char* who)
