@@ -14,9 +14,9 @@
 //
 // The sort is least-significant-digit radix over bits(rows) bits, at most 9 a pass: up to 131072
 // tokens in one launch, by a CTA or a cluster that keeps the keys in shared memory; past that
-// a kernel a pass, each adding up the tiles' digit counts itself (no wait on another CTA): the
-// first counts come from a kernel of their own, each later pass's are gathered by the pass
-// before, which knows where its keys land.
+// a kernel a pass, whose tiles add up one another's digit counts themselves (no wait on another
+// CTA), from 129 tiles on after a kernel that scans them: the first counts come from a kernel of
+// their own, each later pass's are gathered by the pass before, which knows where its keys land.
 #include "sequences.cuh"
 
 #include <cooperative_groups.h>
@@ -218,7 +218,10 @@ constexpr int kClusterItems = 16;
 constexpr uint32_t kClusterKeys = uint32_t(kClusterThreads) * kClusterSize * kClusterItems;  // 131072
 constexpr uint32_t kPortableKeys = kClusterKeys / 2;
 constexpr uint32_t kFewKeys = 8192;    // from here on 16 CTAs, where the device has such clusters, beat 8
-constexpr uint32_t kAloneKeys = 4096;  // sorted by one CTA as fast as by eight, which exchange them
+// Up to here one CTA sorts: by eight, which exchange the keys, the gradient of 2500 to 4096 tokens
+// takes 16.7 to 17.5 us instead of 18.2 to 19.5 where rows are narrow (64 bytes), and 25.1 instead of
+// 24.6 where they are wide (2 KB), since fewer SMs are left to zero meanwhile.
+constexpr uint32_t kAloneKeys = 4096;
 static_assert(kClusterThreads >= int(kMaxBins), "a thread per bin");
 
 /** Shared memory of the sort: the keys by place twice, the ranks' words and counts. */
@@ -1244,10 +1247,10 @@ void launchPass(const GradArgs& a, unsigned tiles, cudaStream_t s, const char* w
  *  about the sort's time (7 us with one key a thread, 14 with four, 30 with sixteen). */
 constexpr int64_t zeroedBesideSort(unsigned perThread) { return (18ll + 6ll * perThread) << 20; }
 
-/** And those that are left to the SMs without a join, whose 10 us of dependent reads they cover (131072
- *  tokens of 8 KB: 370 us with 32 MB, 365 with 144, 377 with all that is left). */
+/** And those that are left to the SMs without a join, whose 10 us of dependent reads they cover, ahead of
+ *  what the sums' kernel zeroes (32 MB instead of 128: 94 us instead of 90 for 4096 tokens into 65536 rows of
+ *  8 KB, 112 instead of 108 for 16384, 365 instead of 359 for 131072 into as many; all that is left: 377). */
 constexpr int64_t kZeroedBesideJoin = 128ll << 20;
-constexpr int64_t kZeroedBesideSums = 24ll << 20;  // but the sums, of 5 us at least, have some first
 
 /** ``asked``: see GradArgs; anything below kEvery withholds rows, which the waits for them then miss. */
 void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const char* who, uint32_t polls = kBulkWaits,
@@ -1387,7 +1390,7 @@ void enqueueGrad(const eagle_b200_embedding_desc& d, const GradPlan& p, const ch
     a.zeroedBefore = d.rows;
     if (a.present != nullptr && p.chunks > 1) {
         const int64_t left = (d.rows - a.zeroed) * a.rowBytes;
-        a.zeroedBefore -= std::min(kZeroedBesideJoin, std::max(left / 2, left - kZeroedBesideSums)) / a.rowBytes;
+        a.zeroedBefore -= std::min(kZeroedBesideJoin, left) / a.rowBytes;
     }
     const int64_t zeroing = a.present == nullptr ? 0 : unitsOf(a.zeroedBefore - a.zeroed);
     const unsigned blocks = gridOf(int64_t(a.sumBlocks) + zeroing, who);
