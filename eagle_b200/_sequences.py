@@ -286,7 +286,9 @@ class EmbeddingGrad(_Call):
     ``grad`` is ``(*tokens.shape, dim)``, float32, bfloat16 or float16, with any strides, a
     broadcast's zeros included (of more than two leading axes: that join into two where the
     tokens' do). ``out`` is (rows, dim), contiguous rows, of ``dtype`` (by
-    default ``grad``'s). With ``accumulate`` the sums are added to ``out`` (required then):
+    default ``grad``'s). Padding is left out where it is marked by an id that the table has no
+    row for (-1); an id of one of its rows is summed, whatever it stands for. With
+    ``accumulate`` the sums are added to ``out`` (required then):
     rows without a token stay as they are. Each row is summed in 32 bits in one order that
     the sizes alone fix and rounded once, so the bits do not depend on the launch. The
     workspace is about 16 bytes a token and a 32-bit row per 4 to 32 tokens.
