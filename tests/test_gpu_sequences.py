@@ -1093,3 +1093,64 @@ def test_gradient_of_many_rows(eb, n):
     want = torch.zeros(named.numel(), dim, device="cuda").index_add_(0, place, grad.float())
     assert torch.equal(got[named].float(), want)
     assert int(got.count_nonzero()) == named.numel() * dim
+
+
+# ------------------------------------------------------------------------- the largest sizes
+
+def test_a_million_requests(eb):
+    """As many requests as are taken: 2^20, a third of them ended, in closed form."""
+    requests, block, width = 2**20, 8, 3
+    r = torch.arange(requests, device="cuda")
+    ended = r % 3 == 1
+    held = torch.where(r % 2 == 0, 1, 0).int()
+    tables = torch.where(torch.arange(width, device="cuda") < held[:, None], r[:, None], -1).int()
+    need = (r % 3 == 0).long() * 2 + (r % 3 == 2).long() * (r % 4)  # three blocks at most, four where the row is too narrow
+    need = torch.where(r % 300 == 2, width + 1, need)
+    lengths = torch.where(need > 0, need * block - r % block, 0).int()
+    fresh = torch.where(ended | (need > width), 0, (need - held).clamp(min=0))
+    upto = torch.cumsum(fresh, 0)
+    available = int(upto[-1]) - 7
+    pool = (torch.randperm(2 * requests, device="cuda") + requests).int()
+    used = torch.zeros(3 * requests, dtype=torch.uint8, device="cuda")
+    used[r[held > 0]] = 1
+    fits = ended | (need <= held) | ((need <= width) & (upto <= available))
+    want = tables.clone()
+    now = fits & (fresh > 0)
+    for j in range(width):
+        row = now & (j < fresh)
+        want[row, (held[row] + j).long()] = pool[(upto - fresh + j)[row]]
+    want_used = used.clone()
+    want_used[r[ended & (held > 0)]] = 0
+    want_used[pool[:int(upto[now].max())].long()] = 1
+    count = torch.tensor([available], dtype=torch.int32, device="cuda")
+    blocks, cells = eb.block_tables(lengths, held, tables, pool, count, block=block, used=used, terminated=ended)
+    assert torch.equal(tables, want) and torch.equal(used, want_used)
+    assert torch.equal(blocks.long(), torch.where(ended, 0, torch.where(fits, torch.maximum(need, held), held)))
+    assert cells.tolist() == [int(upto[now].max()), int((~fits).sum())] and cells[1] > 0
+
+    new = torch.where(ended, 0, r % 5)
+    total, capacity = int(new.sum()), int(new.sum()) + 9
+    got = eb.slot_map(tables, blocks, (r % 5).int(), capacity, block=block, held=blocks, terminated=ended)
+    owner = torch.repeat_interleave(r, new)
+    offsets = torch.cat((new.new_zeros(1), torch.cumsum(new, 0)))
+    position = blocks[owner] + torch.arange(total, device="cuda") - offsets[owner]
+    column = position // block
+    entry = torch.where(column < blocks[owner], tables[owner, column.clamp(max=width - 1)].long(), -1)
+    assert torch.equal(got[0][:total], torch.where(entry < 0, -1, entry * block + position % block))
+    assert torch.equal(got[1][:total].long(), position) and torch.equal(got[2][:total].long(), owner)
+    assert got[0][total:].eq(-1).all() and got[1][total:].eq(0).all() and got[2][total:].eq(-1).all()
+    assert torch.equal(got[3].long(), offsets)
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float32))
+def test_the_widest_rows(eb, dtype):
+    """2^24 values a row, and one less, which lies on no words; whole numbers, so that every sum is exact."""
+    for dim in (2**24, 2**24 - 1):
+        table = torch.randint(-4, 5, (2, dim), device="cuda").to(dtype)
+        ids = torch.tensor([1, -1, 0], device="cuda")
+        got = eb.embedding(table, ids, scale=2.0)
+        assert torch.equal(got[0], 2 * table[1]) and torch.equal(got[2], 2 * table[0]) and not got[1].any()
+        ids = torch.tensor([0] * 3 + [1] * 30 + [2] * 2 + [0] * 165, device="cuda")
+        got = eb.embedding_grad(table[1].expand(200, dim), ids, 3, dtype=torch.float32)
+        for row, n in enumerate((168, 30, 2)):
+            assert torch.equal(got[row], n * table[1].float())
