@@ -1154,3 +1154,31 @@ def test_the_widest_rows(eb, dtype):
         got = eb.embedding_grad(table[1].expand(200, dim), ids, 3, dtype=torch.float32)
         for row, n in enumerate((168, 30, 2)):
             assert torch.equal(got[row], n * table[1].float())
+
+
+def test_gradient_wait_gives_up_past_one_cluster(eb):
+    """The same where the sort takes several kernels and the call zeroes its workspace by a memset: chunks of 64."""
+    import ctypes
+
+    from eagle_b200 import _abi
+
+    n, dim = 140001, 512
+    ids = torch.arange(n, device="cuda") // 3
+    rows = int(ids[-1]) + 1
+    grad = torch.ones(n, dim, dtype=torch.bfloat16, device="cuda")
+    call = eb.EmbeddingGrad(grad, ids, rows)
+    d = _abi.new(_abi.EmbeddingDesc)
+    ctypes.memmove(ctypes.byref(d), ctypes.byref(call._desc), ctypes.sizeof(d))
+    d.stream = torch.cuda.current_stream().cuda_stream
+    _abi.check(_abi.lib().eagle_backend_x_b200_embedding_grad_wait_check(ctypes.byref(d), 1024, 1))
+    torch.cuda.synchronize()
+    lost = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    lost[1:22] = True  # positions 4 to 65: the run that starts at 63 is summed where it starts
+    assert torch.equal(call.out.isnan().all(1), lost) and bool((call.out[~lost] == 3.0).all())
+    with pytest.raises(eb.BackendError, match="wait"):
+        call.check()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    call(side)
+    call.check(side)
+    assert bool((call.out == 3.0).all())
